@@ -451,6 +451,95 @@ int mdd_jsonl_scan(mdd_ctx* ctx, const uint8_t* raw, uint64_t raw_bytes, const u
 int mdd_jsonl_decode(mdd_ctx* ctx, const uint8_t* raw, uint64_t raw_bytes, uint64_t n_lines, const uint8_t* status,
                      const uint64_t* content_pos, const uint64_t* out_offsets, uint8_t* out_text, uint64_t out_capacity);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Document vectors (an EXTENSION: the reference compares documents by their shingles only).  A document is a row of `dim`
+ * numbers; documents whose rows point the same way are near duplicates even where they share no shingle.  Conventions of
+ * this section: matrices are row-major with unit stride inside a row, *_stride is the distance of two rows in elements
+ * (>= dim), outputs without a stride parameter are dense; element types are MDD_F32 / MDD_BF16 / MDD_F16; sums are held in
+ * 32 bits and every output is rounded once.  Workspaces are the caller's, 256-byte aligned, of at least the size that the
+ * *_ws_bytes function (host arithmetic, needs no GPU) gives for the same sizes; two calls that may run at the same time --
+ * two captured graphs that are replayed side by side, say -- need a workspace each.  Nothing here allocates, synchronises
+ * or clears memory with a memset, so every call may be captured into a HIP graph.  The caller's current device is kept. */
+#define MDD_F32 0
+#define MDD_BF16 1
+#define MDD_F16 2
+#define MDD_I8 3   /* signed 8-bit integers, -127 .. 127 */
+#define MDD_E4M3 4 /* OCP e4m3: 3 bits behind the leading one, largest 448, no infinities */
+#define MDD_VEC_MAX_DIM 32768
+
+/* Embedding lookup.  ids (id_bytes 4: int32, 8: int64) name rows of table [n_rows, dim]; an id outside [0, n_rows) is
+ * padding and contributes nothing.
+ *   offsets NULL    out[p] = scale * table[ids[p]]             (n_ids rows; padding: a row of zeros)
+ *   offsets given   document d = ids [offsets[d], offsets[d+1]) as for the packed text (n_docs + 1 ascending entries,
+ *                   clamped to n_ids): out[d] = f * sum of its rows, f = scale, or with mean != 0 scale / (its ids that
+ *                   name a row).  A document without such an id gives zeros.
+ * The order of every sum depends on the sizes alone, so results repeat bit for bit.  n_ids < 2^31. */
+uint64_t mdd_embed_ws_bytes(uint64_t n_ids, uint32_t dim);
+int mdd_embed(mdd_ctx* ctx, const void* table, int type, uint64_t n_rows, uint64_t row_stride, uint32_t dim, const void* ids,
+              int id_bytes, uint64_t n_ids, const uint64_t* offsets, uint64_t n_docs, int mean, float scale, void* out,
+              void* ws, uint64_t ws_bytes);
+/* Its gradient with respect to the table: table_grad [n_rows, dim] (out_type: MDD_F32 or `type`) is overwritten,
+ *   table_grad[v] = sum over the positions p with ids[p] == v of f(p) * grad[row(p)],  row(p) = p or p's document.
+ * The positions are sorted by id (stable), so each row is summed in the order of the positions: no floating atomics.
+ * n_rows < 2^31, n_docs < 2^31. */
+uint64_t mdd_embed_backward_ws_bytes(uint64_t n_ids, uint64_t n_docs, uint64_t n_rows, uint32_t dim);
+int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_stride, uint32_t dim, const void* ids, int id_bytes,
+                       uint64_t n_ids, const uint64_t* offsets, uint64_t n_docs, int mean, float scale, void* table_grad,
+                       int out_type, uint64_t n_rows, void* ws, uint64_t ws_bytes);
+
+/* Root-mean-square norm.  h = x + residual (residual may be NULL: h = x), r = 1 / sqrt(mean(h^2) + eps), weight [dim] of
+ * x's type (NULL: ones).  dim <= MDD_VEC_MAX_DIM.
+ *   norm      y = h * r * weight;  sum_out (may be NULL) = h, rounded to the type;  rstd (may be NULL) = r, float per row
+ *   norm_q8   the same with y in 8 bits (kind MDD_I8 or MDD_E4M3): with top = 127 or 448 and big = the row's largest
+ *             |h * weight|, code = the nearest 8-bit value to h * weight * top / big, ties to even, decided as in exact
+ *             arithmetic, and scale[row] = big * r / top, so that code * scale is y.  A row of zeros gets zeros with scale 0;
+ *             a row with a NaN or an infinity gets zeros with scale NaN.
+ *   backward  h as stored by norm (sum_out, or x), rstd as stored, g = gradient of y, grad_sum (may be NULL) = gradient
+ *             that reaches sum_out by other ways:  x_grad = r * (g*w - h*r * mean(g*w*h*r)) + grad_sum -- the gradient of x
+ *             and of residual alike;  weight_grad (float [dim], may be NULL) = sum over rows of g * h * r. */
+int mdd_rms_norm(mdd_ctx* ctx, const void* x, int type, uint64_t x_stride, const void* residual, uint64_t residual_stride,
+                 const void* weight, float eps, uint64_t n_rows, uint32_t dim, void* y, void* sum_out, float* rstd);
+int mdd_rms_norm_q8(mdd_ctx* ctx, const void* x, int type, uint64_t x_stride, const void* residual, uint64_t residual_stride,
+                    const void* weight, float eps, uint64_t n_rows, uint32_t dim, int kind, void* codes, float* scales,
+                    void* sum_out);
+uint64_t mdd_rms_norm_backward_ws_bytes(uint64_t n_rows, uint32_t dim);
+int mdd_rms_norm_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_stride, const void* h, uint64_t h_stride,
+                          const void* grad_sum, uint64_t grad_sum_stride, const void* weight, const float* rstd,
+                          uint64_t n_rows, uint32_t dim, void* x_grad, float* weight_grad, void* ws, uint64_t ws_bytes);
+
+/* Cosines of candidate edges from 8-bit rows: cosines[e] = a.b / sqrt(a.a * b.b) of the rows edge_u[e] and edge_v[e] of codes
+ * [n_rows, dim] (kind MDD_I8: sums exact in 32-bit integers; MDD_E4M3: sums in float).  A per-row scale cancels, so none is
+ * taken.  A row of zeros, and an edge naming a row >= n_rows, gives 0 (as mdd_signature_matches).  dim <= MDD_VEC_MAX_DIM. */
+int mdd_edge_cosines(mdd_ctx* ctx, const void* codes, int kind, uint64_t row_stride, uint64_t n_rows, uint32_t dim,
+                     const uint32_t* edge_u, const uint32_t* edge_v, uint64_t n_edges, float* cosines);
+/* Orders an edge list by (edge_u, edge_v), in place.  Entries < n_docs <= 2^32 - 1; n_edges < 2^31. */
+uint64_t mdd_sort_edges_ws_bytes(uint64_t n_edges);
+int mdd_sort_edges(mdd_ctx* ctx, uint32_t* edge_u, uint32_t* edge_v, uint64_t n_edges, uint64_t n_docs, void* ws, uint64_t ws_bytes);
+
+/* Microscaled 4-bit matrices.  Each 32 columns of a row share one power of two (e8m0: byte s stands for 2^(s - 127)); an
+ * element is e2m1: 0 .5 1 1.5 2 3 4 6 with a sign.  quantize takes 2^(floor(log2(largest |x|)) - 2) as the block's scale, rounds
+ * x / scale to the nearest element (ties to the even code) and holds values beyond 6 at 6; a block of zeros has scale 2^-127; a
+ * block with a NaN or an infinity has scale byte 255, and every product with it is NaN.
+ * Packed layout, in the order in which the matrix instruction reads it -- tiles of 32 rows x 128 columns, row tiles outermost:
+ *   codes  MDD_MX_CODE_BYTES(rows, dim): [row tile][column tile][block of 32 columns: 4][row: 32][16 bytes, low nibble first]
+ *   scales MDD_MX_SCALE_BYTES(rows, dim): [row tile][column tile][block & 1][row: 32][block >> 1]
+ * Rows and columns that only fill up a tile hold code 0 and scale byte 127.  Both buffers 16-byte aligned.
+ *   matmul   c [m, n] (MDD_F32 or MDD_BF16, c_stride) = alpha * A * B^T,  A [m, dim], B [n, dim] packed
+ *   pairs    every u > v with cos(A_u, A_v) >= min_cosine (0 < min_cosine <= 1; cosine of the 4-bit values), appended to edge_u /
+ *            edge_v in no fixed order, at most edge_cap of them; *n_edges (device u64, set by the call) counts all of them.
+ *            Rows of zeros and rows with a NaN have no pairs.  m < 2^31. */
+#define MDD_MX_TILE_ROWS 32
+#define MDD_MX_TILE_COLS 128
+#define MDD_MX_CODE_BYTES(rows, dim) ((((uint64_t)(rows) + 31) / 32) * (((uint64_t)(dim) + 127) / 128) * 2048)
+#define MDD_MX_SCALE_BYTES(rows, dim) ((((uint64_t)(rows) + 31) / 32) * (((uint64_t)(dim) + 127) / 128) * 128)
+int mdd_mx_quantize(mdd_ctx* ctx, const void* x, int type, uint64_t x_stride, uint64_t n_rows, uint32_t dim, uint8_t* codes,
+                    uint8_t* scales);
+int mdd_mx_matmul(mdd_ctx* ctx, const uint8_t* a_codes, const uint8_t* a_scales, uint64_t m, const uint8_t* b_codes,
+                  const uint8_t* b_scales, uint64_t n, uint32_t dim, float alpha, void* c, int c_type, uint64_t c_stride);
+uint64_t mdd_mx_pairs_ws_bytes(uint64_t m);
+int mdd_mx_pairs(mdd_ctx* ctx, const uint8_t* codes, const uint8_t* scales, uint64_t m, uint32_t dim, float min_cosine,
+                 uint32_t* edge_u, uint32_t* edge_v, uint64_t edge_cap, uint64_t* n_edges, void* ws, uint64_t ws_bytes);
+
 /* Measurement helper: runs `iters` iterations of a dependency-free
  * v_xor/v_add/v_lshr mix on every CU and reports the measured int32 VALU lane-op rate in
  * *tops_host (HOST double, 1e12 lane-ops/s).  Synchronous. */

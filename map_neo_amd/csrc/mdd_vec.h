@@ -1,0 +1,110 @@
+// Shared by the document-vector kernels (mdd_vec.hip, mdd_mx.hip): element types, eight-element loads and stores, wave sums.
+#ifndef MDD_VEC_H
+#define MDD_VEC_H
+
+#include "mdd_common.h"
+
+namespace mddi {
+
+// Restores the caller's current device: the entry points below switch to the context's GPU and must leave no trace of it.
+struct DeviceGuard {
+    int prev = -1;
+    hipError_t err;
+    explicit DeviceGuard(int dev) {
+        err = hipGetDevice(&prev);
+        if (err == hipSuccess && prev != dev) err = hipSetDevice(dev);
+        else prev = -1;
+    }
+    ~DeviceGuard() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+#define ON_DEVICE(ctx)                     \
+    mddi::DeviceGuard guard_((ctx)->device); \
+    if (guard_.err != hipSuccess) return mddi::fail(MDD_ERR_HIP, "selecting device %d failed: %s", (ctx)->device, hipGetErrorString(guard_.err))
+
+inline bool aligned_to(const void* p, uint64_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+inline uint64_t round_up(uint64_t x, uint64_t m) { return (x + m - 1) / m * m; }
+inline uint32_t type_bytes(int t) { return t == MDD_F32 ? 4u : (t == MDD_BF16 || t == MDD_F16) ? 2u : 0u; }
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Rows start where the caller's stride puts them, so an eight-element access may begin at any element: gfx950 serves
+// 16-byte accesses at any byte address (unaligned access mode), and only a row's last 1..7 elements go one by one.
+template <typename T>
+struct vec8;
+template <>
+struct vec8<float> {
+    typedef float raw __attribute__((ext_vector_type(8)));
+    typedef float raw_any __attribute__((ext_vector_type(8), aligned(4)));
+};
+template <>
+struct vec8<__bf16> {
+    typedef __bf16 raw __attribute__((ext_vector_type(8)));
+    typedef __bf16 raw_any __attribute__((ext_vector_type(8), aligned(2)));
+};
+template <>
+struct vec8<_Float16> {
+    typedef _Float16 raw __attribute__((ext_vector_type(8)));
+    typedef _Float16 raw_any __attribute__((ext_vector_type(8), aligned(2)));
+};
+
+template <typename T>
+__device__ __forceinline__ typename vec8<T>::raw load8_raw(const T* __restrict__ p, uint32_t n) {
+    typename vec8<T>::raw v;
+    if (n >= 8) {
+        v = *reinterpret_cast<const typename vec8<T>::raw_any*>(p);
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) v[k] = k < n ? p[k] : (T)0.0f;
+    }
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ f32x8 load8(const T* __restrict__ p, uint32_t n) {
+    return __builtin_convertvector(load8_raw<T>(p, n), f32x8);
+}
+// each element is rounded once, to the nearest (ties to even)
+template <typename T>
+__device__ __forceinline__ void store8(T* __restrict__ p, uint32_t n, f32x8 v) {
+    typename vec8<T>::raw r = __builtin_convertvector(v, typename vec8<T>::raw);
+    if (n >= 8) {
+        *reinterpret_cast<typename vec8<T>::raw_any*>(p) = r;
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++)
+            if (k < n) p[k] = r[k];
+    }
+}
+
+// sum / maximum over the 64 lanes of a wave, the same in every lane; a butterfly, so the order is fixed
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, 64);
+    return v;
+}
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+    for (int m = 32; m; m >>= 1) v = fmax(v, __shfl_xor(v, m, 64));
+    return v;
+}
+
+// runs body(T()) for the element type `t`
+#define MDD_FOR_TYPE(t, T, ...)                                   \
+    do {                                                          \
+        if ((t) == MDD_F32) {                                     \
+            typedef float T;                                      \
+            __VA_ARGS__;                                          \
+        } else if ((t) == MDD_BF16) {                             \
+            typedef __bf16 T;                                     \
+            __VA_ARGS__;                                          \
+        } else {                                                  \
+            typedef _Float16 T;                                   \
+            __VA_ARGS__;                                          \
+        }                                                         \
+    } while (0)
+
+}  // namespace mddi
+#endif  // MDD_VEC_H

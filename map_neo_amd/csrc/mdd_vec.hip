@@ -1,0 +1,1098 @@
+// Document vectors: embedding lookup and its gradient, root-mean-square norm (plain, to 8 bits, backward), cosines of
+// candidate edges on 8-bit rows, edge ordering.  Declarations and contracts: include/mdd.h.
+#include "mdd_vec.h"
+
+#include <type_traits>
+#include <utility>
+
+using namespace mddi;
+
+namespace {
+
+constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
+
+// ------------------------------------------------------------------------------------------------ embedding lookup
+// out[d] = f_d * sum of table rows.  A wave sums one document: LPR lanes side by side cover a row's columns (8 each, a
+// slab of 512 columns per wave, further slabs are waves of their own), the 64 / LPR lane groups take neighbouring
+// positions.  64 ids are read at once and handed out by lane, then up to eight rows per group are in flight.
+// The table of a static embedding (64000 x 256 in bf16: 33 MB) lives in the last-level cache, so the kernel is bound by
+// the cache's gather rate, not by HBM.
+//
+// Documents longer than a piece (2^piece_log2 ids) would leave one wave with all the work: the id axis is cut into pieces, a
+// piece's share of a long document goes to a workspace row in float, and pool_join_kernel adds the shares in order.  A piece
+// holds at most two shares -- of the document it starts in (slot 0) and of the one it ends in (slot 1) -- because a
+// document strictly inside a piece is not long.
+struct PoolArgs {
+    const void* table;
+    uint64_t n_rows, stride;
+    uint32_t dim;
+    const void* ids;
+    uint64_t n_ids;
+    const uint64_t* offsets;
+    uint64_t n_docs;
+    int mean;
+    float scale;
+    const uint32_t* row_count;  // gradient of a mean: ids of the document a row stands for; its rows weigh scale / count
+    uint32_t piece_log2;
+    uint64_t n_pieces;
+    float* part;       // [piece][slot][dim]
+    uint32_t* part_n;  // [piece][slot] ids that name a row
+    void* out;
+};
+
+template <typename T, int U>
+__device__ __forceinline__ void add_rows(const T* __restrict__ table, uint64_t stride, uint32_t row_of_lane, float w_of_lane, bool weighted,
+                                         int first, int step, uint32_t n_cols, f32x8& acc) {
+    typename vec8<T>::raw raw[U];
+    uint32_t r[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        r[u] = __shfl(row_of_lane, first + u * step, 64);
+        raw[u] = load8_raw<T>(table + (uint64_t)(r[u] != NO_ROW ? r[u] : 0) * stride, n_cols);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        f32x8 v = __builtin_convertvector(raw[u], f32x8);
+        const float w = weighted ? __shfl(w_of_lane, first + u * step, 64) : 1.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float x = r[u] != NO_ROW ? v[k] : 0.0f;  // padding read row 0: whatever it holds, NaN included, is dropped
+            acc[k] = weighted ? fmaf(x, w, acc[k]) : acc[k] + x;
+        }
+    }
+}
+
+// sum of the rows named by ids [beg, end) in this lane's columns; n_named = ids that name a row.  Call with all lanes.
+template <typename T, typename ID, int LPR>
+__device__ __forceinline__ f32x8 sum_span(const PoolArgs& a, uint64_t beg, uint64_t end, uint32_t col, uint32_t& n_named) {
+    constexpr int G = 64 / LPR;
+    const T* __restrict__ table = reinterpret_cast<const T*>(a.table) + (col < a.dim ? col : 0);
+    const uint32_t n_cols = col < a.dim ? a.dim - col : 0;
+    const ID* __restrict__ ids = reinterpret_cast<const ID*>(a.ids);
+    const int lane = (int)lane_id(), g = lane / LPR;
+    f32x8 acc = 0.0f;
+    n_named = 0;
+    const bool weighted = a.row_count != nullptr;
+    for (uint64_t p = beg; p < end; p += 64) {
+        uint32_t row = NO_ROW;
+        float w = 0.0f;
+        if (p + lane < end) {
+            const uint64_t id = (uint64_t)(int64_t)ids[p + lane];  // negative ids become huge: padding
+            if (id < a.n_rows) row = (uint32_t)id;
+            if (weighted && row != NO_ROW) w = a.scale / (float)a.row_count[row];
+        }
+        n_named += (uint32_t)__popcll(__ballot(row != NO_ROW));
+        const int n = end - p < 64 ? (int)(end - p) : 64, steps = (n + G - 1) / G;  // steps of G positions, one per group
+        int j = 0;
+        for (; j + 8 <= steps; j += 8) add_rows<T, 8>(table, a.stride, row, w, weighted, j * G + g, G, n_cols, acc);
+        // what is left in batches of 4, 2, 1: at most three more round trips and no row read twice
+        if (j + 4 <= steps) add_rows<T, 4>(table, a.stride, row, w, weighted, j * G + g, G, n_cols, acc), j += 4;
+        if (j + 2 <= steps) add_rows<T, 2>(table, a.stride, row, w, weighted, j * G + g, G, n_cols, acc), j += 2;
+        if (j < steps) add_rows<T, 1>(table, a.stride, row, w, weighted, j * G + g, G, n_cols, acc);
+    }
+#pragma unroll
+    for (int m = LPR; m < 64; m <<= 1)
+#pragma unroll
+        for (int k = 0; k < 8; k++) acc[k] += __shfl_xor(acc[k], m, 64);
+    return acc;
+}
+
+__device__ __forceinline__ float pool_factor(const PoolArgs& a, uint32_t n_named) {
+    if (a.row_count) return 1.0f;  // the rows carried their weights
+    return a.mean ? (n_named ? a.scale / (float)n_named : 0.0f) : a.scale;
+}
+
+// last document whose range begins at or before pos; n_docs when there is none
+__device__ __forceinline__ uint64_t doc_at(const uint64_t* __restrict__ offsets, uint64_t n_docs, uint64_t pos) {
+    uint64_t lo = 0, hi = n_docs;  // offsets[lo - 1] <= pos < offsets[hi]
+    while (lo < hi) {
+        const uint64_t mid = (lo + hi) >> 1;
+        if (offsets[mid] <= pos) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo ? lo - 1 : n_docs;
+}
+
+template <typename T, typename ID, typename O, int LPR>
+__global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
+    const uint32_t lane = lane_id(), col = blockIdx.y * 512u + (lane % LPR) * 8u;
+    const bool writes = lane < LPR && col < a.dim;
+    const uint64_t n_work = a.n_pieces + a.n_docs, stride = (uint64_t)gridDim.x * 4;
+    const uint64_t piece = 1ull << a.piece_log2;
+    for (uint64_t w = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; w < n_work; w += stride) {
+        uint32_t n_named;
+        if (w < a.n_pieces) {  // shares of long documents
+            const uint64_t lo = w << a.piece_log2, hi = lo + piece < a.n_ids ? lo + piece : a.n_ids;
+            const uint64_t d0 = doc_at(a.offsets, a.n_docs, lo), d1 = doc_at(a.offsets, a.n_docs, hi - 1);
+#pragma unroll 1
+            for (int slot = 0; slot < 2; slot++) {
+                const uint64_t d = slot ? d1 : d0;
+                if (d >= a.n_docs || (slot && d1 == d0)) continue;
+                uint64_t beg, end;
+                doc_range(a.offsets, d, a.n_ids, beg, end);
+                if (end - beg <= piece) continue;
+                beg = beg > lo ? beg : lo;
+                end = end < hi ? end : hi;
+                f32x8 acc = sum_span<T, ID, LPR>(a, beg, end, col, n_named);
+                const uint64_t at = w * 2 + slot;
+                if (writes) store8<float>(a.part + at * a.dim + col, a.dim - col, acc);
+                if (lane == 0 && blockIdx.y == 0) a.part_n[at] = n_named;
+            }
+        } else {
+            const uint64_t d = w - a.n_pieces;
+            uint64_t beg, end;
+            doc_range(a.offsets, d, a.n_ids, beg, end);
+            if (a.n_pieces && end - beg > piece) continue;  // pool_join_kernel writes it
+            f32x8 acc = sum_span<T, ID, LPR>(a, beg, end, col, n_named);
+            if (writes) store8<O>(reinterpret_cast<O*>(a.out) + d * a.dim + col, a.dim - col, acc * pool_factor(a, n_named));
+        }
+    }
+}
+
+// A wave per document and 512 columns; only long ones have work: the shares of their pieces, in order, eight at a time.
+template <typename O>
+__global__ __launch_bounds__(256) void pool_join_kernel(PoolArgs a) {
+    const uint32_t lane = lane_id(), col = blockIdx.y * 512u + lane * 8u;
+    const uint64_t piece = 1ull << a.piece_log2, stride = (uint64_t)gridDim.x * 4;
+    for (uint64_t d = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; d < a.n_docs; d += stride) {
+        uint64_t beg, end;
+        doc_range(a.offsets, d, a.n_ids, beg, end);
+        if (end - beg <= piece) continue;
+        const uint64_t first = beg >> a.piece_log2, last = (end - 1) >> a.piece_log2;
+        // a long document leaves its first piece, so it is slot 0 there only if the piece begins with it
+        const uint64_t at0 = first * 2 + (beg > first << a.piece_log2 ? 1 : 0);
+        uint32_t n_named = 0;
+        for (uint64_t k = first + lane; k <= last; k += 64) n_named += a.part_n[k == first ? at0 : k * 2];
+#pragma unroll
+        for (int m = 32; m; m >>= 1) n_named += __shfl_xor(n_named, m, 64);
+        if (col >= a.dim) continue;
+        const float* __restrict__ part = a.part + col;
+        f32x8 acc = load8<float>(part + at0 * a.dim, a.dim - col);
+        uint64_t k = first + 1;
+        for (; k + 8 <= last + 1; k += 8) {
+            f32x8 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] = load8<float>(part + (k + u) * 2 * a.dim, a.dim - col);
+#pragma unroll
+            for (int u = 0; u < 8; u++) acc += v[u];
+        }
+        for (; k <= last; k++) acc += load8<float>(part + k * 2 * a.dim, a.dim - col);
+        store8<O>(reinterpret_cast<O*>(a.out) + d * a.dim + col, a.dim - col, acc * pool_factor(a, n_named));
+    }
+}
+
+// One row per id: eight rows per lane group in flight, read and written once -- bound by HBM where the table is large.
+template <typename T, typename ID, int LPR>
+__global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table, uint64_t n_rows, uint64_t row_stride, uint32_t dim,
+                                                     const ID* __restrict__ ids, uint64_t n_ids, float scale, T* __restrict__ out) {
+    constexpr int G = 64 / LPR, U = LPR < 8 ? LPR : 8;  // positions per wave and round: U * G <= 64
+    const uint32_t lane = lane_id(), g = lane / LPR, col = blockIdx.y * 512u + (lane % LPR) * 8u;
+    const uint64_t stride = (uint64_t)gridDim.x * 4 * (U * G);
+    for (uint64_t p = ((uint64_t)blockIdx.x * 4 + threadIdx.x / 64) * (U * G); p < n_ids; p += stride) {
+        uint32_t row = NO_ROW;
+        if (lane < U * G && p + lane < n_ids) {
+            const uint64_t id = (uint64_t)(int64_t)ids[p + lane];
+            if (id < n_rows) row = (uint32_t)id;
+        }
+        uint32_t r[U];
+        typename vec8<T>::raw raw[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            r[u] = __shfl(row, u * G + g, 64);
+            raw[u] = 0;
+            if (r[u] != NO_ROW && col < dim) raw[u] = load8_raw<T>(table + r[u] * row_stride + col, dim - col);
+        }
+        if (col < dim) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (p + u * G + g < n_ids) {
+                    f32x8 v = __builtin_convertvector(raw[u], f32x8) * scale;
+                    if (r[u] == NO_ROW) v = 0.0f;  // also where the scale is no number
+                    store8<T>(out + (p + u * G + g) * dim + col, dim - col, v);
+                }
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void fill_kernel(T* __restrict__ p, uint64_t n, T v) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) p[i] = v;
+}
+
+// ------------------------------------------------------------------------------------------ stable sort of (key, value)
+// Least significant digit first, 8 bits a pass.  A wave ranks 64 keys at a time in their order: eight ballots give the
+// lanes with the same digit, the ones below are the rank, a counter per wave and digit carries it on -- so equal keys keep
+// their order and nothing depends on which wave runs first.
+__device__ __forceinline__ uint32_t rank_digit(uint32_t digit, bool live, volatile uint32_t* counter) {  // volatile: other lanes write it
+    uint64_t same = __ballot(live);
+#pragma unroll
+    for (int b = 0; b < 8; b++) {
+        const uint64_t set = __ballot(live && (digit >> b & 1));
+        same &= (digit >> b & 1) ? set : ~set;
+    }
+    uint32_t before = 0;
+    if (live) before = counter[digit];
+    const uint32_t rank = before + below(same);
+    __builtin_amdgcn_wave_barrier();
+    if (live && below(same) == 0) counter[digit] = before + (uint32_t)__popcll(same);
+    __builtin_amdgcn_wave_barrier();
+    return rank;
+}
+
+constexpr uint32_t SORT_TILE = 4096, SMALL_SORT = 8192;
+
+__global__ __launch_bounds__(256) void sort_count_kernel(const uint32_t* __restrict__ key, uint32_t n, int shift, uint32_t n_tiles,
+                                                         uint32_t* __restrict__ hist) {
+    __shared__ uint32_t cnt[256];
+    cnt[threadIdx.x] = 0;
+    __syncthreads();
+    const uint32_t base = blockIdx.x * SORT_TILE;
+#pragma unroll 4
+    for (uint32_t k = 0; k < SORT_TILE; k += 256) {
+        const uint32_t i = base + k + threadIdx.x;
+        if (i < n) atomicAdd(&cnt[key[i] >> shift & 255u], 1u);
+    }
+    __syncthreads();
+    hist[(uint64_t)threadIdx.x * n_tiles + blockIdx.x] = cnt[threadIdx.x];
+}
+
+// exclusive sum over the 256 threads of a block; *total = the sum
+__device__ __forceinline__ uint32_t block_scan256(uint32_t v, uint32_t* lds4, uint32_t* total) {
+    const uint32_t lane = lane_id(), wave = threadIdx.x / 64;
+    uint32_t s = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(s, d, 64);
+        if (lane >= (uint32_t)d) s += o;
+    }
+    if (lane == 63) lds4[wave] = s;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; w++) {
+        if (w < wave) before += lds4[w];
+        all += lds4[w];
+    }
+    __syncthreads();
+    *total = all;
+    return before + s - v;
+}
+
+// block = digit: exclusive sums of its tile counts in place, their total behind the table
+__global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t* __restrict__ hist, uint32_t n_tiles) {
+    __shared__ uint32_t lds4[4];
+    uint32_t* row = hist + (uint64_t)blockIdx.x * n_tiles;
+    uint32_t carry = 0;
+    for (uint32_t k = 0; k < n_tiles; k += 256) {
+        const uint32_t i = k + threadIdx.x, v = i < n_tiles ? row[i] : 0;
+        uint32_t total;
+        const uint32_t ex = block_scan256(v, lds4, &total);
+        if (i < n_tiles) row[i] = carry + ex;
+        carry += total;
+    }
+    if (threadIdx.x == 0) hist[(uint64_t)256 * n_tiles + blockIdx.x] = carry;
+}
+
+__global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ val, uint32_t n, int shift,
+                                                           uint32_t n_tiles, const uint32_t* __restrict__ hist, uint32_t* __restrict__ key_out,
+                                                           uint32_t* __restrict__ val_out) {
+    __shared__ uint32_t cnt[4][256], lds4[4];
+    const uint32_t t = threadIdx.x, wave = t / 64, lane = lane_id();
+    for (int w = 0; w < 4; w++) cnt[w][t] = 0;
+    __syncthreads();
+    const uint32_t base = blockIdx.x * SORT_TILE + wave * (SORT_TILE / 4) + lane;
+    uint32_t k_[16], rank[16];
+#pragma unroll
+    for (int r = 0; r < 16; r++) k_[r] = base + r * 64 < n ? key[base + r * 64] : 0;
+#pragma unroll
+    for (int r = 0; r < 16; r++) rank[r] = rank_digit(k_[r] >> shift & 255u, base + r * 64 < n, cnt[wave]);
+    __syncthreads();
+    uint32_t all;
+    uint32_t at = block_scan256(hist[(uint64_t)256 * n_tiles + t], lds4, &all) + hist[(uint64_t)t * n_tiles + blockIdx.x];
+    for (int w = 0; w < 4; w++) {
+        const uint32_t c = cnt[w][t];
+        cnt[w][t] = at;
+        at += c;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+        if (base + r * 64 < n) {
+            const uint32_t to = cnt[wave][k_[r] >> shift & 255u] + rank[r];
+            if (to < n) {  // always, unless the keys change while they are sorted
+                key_out[to] = k_[r];
+                val_out[to] = val[base + r * 64];
+            }
+        }
+}
+
+// up to SMALL_SORT pairs in one block and one launch: all passes in LDS (8 us where the passes above take 12 launches)
+__global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__ key, uint32_t* __restrict__ val, uint32_t n, int bits) {
+    __shared__ uint32_t ks[SMALL_SORT], vs[SMALL_SORT], cnt[16][256], lds4[4];
+    const uint32_t t = threadIdx.x, wave = t / 64, lane = lane_id(), base = wave * 512 + lane;
+    uint32_t k_[8], v_[8], rank[8];
+#pragma unroll
+    for (int r = 0; r < 8; r++) {
+        const uint32_t i = base + r * 64;
+        k_[r] = i < n ? key[i] : 0;
+        v_[r] = i < n ? val[i] : 0;
+    }
+    for (int shift = 0; shift < bits; shift += 8) {
+        for (uint32_t i = t; i < 16 * 256; i += 1024) (&cnt[0][0])[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 8; r++) rank[r] = rank_digit(k_[r] >> shift & 255u, base + r * 64 < n, cnt[wave]);
+        __syncthreads();
+        uint32_t own = 0;
+        if (t < 256)
+            for (int w = 0; w < 16; w++) own += cnt[w][t];
+        uint32_t ex = own;
+        if (wave < 4) {
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t o = __shfl_up(ex, d, 64);
+                if (lane >= (uint32_t)d) ex += o;
+            }
+            if (lane == 63) lds4[wave] = ex;
+        }
+        __syncthreads();
+        if (t < 256) {
+            uint32_t at = ex - own;
+            for (uint32_t w = 0; w < wave; w++) at += lds4[w];
+            for (int w = 0; w < 16; w++) {
+                const uint32_t c = cnt[w][t];
+                cnt[w][t] = at;
+                at += c;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 8; r++)
+            if (base + r * 64 < n) {
+                const uint32_t to = cnt[wave][k_[r] >> shift & 255u] + rank[r];
+                ks[to] = k_[r];
+                vs[to] = v_[r];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            const uint32_t i = base + r * 64;
+            k_[r] = i < n ? ks[i] : 0;
+            v_[r] = i < n ? vs[i] : 0;
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < 8; r++)
+        if (base + r * 64 < n) {
+            key[base + r * 64] = k_[r];
+            val[base + r * 64] = v_[r];
+        }
+}
+
+int bits_of(uint64_t largest) {
+    int b = 1;
+    while (b < 64 && largest >> b) b++;
+    return b;
+}
+uint64_t sort_hist_words(uint64_t n) { return n <= SMALL_SORT ? 0 : 256 * ((n + SORT_TILE - 1) / SORT_TILE) + 256; }
+// sorts (key, val) by key, the values of equal keys in their order.  (key2, val2) are scratch of the same length (unused up to
+// SMALL_SORT pairs); the result is in key / val, which change places with key2 / val2 in every pass
+void sort_pairs(hipStream_t s, uint32_t*& key, uint32_t*& val, uint32_t*& key2, uint32_t*& val2, uint64_t n, int bits, uint32_t* hist) {
+    if (n <= SMALL_SORT) {
+        hipLaunchKernelGGL(small_sort_kernel, dim3(1), dim3(1024), 0, s, key, val, (uint32_t)n, bits);
+        return;
+    }
+    const uint32_t tiles = (uint32_t)((n + SORT_TILE - 1) / SORT_TILE);
+    for (int shift = 0; shift < bits; shift += 8) {
+        hipLaunchKernelGGL(sort_count_kernel, dim3(tiles), dim3(256), 0, s, key, (uint32_t)n, shift, tiles, hist);
+        hipLaunchKernelGGL(sort_scan_kernel, dim3(256), dim3(256), 0, s, hist, tiles);
+        hipLaunchKernelGGL(sort_scatter_kernel, dim3(tiles), dim3(256), 0, s, key, val, (uint32_t)n, shift, tiles, hist, key2, val2);
+        std::swap(key, key2);
+        std::swap(val, val2);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ gradient of the lookup
+// key[p] = id, or n_rows for padding and for positions outside every document; val[p] = the row of the gradient that
+// position p's table row took part in.  With count given, the documents' named ids are counted (whole numbers: the order
+// of the atomics does not matter; one atomic per wave where the wave lies in one document).
+template <typename ID>
+__global__ __launch_bounds__(256) void grad_keys_kernel(const ID* __restrict__ ids, uint64_t n_ids, uint64_t n_rows, const uint64_t* __restrict__ offsets,
+                                                        uint64_t n_docs, uint32_t* __restrict__ count, uint32_t* __restrict__ key, uint32_t* __restrict__ val) {
+    const uint64_t p = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    uint64_t row = p;
+    bool named = false;
+    if (p < n_ids) {
+        const uint64_t id = (uint64_t)(int64_t)ids[p];
+        named = id < n_rows;
+        if (offsets) {
+            row = doc_at(offsets, n_docs, p);
+            uint64_t beg = 0, end = 0;
+            if (row < n_docs) doc_range(offsets, row, n_ids, beg, end);
+            if (p < beg || p >= end) named = false;
+        }
+        key[p] = named ? (uint32_t)id : (uint32_t)n_rows;
+        val[p] = named ? (uint32_t)row : 0u;
+    }
+    if (!count) return;
+    const uint64_t live = __ballot(named);
+    if (!live) return;
+    const int leader = __ffsll((unsigned long long)live) - 1;
+    const uint32_t first = __shfl((uint32_t)row, leader, 64);
+    if (__ballot(named && (uint32_t)row != first) == 0) {
+        if ((int)lane_id() == leader) atomicAdd(&count[first], (uint32_t)__popcll(live));
+    } else if (named) {
+        atomicAdd(&count[row], 1u);
+    }
+}
+
+// start[v] = first sorted position with a key >= v, v = 0 .. n_rows
+__global__ __launch_bounds__(256) void grad_starts_kernel(const uint32_t* __restrict__ key, uint32_t n, uint64_t n_rows, uint64_t* __restrict__ start) {
+    const uint64_t v = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (v > n_rows) return;
+    uint32_t lo = 0, hi = n;
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (key[mid] < v) lo = mid + 1;
+        else hi = mid;
+    }
+    start[v] = lo;
+}
+
+// ------------------------------------------------------------------------------------------------ launching the sums
+uint32_t piece_log2_for(uint64_t n_ids) {
+    // about 8192 pieces (two waves for each of the 4096 that the chip holds at sixteen per CU) of 32 to 1024 ids: short
+    // enough to spread one long document over the chip, long enough that the shares stay a fraction of the rows read
+    uint32_t b = 5;
+    while (b < 10 && (n_ids >> b) > 8192) b++;
+    return b;
+}
+uint64_t n_pieces_for(uint64_t n_ids) {
+    const uint32_t b = piece_log2_for(n_ids);
+    return n_ids <= (1ull << b) ? 0 : (n_ids + (1ull << b) - 1) >> b;  // none is long where all ids fit one piece
+}
+uint64_t pool_ws_bytes(uint64_t n_ids, uint32_t dim) {
+    const uint64_t p = n_pieces_for(n_ids);
+    return p ? round_up(p * 2 * dim * 4, 256) + round_up(p * 2 * 4, 256) : 0;
+}
+
+template <typename T, typename ID, typename O>
+void launch_pool(hipStream_t s, const PoolArgs& a) {
+    const uint32_t slabs = (a.dim + 511) / 512, chunks = (a.dim + 7) / 8;
+    const uint64_t cap = (1u << 20) / slabs + 1;
+    const uint64_t want = (a.n_pieces + a.n_docs + 3) / 4;
+    const dim3 grid((unsigned)(want < cap ? want : cap), slabs), block(256);
+    if (chunks > 32) hipLaunchKernelGGL((pool_kernel<T, ID, O, 64>), grid, block, 0, s, a);
+    else if (chunks > 16) hipLaunchKernelGGL((pool_kernel<T, ID, O, 32>), grid, block, 0, s, a);
+    else if (chunks > 8) hipLaunchKernelGGL((pool_kernel<T, ID, O, 16>), grid, block, 0, s, a);
+    else if (chunks > 4) hipLaunchKernelGGL((pool_kernel<T, ID, O, 8>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((pool_kernel<T, ID, O, 4>), grid, block, 0, s, a);
+    if (a.n_pieces) {
+        const uint64_t docs = (a.n_docs + 3) / 4;
+        hipLaunchKernelGGL((pool_join_kernel<O>), dim3((unsigned)(docs < cap ? docs : cap), slabs), block, 0, s, a);
+    }
+}
+
+template <typename T, typename ID>
+void launch_lookup(hipStream_t s, const T* table, uint64_t n_rows, uint64_t stride, uint32_t dim, const ID* ids, uint64_t n_ids, float scale, T* out) {
+    const uint32_t slabs = (dim + 511) / 512, chunks = (dim + 7) / 8;
+    const uint32_t lpr = chunks > 32 ? 64 : chunks > 16 ? 32 : chunks > 8 ? 16 : chunks > 4 ? 8 : 4;
+    const uint64_t per_block = 4ull * (64 / lpr) * (lpr < 8 ? lpr : 8), cap = (1u << 22) / slabs + 1, want = (n_ids + per_block - 1) / per_block;
+    const dim3 grid((unsigned)(want < cap ? want : cap), slabs), block(256);
+    if (lpr == 64) hipLaunchKernelGGL((lookup_kernel<T, ID, 64>), grid, block, 0, s, table, n_rows, stride, dim, ids, n_ids, scale, out);
+    else if (lpr == 32) hipLaunchKernelGGL((lookup_kernel<T, ID, 32>), grid, block, 0, s, table, n_rows, stride, dim, ids, n_ids, scale, out);
+    else if (lpr == 16) hipLaunchKernelGGL((lookup_kernel<T, ID, 16>), grid, block, 0, s, table, n_rows, stride, dim, ids, n_ids, scale, out);
+    else if (lpr == 8) hipLaunchKernelGGL((lookup_kernel<T, ID, 8>), grid, block, 0, s, table, n_rows, stride, dim, ids, n_ids, scale, out);
+    else hipLaunchKernelGGL((lookup_kernel<T, ID, 4>), grid, block, 0, s, table, n_rows, stride, dim, ids, n_ids, scale, out);
+}
+
+// ------------------------------------------------------------------------------------------------ norm
+// A row is held in registers, 8 * NC columns a lane, by W waves: one up to 2048 columns (no barrier; four rows a block),
+// four up to 8192, sixteen beyond.  x is read once and everything written once: bound by HBM.
+template <int W>
+__device__ __forceinline__ float row_sum(float v, float* lds) {
+    v = wave_sum(v);
+    if (W == 1) return v;
+    if (lane_id() == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    float s = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) s += lds[w];
+    __syncthreads();
+    return s;
+}
+template <int W>
+__device__ __forceinline__ double row_max(double v, double* lds) {
+    v = wave_max(v);
+    if (W == 1) return v;
+    if (lane_id() == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    double s = lds[0];
+#pragma unroll
+    for (int w = 1; w < W; w++) s = fmax(s, lds[w]);
+    __syncthreads();
+    return s;
+}
+
+template <typename T, int NC, int W>
+__global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_kernel(const T* __restrict__ x, uint64_t xs, const T* __restrict__ res, uint64_t rs,
+                                                                    const T* __restrict__ weight, float eps, uint64_t n, uint32_t dim, T* __restrict__ y,
+                                                                    T* __restrict__ sum_out, float* __restrict__ rstd) {
+    constexpr uint32_t RPB = W == 1 ? 4 : 1, TPR = W * 64;
+    __shared__ float lds[W];
+    const uint32_t t = threadIdx.x % TPR;
+    for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < n; row += (uint64_t)gridDim.x * RPB) {
+        f32x8 h[NC];
+        float ss = 0;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const uint32_t col = (c * TPR + t) * 8;
+            h[c] = 0.0f;
+            if (col < dim) {
+                h[c] = load8<T>(x + row * xs + col, dim - col);
+                if (res) h[c] += load8<T>(res + row * rs + col, dim - col);
+                if (sum_out) store8<T>(sum_out + row * dim + col, dim - col, h[c]);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) ss = fmaf(h[c][k], h[c][k], ss);
+        }
+        const float r = 1.0f / sqrtf(row_sum<W>(ss, lds) / (float)dim + eps);
+        if (rstd && t == 0) rstd[row] = r;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const uint32_t col = (c * TPR + t) * 8;
+            if (col >= dim) continue;
+            f32x8 v = h[c] * r;
+            if (weight) v *= load8<T>(weight + col, dim - col);
+            store8<T>(y + row * dim + col, dim - col, v);
+        }
+    }
+}
+
+// The nearest 8-bit value to z = y * top / big.  zf is z rounded to 32 bits, at most 2^-24 of its size off, which is below
+// 1e-5 of a step; only next to a midpoint is z itself formed, a correctly rounded quotient in 64 bits -- rarely, so the codes
+// are those of exact arithmetic and do not depend on how the row was summed, without a division per element.
+template <int KIND>
+__device__ __forceinline__ float nearest8(float zf, double y, double top, double big) {
+    float step = 1.0f;
+    if (KIND == MDD_E4M3) {
+        const int e = (int)(__float_as_uint(zf) >> 23 & 255u) - 127;
+        step = __uint_as_float((uint32_t)((e > -6 ? e : -6) - 3 + 127) << 23);
+    }
+    const float u = zf / step, q = rintf(u);  // the step is a power of two: exact
+    if (fabsf(fabsf(u - q) - 0.5f) > 2e-5f) return q * step;
+    const double z = y * top / big;
+    if (KIND == MDD_E4M3) {  // the step of z itself: zf may lie across a power of two
+        double s = exp2(fmax(floor(log2(fmax(fabs(z), 0.015625))), -6.0) - 3.0);
+        return (float)(rint(z / s) * s);
+    }
+    return (float)rint(z);
+}
+
+template <typename T, int NC, int W, int KIND>
+__global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* __restrict__ x, uint64_t xs, const T* __restrict__ res, uint64_t rs,
+                                                                       const T* __restrict__ weight, float eps, uint64_t n, uint32_t dim,
+                                                                       uint8_t* __restrict__ codes, float* __restrict__ scales, T* __restrict__ sum_out) {
+    constexpr uint32_t RPB = W == 1 ? 4 : 1, TPR = W * 64;
+    __shared__ float lds[W];
+    __shared__ double ldsd[W];
+    const uint32_t t = threadIdx.x % TPR;
+    const float top = KIND == MDD_I8 ? 127.0f : 448.0f;
+    for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < n; row += (uint64_t)gridDim.x * RPB) {
+        double y[NC][8];  // h * weight: a sum and a product of 8 to 24-bit numbers, nearly always exact in 64 bits
+        float ss = 0;
+        double big = 0;
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const uint32_t col = (c * TPR + t) * 8;
+            f32x8 v = 0.0f, o = 0.0f, w = 1.0f;
+            if (col < dim) {
+                v = load8<T>(x + row * xs + col, dim - col);
+                if (res) o = load8<T>(res + row * rs + col, dim - col);
+                if (weight) w = load8<T>(weight + col, dim - col);
+                if (sum_out) store8<T>(sum_out + row * dim + col, dim - col, v + o);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float h = v[k] + o[k];
+                ss = fmaf(h, h, ss);
+                y[c][k] = ((double)v[k] + (double)o[k]) * (double)w[k];
+                bad |= !(fabs(y[c][k]) < __builtin_inf());
+                big = fmax(big, fabs(y[c][k]));
+            }
+        }
+        if (bad) big = __builtin_inf();  // fmax drops a NaN: an infinity stands for both
+        big = row_max<W>(big, ldsd);
+        const float r = 1.0f / sqrtf(row_sum<W>(ss, lds) / (float)dim + eps);
+        const bool fine = big < __builtin_inf();
+        if (t == 0) scales[row] = fine ? (float)big * r / top : __builtin_nanf("");
+        const double inv = big > 0 ? (double)top / big : 0.0;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const uint32_t col = (c * TPR + t) * 8;
+            if (col >= dim) continue;
+            uint32_t pack[2] = {0, 0};
+            if (fine && big > 0) {
+                float q[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) q[k] = nearest8<KIND>((float)(y[c][k] * inv), y[c][k], (double)top, big);
+#pragma unroll
+                for (int k = 0; k < 8; k += 4) {
+                    if (KIND == MDD_I8) {
+                        pack[k / 4] = ((uint32_t)(int)q[k] & 255u) | ((uint32_t)(int)q[k + 1] & 255u) << 8 | ((uint32_t)(int)q[k + 2] & 255u) << 16 |
+                                      ((uint32_t)(int)q[k + 3] & 255u) << 24;
+                    } else {
+                        int p = __builtin_amdgcn_cvt_pk_fp8_f32(q[k], q[k + 1], 0, false);  // exact: q is an e4m3 value
+                        pack[k / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[k + 2], q[k + 3], p, true);
+                    }
+                }
+            }
+            uint8_t* to = codes + row * dim + col;
+            if (dim - col >= 8) {
+                typedef uint32_t pair_any __attribute__((ext_vector_type(2), aligned(1)));
+                *reinterpret_cast<pair_any*>(to) = pair_any{pack[0], pack[1]};
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < 8; k++)
+                    if (col + k < dim) to[k] = (uint8_t)(pack[k / 4] >> (8 * (k % 4)));
+            }
+        }
+    }
+}
+
+// Backward: a fixed number of blocks walks the rows; the weight's gradient stays in registers over a block's rows, goes to a
+// workspace row per block and is added up by weight_grad_kernel in block order.
+template <typename T, int NC, int W>
+__global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_backward_kernel(const T* __restrict__ g, uint64_t gs, const T* __restrict__ h, uint64_t hs,
+                                                                             const T* __restrict__ gsum, uint64_t gss, const T* __restrict__ weight,
+                                                                             const float* __restrict__ rstd, uint64_t n, uint32_t dim, T* __restrict__ dx,
+                                                                             float* __restrict__ part) {
+    constexpr uint32_t RPB = W == 1 ? 4 : 1, TPR = W * 64;
+    __shared__ float lds[W];
+    __shared__ __attribute__((aligned(32))) float across[W == 1 ? 3 * 512 : 8];
+    const uint32_t t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    f32x8 w[NC], dw[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const uint32_t col = (c * TPR + t) * 8;
+        w[c] = 1.0f;
+        if (weight && col < dim) w[c] = load8<T>(weight + col, dim - col);
+        dw[c] = 0.0f;
+    }
+    for (uint64_t row = (uint64_t)blockIdx.x * RPB + sub; row < n; row += (uint64_t)gridDim.x * RPB) {
+        const float r = rstd[row];
+        f32x8 nx[NC], gw[NC];
+        float dot = 0;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const uint32_t col = (c * TPR + t) * 8;
+            nx[c] = 0.0f, gw[c] = 0.0f;
+            if (col < dim) {
+                nx[c] = load8<T>(h + row * hs + col, dim - col) * r;
+                gw[c] = load8<T>(g + row * gs + col, dim - col);
+            }
+            dw[c] += gw[c] * nx[c];
+            gw[c] *= w[c];
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (col + k < dim) dot = fmaf(gw[c][k], nx[c][k], dot);
+        }
+        const float mean = row_sum<W>(dot, lds) / (float)dim;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const uint32_t col = (c * TPR + t) * 8;
+            if (col >= dim) continue;
+            f32x8 v = (gw[c] - nx[c] * mean) * r;
+            if (gsum) v += load8<T>(gsum + row * gss + col, dim - col);
+            store8<T>(dx + row * dim + col, dim - col, v);
+        }
+    }
+    if (!part) return;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const uint32_t col = (c * TPR + t) * 8;
+        if (W == 1) {
+            if (sub) *reinterpret_cast<f32x8*>(&across[(sub - 1) * 512 + t * 8]) = dw[c];
+            __syncthreads();
+            if (!sub)
+                for (int s = 0; s < 3; s++) dw[c] += *reinterpret_cast<const f32x8*>(&across[s * 512 + t * 8]);
+            __syncthreads();
+        }
+        if (sub == 0 && col < dim) store8<float>(part + (uint64_t)blockIdx.x * dim + col, dim - col, dw[c]);
+    }
+}
+
+// 64 columns a block, its 16 waves take every 16th workspace row
+__global__ __launch_bounds__(1024) void weight_grad_kernel(const float* __restrict__ part, uint32_t n_parts, uint32_t dim, float* __restrict__ out) {
+    __shared__ float lds[16][64];
+    const uint32_t lane = lane_id(), wave = threadIdx.x / 64, col = blockIdx.x * 64 + lane;
+    float s = 0;
+    if (col < dim) {
+#pragma unroll 8
+        for (uint32_t p = wave; p < n_parts; p += 16) s += part[(uint64_t)p * dim + col];
+    }
+    lds[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && col < dim) {
+        s = 0;
+#pragma unroll
+        for (int w = 0; w < 16; w++) s += lds[w][lane];
+        out[col] = s;
+    }
+}
+
+uint32_t backward_blocks(uint64_t n, uint32_t dim) {
+    const uint64_t want = dim <= 2048 ? (n + 3) / 4 : n;
+    return (uint32_t)(want < 512 ? want : 512);  // two blocks a CU
+}
+
+// picks NC and W of a row kernel; body(NC, W) as integral constants
+template <typename F>
+void for_width(uint32_t dim, F&& body) {
+    if (dim <= 512) body(std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
+    else if (dim <= 1024) body(std::integral_constant<int, 2>(), std::integral_constant<int, 1>());
+    else if (dim <= 2048) body(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
+    else if (dim <= 4096) body(std::integral_constant<int, 2>(), std::integral_constant<int, 4>());
+    else if (dim <= 8192) body(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
+    else if (dim <= 16384) body(std::integral_constant<int, 2>(), std::integral_constant<int, 16>());
+    else body(std::integral_constant<int, 4>(), std::integral_constant<int, 16>());
+}
+dim3 row_grid(uint64_t n, int W) {
+    const uint64_t want = W == 1 ? (n + 3) / 4 : n;
+    return dim3((unsigned)(want < (1u << 20) ? want : (1u << 20)));
+}
+
+// ------------------------------------------------------------------------------------------------ edge cosines
+// Sixteen lanes take an edge, 16 bytes of both rows a step: four edges a wave.  Bound by the gather of two rows per edge.
+__device__ __forceinline__ u32x4 load_bytes16(const uint8_t* __restrict__ p, uint32_t n) {
+    typedef uint32_t any __attribute__((ext_vector_type(4), aligned(1)));
+    u32x4 v = 0;
+    if (n >= 16) {
+        v = *reinterpret_cast<const any*>(p);
+    } else {
+        for (uint32_t k = 0; k < n; k++) {
+            const uint32_t b = (uint32_t)p[k] << (8 * (k % 4));
+            if (k < 4) v[0] |= b;
+            else if (k < 8) v[1] |= b;
+            else if (k < 12) v[2] |= b;
+            else v[3] |= b;
+        }
+    }
+    return v;
+}
+template <int KIND>
+__global__ __launch_bounds__(256) void edge_cosine_kernel(const uint8_t* __restrict__ codes, uint64_t stride, uint64_t n_rows, uint32_t dim,
+                                                          const uint32_t* __restrict__ eu, const uint32_t* __restrict__ ev, uint64_t n_edges,
+                                                          float* __restrict__ cosines) {
+    const uint32_t t = threadIdx.x % 16;
+    for (uint64_t e = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16; e < n_edges; e += (uint64_t)gridDim.x * 16) {
+        const uint64_t u = eu[e], v = ev[e];
+        const bool ok = u < n_rows && v < n_rows;
+        const uint8_t *a = codes + (ok ? u : 0) * stride, *b = codes + (ok ? v : 0) * stride;
+        float ab, aa, bb;
+        if (KIND == MDD_I8) {
+            int iab = 0, iaa = 0, ibb = 0;  // 32768 products of at most 2^14: below 2^30
+            for (uint32_t c = t * 16; c < (ok ? dim : 0); c += 256) {
+                const u32x4 x = load_bytes16(a + c, dim - c), y = load_bytes16(b + c, dim - c);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    iab = __builtin_amdgcn_sdot4((int)x[k], (int)y[k], iab, false);
+                    iaa = __builtin_amdgcn_sdot4((int)x[k], (int)x[k], iaa, false);
+                    ibb = __builtin_amdgcn_sdot4((int)y[k], (int)y[k], ibb, false);
+                }
+            }
+#pragma unroll
+            for (int m = 8; m; m >>= 1) iab += __shfl_xor(iab, m, 64), iaa += __shfl_xor(iaa, m, 64), ibb += __shfl_xor(ibb, m, 64);
+            ab = (float)iab, aa = (float)iaa, bb = (float)ibb;
+        } else {
+            ab = aa = bb = 0;
+            for (uint32_t c = t * 16; c < (ok ? dim : 0); c += 256) {
+                const u32x4 x = load_bytes16(a + c, dim - c), y = load_bytes16(b + c, dim - c);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    auto x0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[k], false), x1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[k], true);
+                    auto y0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)y[k], false), y1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)y[k], true);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        ab = fmaf(x0[i], y0[i], ab), aa = fmaf(x0[i], x0[i], aa), bb = fmaf(y0[i], y0[i], bb);
+                        ab = fmaf(x1[i], y1[i], ab), aa = fmaf(x1[i], x1[i], aa), bb = fmaf(y1[i], y1[i], bb);
+                    }
+                }
+            }
+#pragma unroll
+            for (int m = 8; m; m >>= 1) ab += __shfl_xor(ab, m, 64), aa += __shfl_xor(aa, m, 64), bb += __shfl_xor(bb, m, 64);
+        }
+        // a product of the squares stays below 2^63, and a NaN in a row comes through
+        if (t == 0) cosines[e] = !ok || aa == 0.0f || bb == 0.0f ? 0.0f : ab / sqrtf(aa * bb);
+    }
+}
+
+int check_matrix(const char* who, const char* what, const void* p, int type, uint64_t stride, uint32_t dim) {
+    REQUIRE(p, "%s: %s is NULL", who, what);
+    REQUIRE(type_bytes(type), "%s: unknown element type %d", who, type);
+    REQUIRE(stride >= dim, "%s: row stride %llu of %s is below dim %u", who, (unsigned long long)stride, what, dim);
+    REQUIRE(aligned_to(p, type_bytes(type)), "%s: %s is not aligned to its elements", who, what);
+    return MDD_OK;
+}
+#define CHECKED(expr)            \
+    do {                         \
+        const int rc_ = (expr);  \
+        if (rc_) return rc_;     \
+    } while (0)
+
+}  // namespace
+
+extern "C" {
+
+uint64_t mdd_embed_ws_bytes(uint64_t n_ids, uint32_t dim) { return pool_ws_bytes(n_ids, dim); }
+
+int mdd_embed(mdd_ctx* ctx, const void* table, int type, uint64_t n_rows, uint64_t row_stride, uint32_t dim, const void* ids,
+              int id_bytes, uint64_t n_ids, const uint64_t* offsets, uint64_t n_docs, int mean, float scale, void* out,
+              void* ws, uint64_t ws_bytes) {
+    const char* who = "mdd_embed";
+    REQUIRE(ctx, "%s: ctx is NULL", who);
+    REQUIRE(dim >= 1 && dim <= MDD_VEC_MAX_DIM, "%s: dim=%u outside [1,%d]", who, dim, MDD_VEC_MAX_DIM);
+    REQUIRE(type_bytes(type), "%s: unknown element type %d", who, type);
+    REQUIRE(id_bytes == 4 || id_bytes == 8, "%s: id_bytes=%d is neither 4 nor 8", who, id_bytes);
+    REQUIRE(n_ids < (1ull << 31) && n_rows < (1ull << 32) - 1, "%s: more than 2^31 - 1 ids or 2^32 - 2 table rows", who);
+    const uint64_t n_out = offsets ? n_docs : n_ids;
+    if (n_out == 0) return MDD_OK;
+    REQUIRE(out && aligned_to(out, type_bytes(type)), "%s: out is NULL or not aligned to its elements", who);
+    REQUIRE(n_ids == 0 || (ids && aligned_to(ids, id_bytes)), "%s: ids is NULL or not aligned", who);
+    if (n_rows) CHECKED(check_matrix(who, "table", table, type, row_stride, dim));
+    const uint64_t need = offsets && n_rows ? pool_ws_bytes(n_ids, dim) : 0;
+    REQUIRE(need == 0 || (ws && aligned_to(ws, 256) && ws_bytes >= need), "%s: workspace of %llu bytes, 256-byte aligned, needed", who,
+            (unsigned long long)need);
+    ON_DEVICE(ctx);
+    if (n_rows == 0 || n_ids == 0) {  // every id is padding
+        const uint64_t n = n_out * dim;
+        const dim3 grid((unsigned)(n / 256 + 1 < 4096 ? n / 256 + 1 : 4096));
+        if (type == MDD_F32) hipLaunchKernelGGL((fill_kernel<uint32_t>), grid, dim3(256), 0, ctx->stream, (uint32_t*)out, n, 0u);
+        else hipLaunchKernelGGL((fill_kernel<uint16_t>), grid, dim3(256), 0, ctx->stream, (uint16_t*)out, n, (uint16_t)0);
+        HIP_TRY(hipGetLastError());
+        return MDD_OK;
+    }
+    if (!offsets) {
+        MDD_FOR_TYPE(type, T, {
+            if (id_bytes == 4) launch_lookup<T, int32_t>(ctx->stream, (const T*)table, n_rows, row_stride, dim, (const int32_t*)ids, n_ids, scale, (T*)out);
+            else launch_lookup<T, int64_t>(ctx->stream, (const T*)table, n_rows, row_stride, dim, (const int64_t*)ids, n_ids, scale, (T*)out);
+        });
+        HIP_TRY(hipGetLastError());
+        return MDD_OK;
+    }
+    PoolArgs a = {table, n_rows, row_stride, dim, ids, n_ids, offsets, n_docs, mean, scale, nullptr, piece_log2_for(n_ids), n_pieces_for(n_ids), (float*)ws,
+                  nullptr, out};
+    if (a.n_pieces) a.part_n = reinterpret_cast<uint32_t*>((uint8_t*)ws + round_up(a.n_pieces * 2 * dim * 4, 256));
+    MDD_FOR_TYPE(type, T, {
+        if (id_bytes == 4) launch_pool<T, int32_t, T>(ctx->stream, a);
+        else launch_pool<T, int64_t, T>(ctx->stream, a);
+    });
+    HIP_TRY(hipGetLastError());
+    return MDD_OK;
+}
+
+static uint64_t backward_parts(uint64_t n_ids, uint64_t n_docs, uint64_t n_rows, uint32_t dim, uint64_t at[5]) {
+    uint64_t o = 0;
+    at[0] = o, o += (n_ids > SMALL_SORT ? 4 : 2) * round_up(n_ids * 4, 256);  // keys, values, and the sort's second pair
+    at[1] = o, o += round_up(sort_hist_words(n_ids) * 4, 256);
+    at[2] = o, o += round_up((n_rows + 1) * 8, 256);          // starts
+    at[3] = o, o += round_up(n_docs * 4, 256);                // ids per document
+    at[4] = o, o += pool_ws_bytes(n_ids, dim);                // shares of long rows
+    return o;
+}
+uint64_t mdd_embed_backward_ws_bytes(uint64_t n_ids, uint64_t n_docs, uint64_t n_rows, uint32_t dim) {
+    uint64_t at[5];
+    return backward_parts(n_ids, n_docs, n_rows, dim, at);
+}
+
+int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_stride, uint32_t dim, const void* ids, int id_bytes,
+                       uint64_t n_ids, const uint64_t* offsets, uint64_t n_docs, int mean, float scale, void* table_grad,
+                       int out_type, uint64_t n_rows, void* ws, uint64_t ws_bytes) {
+    const char* who = "mdd_embed_backward";
+    REQUIRE(ctx, "%s: ctx is NULL", who);
+    REQUIRE(dim >= 1 && dim <= MDD_VEC_MAX_DIM, "%s: dim=%u outside [1,%d]", who, dim, MDD_VEC_MAX_DIM);
+    REQUIRE(type_bytes(type), "%s: unknown element type %d", who, type);
+    REQUIRE(out_type == MDD_F32 || out_type == type, "%s: out_type %d is neither MDD_F32 nor the gradient's type", who, out_type);
+    REQUIRE(id_bytes == 4 || id_bytes == 8, "%s: id_bytes=%d is neither 4 nor 8", who, id_bytes);
+    REQUIRE(n_ids < (1ull << 31) && n_docs < (1ull << 31) && n_rows < (1ull << 31), "%s: 2^31 or more ids, documents or table rows", who);
+    if (n_rows == 0) return MDD_OK;
+    REQUIRE(table_grad && aligned_to(table_grad, type_bytes(out_type)), "%s: table_grad is NULL or not aligned to its elements", who);
+    REQUIRE(n_ids == 0 || (ids && aligned_to(ids, id_bytes)), "%s: ids is NULL or not aligned", who);
+    if (!offsets) n_docs = 0;
+    const uint64_t n_grad = offsets ? n_docs : n_ids;
+    if (n_grad) CHECKED(check_matrix(who, "grad", grad, type, grad_stride, dim));
+    uint64_t at[5];
+    const uint64_t need = n_ids && n_grad ? backward_parts(n_ids, n_docs, n_rows, dim, at) : 0;
+    REQUIRE(need == 0 || (ws && aligned_to(ws, 256) && ws_bytes >= need), "%s: workspace of %llu bytes, 256-byte aligned, needed", who,
+            (unsigned long long)need);
+    ON_DEVICE(ctx);
+    hipStream_t s = ctx->stream;
+    if (n_ids == 0 || n_grad == 0) {
+        const uint64_t n = n_rows * dim;
+        const dim3 grid((unsigned)(n / 256 + 1 < 4096 ? n / 256 + 1 : 4096));
+        if (out_type == MDD_F32) hipLaunchKernelGGL((fill_kernel<uint32_t>), grid, dim3(256), 0, s, (uint32_t*)table_grad, n, 0u);
+        else hipLaunchKernelGGL((fill_kernel<uint16_t>), grid, dim3(256), 0, s, (uint16_t*)table_grad, n, (uint16_t)0);
+        HIP_TRY(hipGetLastError());
+        return MDD_OK;
+    }
+    uint8_t* base = (uint8_t*)ws;
+    uint32_t *key = (uint32_t*)(base + at[0]), *val = key + round_up(n_ids, 64), *key2 = val + round_up(n_ids, 64), *val2 = key2 + round_up(n_ids, 64);
+    uint64_t* start = (uint64_t*)(base + at[2]);
+    uint32_t* count = mean && offsets ? (uint32_t*)(base + at[3]) : nullptr;
+    if (count) hipLaunchKernelGGL((fill_kernel<uint32_t>), dim3((unsigned)(n_docs / 256 + 1 < 4096 ? n_docs / 256 + 1 : 4096)), dim3(256), 0, s, count, n_docs, 0u);
+    const dim3 per_id(grid_for(n_ids, 256));
+    if (id_bytes == 4)
+        hipLaunchKernelGGL((grad_keys_kernel<int32_t>), per_id, dim3(256), 0, s, (const int32_t*)ids, n_ids, n_rows, offsets, n_docs, count, key, val);
+    else
+        hipLaunchKernelGGL((grad_keys_kernel<int64_t>), per_id, dim3(256), 0, s, (const int64_t*)ids, n_ids, n_rows, offsets, n_docs, count, key, val);
+    sort_pairs(s, key, val, key2, val2, n_ids, bits_of(n_rows), (uint32_t*)(base + at[1]));
+    hipLaunchKernelGGL(grad_starts_kernel, dim3(grid_for(n_rows + 1, 256)), dim3(256), 0, s, key, (uint32_t)n_ids, n_rows, start);
+    // the sums themselves are a lookup: table rows are the documents, the sorted positions their ids, grad the table
+    PoolArgs a = {grad, n_grad, grad_stride, dim, val, n_ids, start, n_rows, 0, scale, count, piece_log2_for(n_ids), n_pieces_for(n_ids),
+                  (float*)(base + at[4]), nullptr, table_grad};
+    if (a.n_pieces) a.part_n = reinterpret_cast<uint32_t*>(base + at[4] + round_up(a.n_pieces * 2 * dim * 4, 256));
+    MDD_FOR_TYPE(type, T, {
+        if (out_type == MDD_F32) launch_pool<T, int32_t, float>(s, a);
+        else launch_pool<T, int32_t, T>(s, a);
+    });
+    HIP_TRY(hipGetLastError());
+    return MDD_OK;
+}
+
+int mdd_rms_norm(mdd_ctx* ctx, const void* x, int type, uint64_t x_stride, const void* residual, uint64_t residual_stride,
+                 const void* weight, float eps, uint64_t n_rows, uint32_t dim, void* y, void* sum_out, float* rstd) {
+    const char* who = "mdd_rms_norm";
+    REQUIRE(ctx, "%s: ctx is NULL", who);
+    REQUIRE(dim >= 1 && dim <= MDD_VEC_MAX_DIM, "%s: dim=%u outside [1,%d]", who, dim, MDD_VEC_MAX_DIM);
+    REQUIRE(eps >= 0.0f, "%s: eps=%g is not a number >= 0", who, (double)eps);
+    REQUIRE(type_bytes(type), "%s: unknown element type %d", who, type);
+    if (n_rows == 0) return MDD_OK;
+    CHECKED(check_matrix(who, "x", x, type, x_stride, dim));
+    if (residual) CHECKED(check_matrix(who, "residual", residual, type, residual_stride, dim));
+    if (weight) CHECKED(check_matrix(who, "weight", weight, type, dim, dim));
+    CHECKED(check_matrix(who, "y", y, type, dim, dim));
+    REQUIRE(!sum_out || aligned_to(sum_out, type_bytes(type)), "%s: sum_out is not aligned to its elements", who);
+    REQUIRE(!rstd || aligned_to(rstd, 4), "%s: rstd is not aligned", who);
+    ON_DEVICE(ctx);
+    MDD_FOR_TYPE(type, T, {
+        for_width(dim, [&](auto nc, auto w) {
+            hipLaunchKernelGGL((norm_kernel<T, nc.value, w.value>), row_grid(n_rows, w.value), dim3(w.value == 16 ? 1024 : 256), 0, ctx->stream,
+                               (const T*)x, x_stride, (const T*)residual, residual_stride, (const T*)weight, eps, n_rows, dim, (T*)y, (T*)sum_out, rstd);
+        });
+    });
+    HIP_TRY(hipGetLastError());
+    return MDD_OK;
+}
+
+int mdd_rms_norm_q8(mdd_ctx* ctx, const void* x, int type, uint64_t x_stride, const void* residual, uint64_t residual_stride,
+                    const void* weight, float eps, uint64_t n_rows, uint32_t dim, int kind, void* codes, float* scales, void* sum_out) {
+    const char* who = "mdd_rms_norm_q8";
+    REQUIRE(ctx, "%s: ctx is NULL", who);
+    REQUIRE(dim >= 1 && dim <= MDD_VEC_MAX_DIM, "%s: dim=%u outside [1,%d]", who, dim, MDD_VEC_MAX_DIM);
+    REQUIRE(eps >= 0.0f, "%s: eps=%g is not a number >= 0", who, (double)eps);
+    REQUIRE(type_bytes(type), "%s: unknown element type %d", who, type);
+    REQUIRE(kind == MDD_I8 || kind == MDD_E4M3, "%s: unknown 8-bit kind %d", who, kind);
+    if (n_rows == 0) return MDD_OK;
+    CHECKED(check_matrix(who, "x", x, type, x_stride, dim));
+    if (residual) CHECKED(check_matrix(who, "residual", residual, type, residual_stride, dim));
+    if (weight) CHECKED(check_matrix(who, "weight", weight, type, dim, dim));
+    REQUIRE(codes && scales && aligned_to(scales, 4), "%s: NULL buffer, or scales not aligned", who);
+    REQUIRE(!sum_out || aligned_to(sum_out, type_bytes(type)), "%s: sum_out is not aligned to its elements", who);
+    ON_DEVICE(ctx);
+    MDD_FOR_TYPE(type, T, {
+        for_width(dim, [&](auto nc, auto w) {
+            auto kernel = kind == MDD_I8 ? norm_q8_kernel<T, nc.value, w.value, MDD_I8> : norm_q8_kernel<T, nc.value, w.value, MDD_E4M3>;
+            hipLaunchKernelGGL(kernel, row_grid(n_rows, w.value), dim3(w.value == 16 ? 1024 : 256), 0, ctx->stream, (const T*)x, x_stride,
+                               (const T*)residual, residual_stride, (const T*)weight, eps, n_rows, dim, (uint8_t*)codes, scales, (T*)sum_out);
+        });
+    });
+    HIP_TRY(hipGetLastError());
+    return MDD_OK;
+}
+
+uint64_t mdd_rms_norm_backward_ws_bytes(uint64_t n_rows, uint32_t dim) { return round_up((uint64_t)backward_blocks(n_rows, dim) * dim * 4, 256); }
+
+int mdd_rms_norm_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_stride, const void* h, uint64_t h_stride,
+                          const void* grad_sum, uint64_t grad_sum_stride, const void* weight, const float* rstd,
+                          uint64_t n_rows, uint32_t dim, void* x_grad, float* weight_grad, void* ws, uint64_t ws_bytes) {
+    const char* who = "mdd_rms_norm_backward";
+    REQUIRE(ctx, "%s: ctx is NULL", who);
+    REQUIRE(dim >= 1 && dim <= MDD_VEC_MAX_DIM, "%s: dim=%u outside [1,%d]", who, dim, MDD_VEC_MAX_DIM);
+    REQUIRE(type_bytes(type), "%s: unknown element type %d", who, type);
+    REQUIRE(!weight_grad || aligned_to(weight_grad, 4), "%s: weight_grad is not aligned", who);
+    if (n_rows) {
+        CHECKED(check_matrix(who, "grad", grad, type, grad_stride, dim));
+        CHECKED(check_matrix(who, "h", h, type, h_stride, dim));
+        if (grad_sum) CHECKED(check_matrix(who, "grad_sum", grad_sum, type, grad_sum_stride, dim));
+        if (weight) CHECKED(check_matrix(who, "weight", weight, type, dim, dim));
+        CHECKED(check_matrix(who, "x_grad", x_grad, type, dim, dim));
+        REQUIRE(rstd && aligned_to(rstd, 4), "%s: rstd is NULL or not aligned", who);
+    }
+    const uint32_t blocks = backward_blocks(n_rows, dim);
+    const uint64_t need = mdd_rms_norm_backward_ws_bytes(n_rows, dim);
+    REQUIRE(!weight_grad || n_rows == 0 || (ws && aligned_to(ws, 256) && ws_bytes >= need), "%s: workspace of %llu bytes, 256-byte aligned, needed", who,
+            (unsigned long long)need);
+    ON_DEVICE(ctx);
+    if (n_rows == 0) {
+        if (weight_grad) hipLaunchKernelGGL((fill_kernel<float>), dim3((dim + 255) / 256), dim3(256), 0, ctx->stream, weight_grad, (uint64_t)dim, 0.0f);
+        HIP_TRY(hipGetLastError());
+        return MDD_OK;
+    }
+    float* part = weight_grad ? (float*)ws : nullptr;
+    MDD_FOR_TYPE(type, T, {
+        for_width(dim, [&](auto nc, auto w) {
+            hipLaunchKernelGGL((norm_backward_kernel<T, nc.value, w.value>), dim3(blocks), dim3(w.value == 16 ? 1024 : 256), 0, ctx->stream, (const T*)grad,
+                               grad_stride, (const T*)h, h_stride, (const T*)grad_sum, grad_sum_stride, (const T*)weight, rstd, n_rows, dim, (T*)x_grad, part);
+        });
+    });
+    if (weight_grad)
+        hipLaunchKernelGGL(weight_grad_kernel, dim3((dim + 63) / 64), dim3(1024), 0, ctx->stream, part, blocks, dim, weight_grad);
+    HIP_TRY(hipGetLastError());
+    return MDD_OK;
+}
+
+int mdd_edge_cosines(mdd_ctx* ctx, const void* codes, int kind, uint64_t row_stride, uint64_t n_rows, uint32_t dim,
+                     const uint32_t* edge_u, const uint32_t* edge_v, uint64_t n_edges, float* cosines) {
+    const char* who = "mdd_edge_cosines";
+    REQUIRE(ctx, "%s: ctx is NULL", who);
+    REQUIRE(kind == MDD_I8 || kind == MDD_E4M3, "%s: unknown 8-bit kind %d", who, kind);
+    REQUIRE(dim >= 1 && dim <= MDD_VEC_MAX_DIM, "%s: dim=%u outside [1,%d]", who, dim, MDD_VEC_MAX_DIM);
+    REQUIRE(row_stride >= dim, "%s: row stride below dim", who);
+    if (n_edges == 0) return MDD_OK;
+    REQUIRE((codes || n_rows == 0) && edge_u && edge_v && cosines, "%s: NULL buffer", who);
+    ON_DEVICE(ctx);
+    const uint64_t want = (n_edges + 15) / 16, cap = (uint64_t)ctx->cus * 64;
+    auto kernel = kind == MDD_I8 ? edge_cosine_kernel<MDD_I8> : edge_cosine_kernel<MDD_E4M3>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(want < cap ? want : cap)), dim3(256), 0, ctx->stream, (const uint8_t*)codes, row_stride, n_rows, dim, edge_u,
+                       edge_v, n_edges, cosines);
+    HIP_TRY(hipGetLastError());
+    return MDD_OK;
+}
+
+uint64_t mdd_sort_edges_ws_bytes(uint64_t n_edges) {
+    return n_edges <= SMALL_SORT ? 0 : 2 * round_up(n_edges * 4, 256) + round_up(sort_hist_words(n_edges) * 4, 256);
+}
+
+int mdd_sort_edges(mdd_ctx* ctx, uint32_t* edge_u, uint32_t* edge_v, uint64_t n_edges, uint64_t n_docs, void* ws, uint64_t ws_bytes) {
+    const char* who = "mdd_sort_edges";
+    REQUIRE(ctx, "%s: ctx is NULL", who);
+    REQUIRE(n_edges < (1ull << 31) && n_docs <= 0xFFFFFFFFull, "%s: 2^31 or more edges, or 2^32 or more documents", who);
+    if (n_edges <= 1) return MDD_OK;
+    REQUIRE(edge_u && edge_v, "%s: NULL buffer", who);
+    const uint64_t need = mdd_sort_edges_ws_bytes(n_edges);
+    REQUIRE(need == 0 || (ws && aligned_to(ws, 256) && ws_bytes >= need), "%s: workspace of %llu bytes, 256-byte aligned, needed", who,
+            (unsigned long long)need);
+    ON_DEVICE(ctx);
+    const int bits = bits_of(n_docs ? n_docs - 1 : 0);
+    uint32_t *u = edge_u, *v = edge_v, *v2 = (uint32_t*)ws, *u2 = v2 + round_up(n_edges, 64), *hist = u2 + round_up(n_edges, 64);
+    // by the second column, then stably by the first; the passes of both together are even in number, so the result ends up
+    // in the caller's arrays
+    sort_pairs(ctx->stream, v, u, v2, u2, n_edges, bits, hist);
+    sort_pairs(ctx->stream, u, v, u2, v2, n_edges, bits, hist);
+    HIP_TRY(hipGetLastError());
+    return MDD_OK;
+}
+
+}  // extern "C"

@@ -11,7 +11,7 @@ SO_PATH = os.path.join(_HERE, "libmdd_hip.so")
 MDD_UNIT = {"char": 0, "word": 1}
 
 # name -> (restype, argtypes); the single source the loader and the symbol test share
-_vp, _u64, _int, _u32 = C.c_void_p, C.c_uint64, C.c_int, C.c_uint32
+_vp, _u64, _int, _u32, _f32 = C.c_void_p, C.c_uint64, C.c_int, C.c_uint32, C.c_float
 SIGNATURES = {
     "mdd_version": (_int, []),
     "mdd_last_error": (C.c_char_p, []),
@@ -65,6 +65,21 @@ SIGNATURES = {
     "mdd_jsonl_line_begins": (_int, [_vp, _vp, _u64, _vp, _vp, _u64]),
     "mdd_jsonl_scan": (_int, [_vp, _vp, _u64, _vp, _u64, C.c_char_p, C.c_char_p, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mdd_jsonl_decode": (_int, [_vp, _vp, _u64, _u64, _vp, _vp, _vp, _vp, _u64]),
+    "mdd_embed_ws_bytes": (_u64, [_u64, _u32]),
+    "mdd_embed": (_int, [_vp, _vp, _int, _u64, _u64, _u32, _vp, _int, _u64, _vp, _u64, _int, _f32, _vp, _vp, _u64]),
+    "mdd_embed_backward_ws_bytes": (_u64, [_u64, _u64, _u64, _u32]),
+    "mdd_embed_backward": (_int, [_vp, _vp, _int, _u64, _u32, _vp, _int, _u64, _vp, _u64, _int, _f32, _vp, _int, _u64, _vp, _u64]),
+    "mdd_rms_norm": (_int, [_vp, _vp, _int, _u64, _vp, _u64, _vp, _f32, _u64, _u32, _vp, _vp, _vp]),
+    "mdd_rms_norm_q8": (_int, [_vp, _vp, _int, _u64, _vp, _u64, _vp, _f32, _u64, _u32, _int, _vp, _vp, _vp]),
+    "mdd_rms_norm_backward_ws_bytes": (_u64, [_u64, _u32]),
+    "mdd_rms_norm_backward": (_int, [_vp, _vp, _int, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _u64, _u32, _vp, _vp, _vp, _u64]),
+    "mdd_edge_cosines": (_int, [_vp, _vp, _int, _u64, _u64, _u32, _vp, _vp, _u64, _vp]),
+    "mdd_sort_edges_ws_bytes": (_u64, [_u64]),
+    "mdd_sort_edges": (_int, [_vp, _vp, _vp, _u64, _u64, _vp, _u64]),
+    "mdd_mx_quantize": (_int, [_vp, _vp, _int, _u64, _u64, _u32, _vp, _vp]),
+    "mdd_mx_matmul": (_int, [_vp, _vp, _vp, _u64, _vp, _vp, _u64, _u32, _f32, _vp, _int, _u64]),
+    "mdd_mx_pairs_ws_bytes": (_u64, [_u64]),
+    "mdd_mx_pairs": (_int, [_vp, _vp, _vp, _u64, _u32, _f32, _vp, _vp, _u64, _vp, _vp, _u64]),
     "mdd_valu_calibrate": (_int, [_vp, _int, C.POINTER(C.c_double)]),
 }
 

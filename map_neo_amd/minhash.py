@@ -20,6 +20,7 @@ import numpy as np
 import torch
 
 from . import lib as _lib
+from .vectors import MxMatrix, VectorOps  # noqa: F401
 
 # reference constants (EN:17-20, ZH-1:14-17)
 WIDTH = 13
@@ -95,8 +96,8 @@ def _ptr(t: Optional[torch.Tensor]):
     return C.c_void_p(t.data_ptr()) if t is not None and t.numel() > 0 else C.c_void_p(0)
 
 
-class Engine:
-    """One context = one (GPU, stream).  Not thread-safe; one per rank."""
+class Engine(VectorOps):
+    """One context = one (GPU, stream).  Not thread-safe; one per rank.  The document-vector methods are in vectors.VectorOps."""
 
     def __init__(self, device: Optional[int] = None):
         self.L = _lib.load()
