@@ -527,7 +527,9 @@ int mdd_sort_edges(mdd_ctx* ctx, uint32_t* edge_u, uint32_t* edge_v, uint64_t n_
  *   matmul   c [m, n] (MDD_F32 or MDD_BF16, c_stride) = alpha * A * B^T,  A [m, dim], B [n, dim] packed
  *   pairs    every u > v with cos(A_u, A_v) >= min_cosine (0 < min_cosine <= 1; cosine of the 4-bit values), appended to edge_u /
  *            edge_v in no fixed order, at most edge_cap of them; *n_edges (device u64, set by the call) counts all of them.
- *            Rows of zeros and rows with a NaN have no pairs.  m < 2^31. */
+ *            Rows of zeros and rows with a NaN have no pairs.  Rows of similar length are fastest.  m <= MDD_MX_MAX_PAIR_ROWS
+ *            (2^22: 10^13 pairs; larger sets are compared block by block with matmul). */
+#define MDD_MX_MAX_PAIR_ROWS 4194304
 #define MDD_MX_TILE_ROWS 32
 #define MDD_MX_TILE_COLS 128
 #define MDD_MX_CODE_BYTES(rows, dim) ((((uint64_t)(rows) + 31) / 32) * (((uint64_t)(dim) + 127) / 128) * 2048)

@@ -166,147 +166,269 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(const uint8_t* __restric
     }
 }
 
-// Tiled product.  A block of WR x WC waves computes (WR * FM * 32) x (WC * FN * 32) of C.  Column tiles (128 columns) go from
-// memory straight into LDS, three in rotation: while one is multiplied, the next is complete or landing and the one after is
-// requested, so a load has two steps to arrive and a step needs one barrier (behind it every wave is done with the buffer
-// that is requested next).
-template <int WR, int WC, int FM, int FN>
+// Tiled product.  A block of WR x WC waves computes (WR * FM * 32) x (WC * FN * 32) of C and walks a list of such tiles.  Column
+// tiles (128 columns: a step) go from memory straight into LDS, three buffers in rotation, in one stream of steps that runs
+// on across the tiles of the list: while a tile's results leave, the next tile's first steps are landing.  A step is two
+// halves of 64 columns.  The fragments of a half are read from LDS while the half before is multiplied:
+//     read half 1 of step s                                   | multiply half 0 of step s
+//     wait for step s + 1, barrier, request step s + 3 into the buffer of step s
+//     read half 0 of step s + 1                               | multiply half 1 of step s
+// so a load has two steps to arrive, a step needs one barrier, and neither LDS nor memory latency stands before the matrix
+// unit.
+template <int WR_, int WC_, int FM_, int FN_>
 struct Block {
+    static constexpr int WR = WR_, WC = WC_, FM = FM_, FN = FN_;
     static constexpr int WAVES = WR * WC, TA = WR * FM, TB = WC * FN, TILES = TA + TB, PER_WAVE = TILES / WAVES;
-    static constexpr uint32_t STAGE = TILES * (TILE + STILE), LDS = 3 * STAGE;
+    static constexpr uint32_t STAGE = TILES * (TILE + STILE), LDS = 3 * STAGE, OUT = 4096;  // OUT: a wave's room to turn results round
     static constexpr int LOADS = PER_WAVE * 2 + 1;  // per wave and step: two halves of each of its tiles, and their scales
     static_assert(TILES % WAVES == 0 && PER_WAVE * 8 <= 64, "every wave loads whole tiles, their scales in one instruction");
 };
+using Big = Block<4, 2, 2, 4>;    // 256 x 256, 8 waves, one block a CU
+using Small = Block<2, 2, 2, 2>;  // 128 x 128, 4 waves, two blocks a CU
 
 __device__ __forceinline__ void to_lds(const uint8_t* g, uint8_t* l) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g, (__attribute__((address_space(3))) uint32_t*)l, 16, 0, 0);
 }
+// Waits by the builtin, not by a statement in assembly: the compiler then knows that nothing before is left to wait for.
+// (vmcnt bits 0-3 and 14-15, expcnt 4-6, lgkmcnt 8-11)
+template <int N>
+__device__ __forceinline__ void wait_memory() {  // at most N of this wave's memory operations outstanding
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0xF70);
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_lds() {  // this wave's LDS reads done
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+}
 
-template <int WR, int WC, int FM, int FN>
-__device__ __forceinline__ void mx_tile(const uint8_t* __restrict__ ac, const uint8_t* __restrict__ as, uint64_t a0, uint64_t a_tiles,
-                                        const uint8_t* __restrict__ bc, const uint8_t* __restrict__ bs, uint64_t b0, uint64_t b_tiles,
-                                        uint32_t col_tiles, uint8_t* lds, f32x16 (&acc)[FM][FN]) {
-    using B = Block<WR, WC, FM, FN>;
-    const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave / WC, wc = wave % WC;
-    // this wave's share of a step's loads: PER_WAVE tiles; row tiles past the end repeat the last one (their results are not used)
-    const uint8_t* src[B::PER_WAVE];
-#pragma unroll
-    for (int i = 0; i < B::PER_WAVE; i++) {
-        const uint32_t t = wave * B::PER_WAVE + i;
-        const bool is_a = t < B::TA;
-        uint64_t rt = is_a ? a0 + t : b0 + t - B::TA;
-        const uint64_t last = (is_a ? a_tiles : b_tiles) - 1;
-        rt = rt < last ? rt : last;
-        src[i] = (is_a ? ac : bc) + rt * col_tiles * TILE + lane * 16;
-    }
-    const uint8_t* ssrc;
-    {
-        const uint32_t t = wave * B::PER_WAVE + (lane / 8 < B::PER_WAVE ? lane / 8 : 0);
-        const bool is_a = t < B::TA;
-        uint64_t rt = is_a ? a0 + t : b0 + t - B::TA;
-        const uint64_t last = (is_a ? a_tiles : b_tiles) - 1;
-        rt = rt < last ? rt : last;
-        ssrc = (is_a ? as : bs) + rt * col_tiles * STILE + lane % 8 * 16;
-    }
-    auto request = [&](uint32_t k, uint32_t buf) {
-        uint8_t* to = lds + buf * B::STAGE;
-#pragma unroll
-        for (int i = 0; i < B::PER_WAVE; i++) {
-            uint8_t* l = to + (wave * B::PER_WAVE + i) * TILE;
-            to_lds(src[i] + (uint64_t)k * TILE, l);
-            to_lds(src[i] + (uint64_t)k * TILE + 1024, l + 1024);
-        }
-        if (lane < B::PER_WAVE * 8) to_lds(ssrc + (uint64_t)k * STILE, to + B::TILES * TILE + wave * B::PER_WAVE * STILE);
-    };
+// The compiler would move a half's products down behind the barrier, next to their use in the other half's; an empty
+// statement that takes the results keeps them before it, where they cover the LDS reads and the wait.
+template <int FM, int FN>
+__device__ __forceinline__ void keep_here(f32x16 (&acc)[FM][FN]) {
 #pragma unroll
     for (int i = 0; i < FM; i++)
 #pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = 0.0f;
-    request(0, 0);
-    if (col_tiles > 1) request(1, 1);
-    uint32_t buf = 0;
-#pragma unroll 1
-    for (uint32_t k = 0; k < col_tiles; k++) {
-        // the loads of step k are in LDS once at most those of step k + 1 are outstanding; and this wave has read all that
-        // it wants of the buffer of step k - 1, which is requested anew behind the barrier
-        if (k + 1 < col_tiles) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(B::LOADS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        if (k + 2 < col_tiles) request(k + 2, buf == 0 ? 2 : buf - 1);
-        const uint8_t *la = lds + buf * B::STAGE + (wr * FM) * TILE, *lb = lds + buf * B::STAGE + (B::TA + wc * FN) * TILE;
-        const uint8_t *sa = lds + buf * B::STAGE + B::TILES * TILE + (wr * FM) * STILE, *sb = lds + buf * B::STAGE + B::TILES * TILE + (B::TA + wc * FN) * STILE;
-        int xa[FM], xb[FN];
+        for (int j = 0; j < FN; j++) asm volatile("" : "+v"(acc[i][j]));
+}
+
+struct Packed {
+    const uint8_t *codes, *scales;
+    uint32_t tiles;  // row tiles
+};
+struct Place {
+    uint32_t i0, j0;  // first row tile of A and of B; the same in every lane
+    bool valid;
+};
+__device__ __forceinline__ Place place_at(uint32_t i0, uint32_t j0) { return {(uint32_t)__builtin_amdgcn_readfirstlane(i0), (uint32_t)__builtin_amdgcn_readfirstlane(j0), true}; }
+constexpr uint64_t MAX_TILES = 1ull << 31;  // of a list
+
+// next(cursor) is the block's next tile, from cursor 0 on (valid = false: the list is done).  finish(place, acc) takes a tile's
+// results; it returns whether it has issued at least STORES memory operations.
+template <typename B, int STORES, typename F, typename G>
+__device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32_t col_tiles, uint8_t* lds, F&& next, G&& finish) {
+    constexpr int FM = B::FM, FN = B::FN;
+    const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave / B::WC, wc = wave % B::WC;
+    uint32_t req_cursor = 0, cursor = 0;
+    Place req = next(req_cursor), cur = next(cursor);
+    if (!cur.valid) return;
+    uint32_t req_k = 0, req_buf = 0;
+    const uint8_t *src[B::PER_WAVE], *ssrc;
+    auto aim = [&]() {  // this wave's share: PER_WAVE row tiles.  Tiles past the end repeat the last one; their results are not used
+        auto at = [&](uint32_t t, const uint8_t* pa, const uint8_t* pb, uint32_t bytes) {
+            const bool is_a = t < (uint32_t)B::TA;
+            const uint32_t rt = is_a ? req.i0 + t : req.j0 + t - B::TA, last = (is_a ? a.tiles : b.tiles) - 1;
+            return (is_a ? pa : pb) + (uint64_t)(rt < last ? rt : last) * col_tiles * bytes;
+        };
 #pragma unroll
-        for (int i = 0; i < FM; i++) xa[i] = *reinterpret_cast<const uint16_t*>(sa + i * STILE + lane * 2);
+        for (int i = 0; i < B::PER_WAVE; i++) src[i] = at(wave * B::PER_WAVE + i, a.codes, b.codes, TILE);
+        ssrc = at(wave * B::PER_WAVE + (lane / 8 < B::PER_WAVE ? lane / 8 : 0), a.scales, b.scales, STILE) + lane % 8 * 16;
+    };
+    aim();
+    auto request = [&]() -> bool {  // the stream's next step; false when the list is done
+        if (!req.valid) return false;
+        uint8_t* to = lds + req_buf * B::STAGE;
 #pragma unroll
-        for (int j = 0; j < FN; j++) xb[j] = *reinterpret_cast<const uint16_t*>(sb + j * STILE + lane * 2);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            i32x4 a[FM], b[FN];
-#pragma unroll
-            for (int i = 0; i < FM; i++) a[i] = *reinterpret_cast<const i32x4*>(la + i * TILE + h * 1024 + lane * 16);
-#pragma unroll
-            for (int j = 0; j < FN; j++) b[j] = *reinterpret_cast<const i32x4*>(lb + j * TILE + h * 1024 + lane * 16);
-#pragma unroll
-            for (int i = 0; i < FM; i++)
-#pragma unroll
-                for (int j = 0; j < FN; j++) acc[i][j] = mma(b[j], xb[j], a[i], xa[i], acc[i][j], h);
+        for (int i = 0; i < B::PER_WAVE; i++) {
+            uint8_t* l = to + (wave * B::PER_WAVE + i) * TILE;
+            const uint8_t* g = src[i] + (uint64_t)req_k * TILE;
+            to_lds(g + lane * 16, l);
+            to_lds(g + 1024 + lane * 16, l + 1024);
         }
-        buf = buf == 2 ? 0 : buf + 1;
+        if (lane < B::PER_WAVE * 8) to_lds(ssrc + (uint64_t)req_k * STILE, to + B::TILES * TILE + wave * B::PER_WAVE * STILE);
+        req_buf = req_buf == 2 ? 0 : req_buf + 1;
+        if (++req_k == col_tiles) {
+            req_k = 0;
+            req = next(req_cursor);
+            if (req.valid) aim();
+        }
+        return true;
+    };
+    i32x4 fa[2][FM], fb[2][FN];
+    int xa[FM], xb[FN], ya[FM], yb[FN];  // a step's scales, both halves in one register; the next step's
+    auto read_half = [&](uint32_t buf, int h) {
+        const uint8_t* l = lds + buf * B::STAGE + h * 1024 + lane * 16;
+#pragma unroll
+        for (int i = 0; i < FM; i++) fa[h][i] = *reinterpret_cast<const i32x4*>(l + (wr * FM + i) * TILE);
+#pragma unroll
+        for (int j = 0; j < FN; j++) fb[h][j] = *reinterpret_cast<const i32x4*>(l + (B::TA + wc * FN + j) * TILE);
+    };
+    auto read_scales = [&](uint32_t buf) {
+        const uint8_t* s = lds + buf * B::STAGE + B::TILES * TILE + lane * 2;
+#pragma unroll
+        for (int i = 0; i < FM; i++) ya[i] = *reinterpret_cast<const uint16_t*>(s + (wr * FM + i) * STILE);
+#pragma unroll
+        for (int j = 0; j < FN; j++) yb[j] = *reinterpret_cast<const uint16_t*>(s + (B::TA + wc * FN + j) * STILE);
+    };
+    f32x16 acc[FM][FN];
+    auto multiply = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) acc[i][j] = mma(fb[h][j], xb[j], fa[h][i], xa[i], acc[i][j], h);
+    };
+    auto take_scales = [&]() {
+#pragma unroll
+        for (int i = 0; i < FM; i++) xa[i] = ya[i];
+#pragma unroll
+        for (int j = 0; j < FN; j++) xb[j] = yb[j];
+    };
+
+    int ahead = -1;  // steps requested behind the current one
+#pragma unroll 1
+    for (int r = 0; r < 3; r++) ahead += request() ? 1 : 0;
+    wait_memory<0>();
+    __builtin_amdgcn_s_barrier();
+    uint32_t buf = 0;
+    read_scales(0);
+    read_half(0, 0);
+    take_scales();
+    int behind = 0;  // steps for which finish's operations are younger than the loads waited for
+    while (cur.valid) {
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) acc[i][j] = 0.0f;
+        wait_lds();
+#pragma unroll 1
+        for (uint32_t k = 0; k < col_tiles; k++) {
+            read_half(buf, 1);
+            __builtin_amdgcn_sched_barrier(0);  // reads first: they take as long as the products that follow
+            multiply(0);
+            keep_here(acc);
+            // step s + 1 has landed when only younger operations are left: the loads of step s + 2, and for two steps after a
+            // tile the stores of its results.  And this wave has read all it wants of the buffer of step s, which is requested
+            // anew behind the barrier.
+            wait_lds();
+            if (ahead <= 1) wait_memory<0>();
+            else if (behind > 0) wait_memory<B::LOADS + STORES>();
+            else wait_memory<B::LOADS>();
+            __builtin_amdgcn_s_barrier();
+            if (!request()) ahead--;
+            behind--;
+            buf = buf == 2 ? 0 : buf + 1;
+            read_scales(buf);  // behind the last step: whatever the buffer holds, not used
+            read_half(buf, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(1);
+            keep_here(acc);
+            __builtin_amdgcn_sched_barrier(0);  // the reads have had the products' time to arrive
+            take_scales();
+        }
+        behind = finish(cur, acc) ? 2 : 0;
+        cur = next(cursor);
     }
-    __syncthreads();  // the next tile's first loads go into buffers that a slower wave may still be reading
 }
 
 // Work order.  Blocks go to the eight XCDs in turn, so XCD x gets a run of consecutive tiles of the list, and the list walks
-// eight row tiles at a time down the columns: the 32 blocks that an XCD runs together share 8 + 4 tiles out of its L2.
-__device__ __forceinline__ uint64_t xcd_order(uint64_t b, uint64_t n) {
-    const uint64_t per = n / 8;  // the last n % 8 keep their place
+// eight block rows at a time down the columns: the 32 blocks that an XCD runs together share 8 + 4 tiles out of its L2.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t n) {
+    const uint32_t per = n / 8;  // the last n % 8 keep their place
     return b < per * 8 ? (b % 8) * per + b / 8 : b;
 }
+// position in the list of this block's round that begins at `first`; `total` when there is none
+__device__ __forceinline__ uint32_t list_place(uint32_t first, uint32_t total) {
+    if (first >= total || blockIdx.x >= total - first) return total;
+    return first + xcd_order(blockIdx.x, total - first < gridDim.x ? total - first : gridDim.x);
+}
 
-template <typename O, int WR, int WC, int FM, int FN>
-__global__ __launch_bounds__(WR * WC * 64) void mx_matmul_kernel(const uint8_t* __restrict__ ac, const uint8_t* __restrict__ as, uint64_t m, uint64_t a_tiles,
-                                                                 const uint8_t* __restrict__ bc, const uint8_t* __restrict__ bs, uint64_t n,
-                                                                 uint64_t b_tiles, uint32_t col_tiles, float alpha, O* __restrict__ c, uint64_t cs) {
-    using B = Block<WR, WC, FM, FN>;
+// Results leave through LDS: a lane holds four neighbouring columns of one row, which alone would be 32 rows of 16 bytes per
+// store; turned round in 4 KB of LDS (32 rows x 128 bytes, 16-byte pieces exchanged by row against bank conflicts) eight lanes
+// write 128 bytes of a row.
+template <typename O, typename B>
+__global__ __launch_bounds__(B::WAVES * 64) void mx_matmul_kernel(const Packed a, uint64_t m, const Packed b, uint64_t n, uint32_t col_tiles, float alpha,
+                                                                  O* __restrict__ c, uint64_t cs) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    const uint64_t gm = (a_tiles + B::TA - 1) / B::TA, gn = (b_tiles + B::TB - 1) / B::TB, total = gm * gn;
-    for (uint64_t t = blockIdx.x; t < total; t += gridDim.x) {
-        const uint64_t first = t - blockIdx.x, here = total - first < gridDim.x ? total - first : gridDim.x;
-        const uint64_t l = first + xcd_order(blockIdx.x, here);
-        const uint64_t band = l / (8 * gn), rows = gm - band * 8 < 8 ? gm - band * 8 : 8, in = l - band * 8 * gn;
-        const uint64_t i0 = (band * 8 + in % rows) * B::TA, j0 = in / rows * B::TB;
-        f32x16 acc[FM][FN];
-        mx_tile<WR, WC, FM, FN>(ac, as, i0, a_tiles, bc, bs, j0, b_tiles, col_tiles, lds, acc);
-        const uint32_t lane = lane_id(), wave = threadIdx.x / 64, wr = wave / WC, wc = wave % WC;
+    constexpr int JO = 4 / sizeof(O);  // column tiles turned round together: 128 bytes of a row
+    constexpr int STORES = B::FM * B::FN / JO * 4;
+    static_assert(B::LOADS + STORES <= 63, "the wait counter holds six bits");
+    const uint32_t gm = (a.tiles + B::TA - 1) / B::TA, gn = (b.tiles + B::TB - 1) / B::TB, total = gm * gn;
+    auto next = [&](uint32_t& cursor) -> Place {
+        const uint32_t l = list_place(cursor, total);
+        cursor += gridDim.x;  // total and the grid are below 2^31: no wrap
+        if (l >= total) return {0, 0, false};
+        const uint32_t band = l / (8 * gn), rows = gm - band * 8 < 8 ? gm - band * 8 : 8, in = l - band * 8 * gn, col = in / rows;
+        return place_at((band * 8 + in - col * rows) * B::TA, col * B::TB);
+    };
+    auto finish = [&](const Place& t, f32x16 (&acc)[B::FM][B::FN]) -> bool {
+        typedef O piece __attribute__((ext_vector_type(16 / sizeof(O))));
+        typedef O piece_any __attribute__((ext_vector_type(16 / sizeof(O)), aligned(sizeof(O))));
+        typedef O quad __attribute__((ext_vector_type(4)));
+        constexpr uint32_t PE = 16 / sizeof(O);
+        const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave / B::WC, wc = wave % B::WC, r = lane % 32;
+        uint8_t* turn = lds + B::LDS + wave * B::OUT;
+        const bool inside = (uint64_t)(t.i0 + B::TA) * 32 <= m && (uint64_t)(t.j0 + B::TB) * 32 <= n;
 #pragma unroll
-        for (int i = 0; i < FM; i++) {
-            const uint64_t row = (i0 + wr * FM + i) * 32 + lane % 32;
-            if (row >= m) continue;
+        for (int i = 0; i < B::FM; i++)
 #pragma unroll
-            for (int j = 0; j < FN; j++)
+            for (int j0 = 0; j0 < B::FN; j0 += JO) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const uint64_t col = (j0 + wc * FN + j) * 32 + q * 8 + lane / 32 * 4;
-                    if (col < n)
-                        store_quad<O>(c + row * cs + col, (uint32_t)(n - col < 4 ? n - col : 4), alpha * acc[i][j][q * 4], alpha * acc[i][j][q * 4 + 1],
-                                      alpha * acc[i][j][q * 4 + 2], alpha * acc[i][j][q * 4 + 3]);
+                for (int j = 0; j < JO; j++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const f32x16& v = acc[i][j0 + j];
+                        const quad o = {(O)(alpha * v[q * 4]), (O)(alpha * v[q * 4 + 1]), (O)(alpha * v[q * 4 + 2]), (O)(alpha * v[q * 4 + 3])};
+                        const uint32_t byte = (j * 32 + q * 8 + lane / 32 * 4) * sizeof(O);
+                        *reinterpret_cast<quad*>(turn + r * 128 + ((byte / 16 ^ (r & 7)) * 16 | byte % 16)) = o;
+                    }
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const uint32_t rr = s * 8 + lane / 8, cc = lane % 8;
+                    const piece o = *reinterpret_cast<const piece*>(turn + rr * 128 + (cc ^ (rr & 7)) * 16);
+                    const uint64_t row = (uint64_t)(t.i0 + wr * B::FM + i) * 32 + rr, col = (uint64_t)(t.j0 + wc * B::FN + j0) * 32 + cc * PE;
+                    O* to = c + row * cs + col;
+                    if (inside) {
+                        *reinterpret_cast<piece_any*>(to) = o;
+                    } else if (row < m && col < n) {
+                        if (n - col >= PE) {
+                            *reinterpret_cast<piece_any*>(to) = o;
+                        } else {
+#pragma unroll
+                            for (uint32_t k = 0; k < PE; k++)
+                                if (col + k < n) to[k] = o[k];
+                        }
+                    }
                 }
-        }
-    }
+            }
+        return inside;
+    };
+    mx_stream<B, STORES>(a, b, col_tiles, lds, next, finish);
 }
 
 // ------------------------------------------------------------------------------------------------ near pairs
-// Length of every row of 4-bit values.  The magnitudes (doubled: 0 1 2 3 4 6 8 12) are looked up four at a time with a byte
-// permute and squared with a byte dot product: a block of 32 columns is summed in whole numbers.  A row of zeros gets an
-// infinite length, which no product reaches.
+// Length of every row of 4-bit values, and the least of every row tile.  The magnitudes (doubled: 0 1 2 3 4 6 8 12) are looked
+// up four at a time with a byte permute and squared with a byte dot product: a block of 32 columns is summed in whole
+// numbers.  A row of zeros gets an infinite length, which no product reaches.
 __global__ __launch_bounds__(128) void mx_length_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t col_tiles,
-                                                        uint64_t row_tiles, float* __restrict__ length, unsigned long long* n_edges) {
+                                                        uint64_t row_tiles, float* __restrict__ length, float* __restrict__ least,
+                                                        unsigned long long* n_edges) {
     __shared__ float lds[4][32];
     const uint32_t kb = threadIdx.x / 32, r = threadIdx.x % 32;
     if (blockIdx.x == 0 && threadIdx.x == 0) *n_edges = 0;
     for (uint64_t rt = blockIdx.x; rt < row_tiles; rt += gridDim.x) {
         float s = 0;
+#pragma unroll 4
         for (uint32_t ct = 0; ct < col_tiles; ct++) {
             const uint64_t tile = rt * col_tiles + ct;
             const u32x4 p = *reinterpret_cast<const u32x4*>(codes + tile * TILE + kb * 512 + r * 16);
@@ -325,52 +447,61 @@ __global__ __launch_bounds__(128) void mx_length_kernel(const uint8_t* __restric
         __syncthreads();
         if (kb == 0) {
             s = lds[0][r] + lds[1][r] + lds[2][r] + lds[3][r];
-            length[rt * 32 + r] = s == 0.0f ? __builtin_inff() : sqrtf(s);
+            s = s == 0.0f ? __builtin_inff() : sqrtf(s);
+            length[rt * 32 + r] = s;
+            float low = s == s ? s : __builtin_inff();
+#pragma unroll
+            for (int d = 16; d; d >>= 1) low = fminf(low, __shfl_xor(low, d, 64));
+            if (r == 0) least[rt] = low;
         }
         __syncthreads();
     }
 }
 
-// The product of a matrix with itself, lower triangle only; instead of storing C a lane compares each element with
-// min_cosine times the two lengths and appends the pairs that reach it.  Pairs are rare, so the append may cost: one atomic
-// per element position and wave that holds any.  C (n^2 numbers) is never written.
-template <int WR, int WC, int FM, int FN>
-__global__ __launch_bounds__(WR * WC * 64) void mx_pairs_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint64_t n,
-                                                                uint64_t row_tiles, uint32_t col_tiles, const float* __restrict__ length, float min_cosine,
-                                                                uint32_t* __restrict__ eu, uint32_t* __restrict__ ev, uint64_t cap,
-                                                                unsigned long long* __restrict__ n_edges) {
-    using B = Block<WR, WC, FM, FN>;
+// The product of a matrix with itself, lower triangle only; C (n^2 numbers) is never written.  A wave first compares the largest
+// element of each 32 x 32 piece with min_cosine times the least lengths of its rows and columns, half an instruction per
+// element; where that is reached (near pairs are rare, and so is it unless lengths differ much inside a row tile) each
+// element is compared with its own two lengths, and the pairs are appended with one atomic per element position and wave.
+template <typename B>
+__global__ __launch_bounds__(B::WAVES * 64) void mx_pairs_kernel(const Packed a, uint64_t n, uint32_t col_tiles, const float* __restrict__ length,
+                                                                 const float* __restrict__ least, float min_cosine, uint32_t* __restrict__ eu,
+                                                                 uint32_t* __restrict__ ev, uint64_t cap, unsigned long long* __restrict__ n_edges) {
     static_assert(B::TA == B::TB, "square blocks: the diagonal ones hold both sides");
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    const uint64_t g = (row_tiles + B::TA - 1) / B::TA, bands = (g + 7) / 8, total = 32 * bands * (bands + 1);
-    for (uint64_t t = blockIdx.x; t < total; t += gridDim.x) {
-        const uint64_t first = t - blockIdx.x, here = total - first < gridDim.x ? total - first : gridDim.x;
-        const uint64_t l = first + xcd_order(blockIdx.x, here);
-        // band b: eight block rows, 8 (b + 1) block columns, after 32 b (b + 1) places
-        uint64_t b = (uint64_t)((__builtin_sqrtf(1.0f + (float)l / 8.0f) - 1.0f) * 0.5f);
-        while (32 * b * (b + 1) > l) b--;
-        while (32 * (b + 1) * (b + 2) <= l) b++;
-        const uint64_t in = l - 32 * b * (b + 1), bi = b * 8 + in % 8, bj = in / 8;
-        if (bi >= g || bj > bi) continue;  // the same for the whole block
-        const uint64_t i0 = bi * B::TA, j0 = bj * B::TB;
-        f32x16 acc[FM][FN];
-        mx_tile<WR, WC, FM, FN>(codes, scales, i0, row_tiles, codes, scales, j0, row_tiles, col_tiles, lds, acc);
-        const uint32_t lane = lane_id(), wave = threadIdx.x / 64, wr = wave / WC, wc = wave % WC;
+    const uint32_t g = (a.tiles + B::TA - 1) / B::TA, bands = (g + 7) / 8, total = 32 * bands * (bands + 1);
+    auto next = [&](uint32_t& cursor) -> Place {
+        for (;;) {
+            const uint32_t l = list_place(cursor, total);
+            cursor += gridDim.x;
+            if (l >= total) return {0, 0, false};
+            // band: eight block rows, 8 (band + 1) block columns, after 32 band (band + 1) places
+            uint32_t band = (uint32_t)((__builtin_sqrtf(1.0f + (float)l / 8.0f) - 1.0f) * 0.5f);
+            while (32 * band * (band + 1) > l) band--;
+            while (32 * (band + 1) * (band + 2) <= l) band++;
+            const uint32_t in = l - 32 * band * (band + 1), bi = band * 8 + in % 8, bj = in / 8;
+            if (bi < g && bj <= bi) return place_at(bi * B::TA, bj * B::TB);
+        }
+    };
+    auto finish = [&](const Place& t, f32x16 (&acc)[B::FM][B::FN]) -> bool {
+        const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave / B::WC, wc = wave % B::WC;
+        const uint32_t last = a.tiles - 1, it = t.i0 + wr * B::FM, jt = t.j0 + wc * B::FN;
 #pragma unroll
-        for (int i = 0; i < FM; i++) {
-            const uint64_t u = (i0 + wr * FM + i) * 32 + lane % 32;
-            const float need = u < n ? min_cosine * length[u] : __builtin_inff();
+        for (int i = 0; i < B::FM; i++) {
+            const float li = it + i <= last ? least[it + i] * min_cosine : __builtin_inff();
 #pragma unroll
-            for (int j = 0; j < FN; j++)
+            for (int j = 0; j < B::FN; j++) {
+                const float lj = jt + j <= last ? least[jt + j] : __builtin_inff();
+                float top = acc[i][j][0];
+#pragma unroll
+                for (int k = 1; k < 16; k++) top = fmaxf(top, acc[i][j][k]);
+                if (__ballot(top >= li * lj) == 0) continue;
+                const uint64_t u = ((uint64_t)it + i) * 32 + lane % 32;
+                const float need = u < n ? min_cosine * length[u] : __builtin_inff();
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    const uint64_t v0 = (j0 + wc * FN + j) * 32 + q * 8 + lane / 32 * 4;
+                    const uint64_t v0 = ((uint64_t)jt + j) * 32 + q * 8 + lane / 32 * 4;
                     f32x4 len = __builtin_inff();
-                    if (v0 < row_tiles * 32) len = *reinterpret_cast<const f32x4*>(length + v0);  // filled up to whole tiles
-                    bool any = false;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) any |= acc[i][j][q * 4 + k] >= need * len[k];
-                    if (__ballot(any) == 0) continue;
+                    if (jt + j <= last) len = *reinterpret_cast<const f32x4*>(length + v0);  // filled up to whole tiles
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const uint64_t v = v0 + k;
@@ -388,12 +519,18 @@ __global__ __launch_bounds__(WR * WC * 64) void mx_pairs_kernel(const uint8_t* _
                         }
                     }
                 }
+            }
         }
-    }
+        return false;
+    };
+    mx_stream<B, 0>(a, a, col_tiles, lds, next, finish);
 }
 
-using Big = Block<2, 4, 4, 2>;    // 256 x 256, 8 waves
-using Small = Block<2, 2, 2, 2>;  // 128 x 128, 4 waves
+// Large blocks read half as much from L2 per product, small ones fill the chip with fewer tiles: whichever needs less time
+// in rounds of the whole chip, a large round counted as four small ones of two blocks a CU at 5/4 of the time per product.
+bool large_blocks(uint64_t big_tiles, uint64_t small_tiles, uint64_t cus) {
+    return (big_tiles + cus - 1) / cus * 4 * 4 <= (small_tiles + 2 * cus - 1) / (2 * cus) * 2 * 5;
+}
 
 int check_packed(const char* who, const char* what, const void* codes, const void* scales) {
     REQUIRE(codes && scales, "%s: %s is NULL", who, what);
@@ -445,8 +582,9 @@ int mdd_mx_matmul(mdd_ctx* ctx, const uint8_t* a_codes, const uint8_t* a_scales,
     if (rc) return rc;
     REQUIRE(c && aligned_to(c, type_bytes(c_type)), "%s: c is NULL or not aligned to its elements", who);
     REQUIRE(c_stride >= n, "%s: c_stride below n", who);
-    ON_DEVICE(ctx);
     const uint64_t at = (m + 31) / 32, bt = (n + 31) / 32;
+    REQUIRE((at / Small::TA + 1) * (bt / Small::TB + 1) < MAX_TILES, "%s: m x n is above 2^31 tiles of 128 x 128", who);
+    ON_DEVICE(ctx);
     const uint32_t ct = (dim + 127) / 128;
     auto run = [&](auto* out) -> hipError_t {
         typedef std::remove_pointer_t<decltype(out)> O;
@@ -459,28 +597,25 @@ int mdd_mx_matmul(mdd_ctx* ctx, const uint8_t* a_codes, const uint8_t* a_scales,
                                b_scales, n, bt, ct, alpha, out, c_stride);
             return hipGetLastError();
         }
-        const uint64_t big = ((at + Big::TA - 1) / Big::TA) * ((bt + Big::TB - 1) / Big::TB), cap = 1u << 22;
-        if (big >= (uint64_t)ctx->cus) {  // large blocks read a quarter less from L2 per product; smaller ones where they would leave CUs idle
-            auto kernel = mx_matmul_kernel<O, 2, 4, 4, 2>;
-            hipError_t e = allow_lds(kernel, Big::LDS);
+        const Packed pa = {a_codes, a_scales, (uint32_t)at}, pb = {b_codes, b_scales, (uint32_t)bt};
+        const uint64_t cus = (uint64_t)ctx->cus;
+        const uint64_t big = ((at + Big::TA - 1) / Big::TA) * ((bt + Big::TB - 1) / Big::TB), small = ((at + Small::TA - 1) / Small::TA) * ((bt + Small::TB - 1) / Small::TB);
+        auto launch = [&](auto block, uint64_t tiles, uint64_t blocks) -> hipError_t {
+            typedef decltype(block) B;
+            constexpr uint32_t bytes = B::LDS + B::WAVES * B::OUT;
+            const hipError_t e = allow_lds(mx_matmul_kernel<O, B>, bytes);
             if (e != hipSuccess) return e;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)(big < cap ? big : cap)), dim3(Big::WAVES * 64), Big::LDS, ctx->stream, a_codes, a_scales, m, at, b_codes,
-                               b_scales, n, bt, ct, alpha, out, c_stride);
-        } else {
-            const uint64_t small = ((at + Small::TA - 1) / Small::TA) * ((bt + Small::TB - 1) / Small::TB);
-            auto kernel = mx_matmul_kernel<O, 2, 2, 2, 2>;
-            hipError_t e = allow_lds(kernel, Small::LDS);
-            if (e != hipSuccess) return e;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)(small < cap ? small : cap)), dim3(Small::WAVES * 64), Small::LDS, ctx->stream, a_codes, a_scales, m, at,
-                               b_codes, b_scales, n, bt, ct, alpha, out, c_stride);
-        }
-        return hipGetLastError();
+            hipLaunchKernelGGL((mx_matmul_kernel<O, B>), dim3((unsigned)(tiles < blocks ? tiles : blocks)), dim3(B::WAVES * 64), bytes, ctx->stream, pa, m, pb, n,
+                               ct, alpha, out, c_stride);
+            return hipGetLastError();
+        };
+        return large_blocks(big, small, cus) ? launch(Big(), big, cus) : launch(Small(), small, 2 * cus);
     };
     HIP_TRY(c_type == MDD_F32 ? run((float*)c) : run((__bf16*)c));
     return MDD_OK;
 }
 
-uint64_t mdd_mx_pairs_ws_bytes(uint64_t m) { return round_up(round_up(m, 32) * 4, 256); }
+uint64_t mdd_mx_pairs_ws_bytes(uint64_t m) { return round_up(round_up(m, 32) * 4, 256) + round_up((m + 31) / 32 * 4, 256); }
 
 int mdd_mx_pairs(mdd_ctx* ctx, const uint8_t* codes, const uint8_t* scales, uint64_t m, uint32_t dim, float min_cosine,
                  uint32_t* edge_u, uint32_t* edge_v, uint64_t edge_cap, uint64_t* n_edges, void* ws, uint64_t ws_bytes) {
@@ -488,7 +623,7 @@ int mdd_mx_pairs(mdd_ctx* ctx, const uint8_t* codes, const uint8_t* scales, uint
     REQUIRE(ctx && n_edges, "%s: NULL argument", who);
     REQUIRE(dim >= 1 && dim <= MDD_VEC_MAX_DIM, "%s: dim=%u outside [1,%d]", who, dim, MDD_VEC_MAX_DIM);
     REQUIRE(min_cosine > 0.0f && min_cosine <= 1.0f, "%s: min_cosine=%g outside (0,1]", who, (double)min_cosine);
-    REQUIRE(m < (1ull << 31), "%s: 2^31 or more rows", who);
+    REQUIRE(m <= MDD_MX_MAX_PAIR_ROWS, "%s: more than 2^22 rows", who);
     REQUIRE(edge_cap == 0 || (edge_u && edge_v), "%s: NULL buffer", who);
     const uint64_t need = mdd_mx_pairs_ws_bytes(m);
     if (m) {
@@ -500,22 +635,21 @@ int mdd_mx_pairs(mdd_ctx* ctx, const uint8_t* codes, const uint8_t* scales, uint
     const uint64_t rt = (m + 31) / 32;
     const uint32_t ct = (dim + 127) / 128;
     auto* count = reinterpret_cast<unsigned long long*>(n_edges);
+    float *length = (float*)ws, *least = length + round_up(m, 64);
     hipLaunchKernelGGL(mx_length_kernel, dim3((unsigned)(rt < 1 ? 1 : rt < (1u << 20) ? rt : (1u << 20))), dim3(128), 0, ctx->stream, codes, scales, ct, rt,
-                       (float*)ws, count);
+                       length, least, count);
     if (m) {
-        auto bands = [&](uint64_t t) { return ((rt + t - 1) / t + 7) / 8; };
-        const uint64_t b = bands(Big::TA), big = (rt + Big::TA - 1) / Big::TA, cap = 1u << 22;
-        if (big * (big + 1) / 2 >= (uint64_t)ctx->cus) {
-            const uint64_t total = 32 * b * (b + 1);
-            HIP_TRY(allow_lds(mx_pairs_kernel<2, 4, 4, 2>, Big::LDS));
-            hipLaunchKernelGGL((mx_pairs_kernel<2, 4, 4, 2>), dim3((unsigned)(total < cap ? total : cap)), dim3(Big::WAVES * 64), Big::LDS, ctx->stream, codes,
-                               scales, m, rt, ct, (const float*)ws, min_cosine, edge_u, edge_v, edge_cap, count);
-        } else {
-            const uint64_t s = bands(Small::TA), total = 32 * s * (s + 1);
-            HIP_TRY(allow_lds(mx_pairs_kernel<2, 2, 2, 2>, Small::LDS));
-            hipLaunchKernelGGL((mx_pairs_kernel<2, 2, 2, 2>), dim3((unsigned)(total < cap ? total : cap)), dim3(Small::WAVES * 64), Small::LDS, ctx->stream,
-                               codes, scales, m, rt, ct, (const float*)ws, min_cosine, edge_u, edge_v, edge_cap, count);
-        }
+        const uint64_t cus = (uint64_t)ctx->cus, big = (rt + Big::TA - 1) / Big::TA, small = (rt + Small::TA - 1) / Small::TA;
+        auto launch = [&](auto block, uint64_t g, uint64_t blocks) -> hipError_t {
+            typedef decltype(block) B;
+            const hipError_t e = allow_lds(mx_pairs_kernel<B>, B::LDS);
+            if (e != hipSuccess) return e;
+            const uint64_t places = 32 * ((g + 7) / 8) * ((g + 7) / 8 + 1);
+            hipLaunchKernelGGL((mx_pairs_kernel<B>), dim3((unsigned)(places < blocks ? places : blocks)), dim3(B::WAVES * 64), B::LDS, ctx->stream,
+                               Packed{codes, scales, (uint32_t)rt}, m, ct, length, least, min_cosine, edge_u, edge_v, edge_cap, count);
+            return hipGetLastError();
+        };
+        HIP_TRY(large_blocks(big * (big + 1) / 2, small * (small + 1) / 2, cus) ? launch(Big(), big, cus) : launch(Small(), small, 2 * cus));
     }
     HIP_TRY(hipGetLastError());
     return MDD_OK;
