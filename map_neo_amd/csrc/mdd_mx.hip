@@ -170,24 +170,28 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(const uint8_t* __restric
 // tiles (128 columns: a step) go from memory straight into LDS, three buffers in rotation, in one stream of steps that runs
 // on across the tiles of the list: while a tile's results leave, the next tile's first steps are landing.  A step is two
 // halves of 64 columns.  The fragments of a half are read from LDS while the half before is multiplied:
-//     read half 1 of step s                                   | multiply half 0 of step s
-//     wait for step s + 1, barrier, request step s + 3 into the buffer of step s
-//     read half 0 of step s + 1                               | multiply half 1 of step s
-// so a load has two steps to arrive, a step needs one barrier, and neither LDS nor memory latency stands before the matrix
-// unit.
+//     multiply half 0 of step s, and between the products: read half 1 of step s
+//     wait for step s + 1, barrier
+//     multiply half 1 of step s, and between them: read half 0 of step s + 1, request step s + 3 into the buffer of step s
+// so a load has two steps to arrive, a step needs one barrier, and neither LDS nor memory latency nor the issue of loads stands
+// before the matrix unit.
 template <int WR_, int WC_, int FM_, int FN_>
 struct Block {
     static constexpr int WR = WR_, WC = WC_, FM = FM_, FN = FN_;
     static constexpr int WAVES = WR * WC, TA = WR * FM, TB = WC * FN, TILES = TA + TB, PER_WAVE = TILES / WAVES;
     static constexpr uint32_t STAGE = TILES * (TILE + STILE), LDS = 3 * STAGE, OUT = 4096;  // OUT: a wave's room to turn results round
     static constexpr int LOADS = PER_WAVE * 2 + 1;  // per wave and step: two halves of each of its tiles, and their scales
-    static_assert(TILES % WAVES == 0 && PER_WAVE * 8 <= 64, "every wave loads whole tiles, their scales in one instruction");
+    static_assert(TILES == 2 * WAVES, "every wave loads two tiles, and their scales in one instruction of four bytes a lane");
 };
 using Big = Block<4, 2, 2, 4>;    // 256 x 256, 8 waves, one block a CU
 using Small = Block<2, 2, 2, 2>;  // 128 x 128, 4 waves, two blocks a CU
 
+// 16 (4) bytes of every lane from its own address to LDS, lane after lane from l on
 __device__ __forceinline__ void to_lds(const uint8_t* g, uint8_t* l) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g, (__attribute__((address_space(3))) uint32_t*)l, 16, 0, 0);
+}
+__device__ __forceinline__ void to_lds4(const uint8_t* g, uint8_t* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g, (__attribute__((address_space(3))) uint32_t*)l, 4, 0, 0);
 }
 // Waits by the builtin, not by a statement in assembly: the compiler then knows that nothing before is left to wait for.
 // (vmcnt bits 0-3 and 14-15, expcnt 4-6, lgkmcnt 8-11)
@@ -243,36 +247,39 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
         };
 #pragma unroll
         for (int i = 0; i < B::PER_WAVE; i++) src[i] = at(wave * B::PER_WAVE + i, a.codes, b.codes, TILE);
-        ssrc = at(wave * B::PER_WAVE + (lane / 8 < B::PER_WAVE ? lane / 8 : 0), a.scales, b.scales, STILE) + lane % 8 * 16;
+        ssrc = at(wave * B::PER_WAVE + lane / 32, a.scales, b.scales, STILE) + lane % 32 * 4;
     };
     aim();
-    auto request = [&]() -> bool {  // the stream's next step; false when the list is done
-        if (!req.valid) return false;
-        uint8_t* to = lds + req_buf * B::STAGE;
+    // A request is one load instruction of 1 KB at a time, `item` 0 .. LOADS - 1, so that it can be strewn among the products.
+    const uint8_t *from[B::PER_WAVE], *sfrom;
+    uint8_t* into;
+    auto turn_to_next = [&]() {  // the stream's next step.  Behind the list's end the last tile again: never used, always there
 #pragma unroll
-        for (int i = 0; i < B::PER_WAVE; i++) {
-            uint8_t* l = to + (wave * B::PER_WAVE + i) * TILE;
-            const uint8_t* g = src[i] + (uint64_t)req_k * TILE;
-            to_lds(g + lane * 16, l);
-            to_lds(g + 1024 + lane * 16, l + 1024);
-        }
-        if (lane < B::PER_WAVE * 8) to_lds(ssrc + (uint64_t)req_k * STILE, to + B::TILES * TILE + wave * B::PER_WAVE * STILE);
+        for (int i = 0; i < B::PER_WAVE; i++) from[i] = src[i] + (uint64_t)req_k * TILE;
+        sfrom = ssrc + (uint64_t)req_k * STILE;
+        into = lds + req_buf * B::STAGE;
         req_buf = req_buf == 2 ? 0 : req_buf + 1;
         if (++req_k == col_tiles) {
             req_k = 0;
-            req = next(req_cursor);
-            if (req.valid) aim();
+            const Place t = next(req_cursor);
+            if (t.valid) {
+                req = t;
+                aim();
+            }
         }
-        return true;
+    };
+    auto request = [&](int item) {
+        if (item < 2 * B::PER_WAVE)
+            to_lds(from[item / 2] + item % 2 * 1024 + lane * 16, into + (wave * B::PER_WAVE + item / 2) * TILE + item % 2 * 1024);
+        else
+            to_lds4(sfrom, into + B::TILES * TILE + wave * B::PER_WAVE * STILE);
     };
     i32x4 fa[2][FM], fb[2][FN];
     int xa[FM], xb[FN], ya[FM], yb[FN];  // a step's scales, both halves in one register; the next step's
-    auto read_half = [&](uint32_t buf, int h) {
+    auto read_one = [&](uint32_t buf, int h, int item) {  // fragments 0 .. FM + FN - 1
         const uint8_t* l = lds + buf * B::STAGE + h * 1024 + lane * 16;
-#pragma unroll
-        for (int i = 0; i < FM; i++) fa[h][i] = *reinterpret_cast<const i32x4*>(l + (wr * FM + i) * TILE);
-#pragma unroll
-        for (int j = 0; j < FN; j++) fb[h][j] = *reinterpret_cast<const i32x4*>(l + (B::TA + wc * FN + j) * TILE);
+        if (item < FM) fa[h][item] = *reinterpret_cast<const i32x4*>(l + (wr * FM + item) * TILE);
+        else fb[h][item - FM] = *reinterpret_cast<const i32x4*>(l + (B::TA + wc * FN + item - FM) * TILE);
     };
     auto read_scales = [&](uint32_t buf) {
         const uint8_t* s = lds + buf * B::STAGE + B::TILES * TILE + lane * 2;
@@ -282,11 +289,9 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
         for (int j = 0; j < FN; j++) yb[j] = *reinterpret_cast<const uint16_t*>(s + (B::TA + wc * FN + j) * STILE);
     };
     f32x16 acc[FM][FN];
-    auto multiply = [&](int h) {
-#pragma unroll
-        for (int i = 0; i < FM; i++)
-#pragma unroll
-            for (int j = 0; j < FN; j++) acc[i][j] = mma(fb[h][j], xb[j], fa[h][i], xa[i], acc[i][j], h);
+    auto multiply = [&](int h, int x) {
+        const int i = x / FN, j = x % FN;
+        acc[i][j] = mma(fb[h][j], xb[j], fa[h][i], xa[i], acc[i][j], h);
     };
     auto take_scales = [&]() {
 #pragma unroll
@@ -294,15 +299,21 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
 #pragma unroll
         for (int j = 0; j < FN; j++) xb[j] = yb[j];
     };
+    constexpr int PRODUCTS = FM * FN, READS = FM + FN, ITEMS = READS + 1 + B::LOADS;
+    constexpr int A_EACH = (READS + PRODUCTS - 3) / (PRODUCTS - 2), B_EACH = (ITEMS + PRODUCTS - 1) / PRODUCTS;
 
-    int ahead = -1;  // steps requested behind the current one
 #pragma unroll 1
-    for (int r = 0; r < 3; r++) ahead += request() ? 1 : 0;
-    wait_memory<0>();
+    for (int r = 0; r < 3; r++) {
+        turn_to_next();
+#pragma unroll
+        for (int i = 0; i < B::LOADS; i++) request(i);
+    }
+    wait_memory<2 * B::LOADS>();
     __builtin_amdgcn_s_barrier();
     uint32_t buf = 0;
     read_scales(0);
-    read_half(0, 0);
+#pragma unroll
+    for (int i = 0; i < READS; i++) read_one(0, 0, i);
     take_scales();
     int behind = 0;  // steps for which finish's operations are younger than the loads waited for
     while (cur.valid) {
@@ -313,25 +324,38 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
         wait_lds();
 #pragma unroll 1
         for (uint32_t k = 0; k < col_tiles; k++) {
-            read_half(buf, 1);
-            __builtin_amdgcn_sched_barrier(0);  // reads first: they take as long as the products that follow
-            multiply(0);
+            turn_to_next();
+            // a product keeps the matrix unit busy for 32 cycles: what else a half has to issue goes between them
+#pragma unroll
+            for (int x = 0; x < PRODUCTS; x++) {
+                multiply(0, x);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = x * A_EACH; i < (x + 1) * A_EACH && i < READS; i++) read_one(buf, 1, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             keep_here(acc);
             // step s + 1 has landed when only younger operations are left: the loads of step s + 2, and for two steps after a
             // tile the stores of its results.  And this wave has read all it wants of the buffer of step s, which is requested
             // anew behind the barrier.
             wait_lds();
-            if (ahead <= 1) wait_memory<0>();
-            else if (behind > 0) wait_memory<B::LOADS + STORES>();
+            if (behind > 0) wait_memory<B::LOADS + STORES>();
             else wait_memory<B::LOADS>();
             __builtin_amdgcn_s_barrier();
-            if (!request()) ahead--;
             behind--;
-            buf = buf == 2 ? 0 : buf + 1;
-            read_scales(buf);  // behind the last step: whatever the buffer holds, not used
-            read_half(buf, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(1);
+            buf = buf == 2 ? 0 : buf + 1;  // behind the last step: whatever the buffer holds, not used
+#pragma unroll
+            for (int x = 0; x < PRODUCTS; x++) {
+                multiply(1, x);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = x * B_EACH; i < (x + 1) * B_EACH && i < ITEMS; i++) {
+                    if (i < READS) read_one(buf, 0, i);
+                    else if (i == READS) read_scales(buf);
+                    else request(i - READS - 1);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             keep_here(acc);
             __builtin_amdgcn_sched_barrier(0);  // the reads have had the products' time to arrive
             take_scales();
@@ -339,6 +363,7 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
         behind = finish(cur, acc) ? 2 : 0;
         cur = next(cursor);
     }
+    wait_memory<0>();  // loads into LDS do not outlive the block
 }
 
 // Work order.  Blocks go to the eight XCDs in turn, so XCD x gets a run of consecutive tiles of the list, and the list walks
