@@ -238,6 +238,7 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
     Place req = next(req_cursor), cur = next(cursor);
     if (!cur.valid) return;
     uint32_t req_k = 0, req_buf = 0;
+    Place ahead = {0, 0, false};  // the tile last turned to
     const uint8_t *src[B::PER_WAVE], *ssrc;
     auto aim = [&]() {  // this wave's share: PER_WAVE row tiles.  Tiles past the end repeat the last one; their results are not used
         auto at = [&](uint32_t t, const uint8_t* pa, const uint8_t* pb, uint32_t bytes) {
@@ -261,9 +262,9 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
         req_buf = req_buf == 2 ? 0 : req_buf + 1;
         if (++req_k == col_tiles) {
             req_k = 0;
-            const Place t = next(req_cursor);
-            if (t.valid) {
-                req = t;
+            ahead = next(req_cursor);
+            if (ahead.valid) {
+                req = ahead;
                 aim();
             }
         }
@@ -289,9 +290,10 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
         for (int j = 0; j < FN; j++) yb[j] = *reinterpret_cast<const uint16_t*>(s + (B::TA + wc * FN + j) * STILE);
     };
     f32x16 acc[FM][FN];
-    auto multiply = [&](int h, int x) {
+    auto multiply = [&](int h, int x, bool fresh) {  // fresh: the tile's first product, to nothing added
         const int i = x / FN, j = x % FN;
-        acc[i][j] = mma(fb[h][j], xb[j], fa[h][i], xa[i], acc[i][j], h);
+        const f32x16 none = 0.0f;
+        acc[i][j] = mma(fb[h][j], xb[j], fa[h][i], xa[i], fresh ? none : acc[i][j], h);
     };
     auto take_scales = [&]() {
 #pragma unroll
@@ -316,52 +318,52 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
     for (int i = 0; i < READS; i++) read_one(0, 0, i);
     take_scales();
     int behind = 0;  // steps for which finish's operations are younger than the loads waited for
-    while (cur.valid) {
+    auto step = [&](auto fresh) {
+        turn_to_next();
+        // a product keeps the matrix unit busy for 32 cycles: what else a half has to issue goes between them
 #pragma unroll
-        for (int i = 0; i < FM; i++)
+        for (int x = 0; x < PRODUCTS; x++) {
+            multiply(0, x, decltype(fresh)::value);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < FN; j++) acc[i][j] = 0.0f;
-        wait_lds();
-#pragma unroll 1
-        for (uint32_t k = 0; k < col_tiles; k++) {
-            turn_to_next();
-            // a product keeps the matrix unit busy for 32 cycles: what else a half has to issue goes between them
-#pragma unroll
-            for (int x = 0; x < PRODUCTS; x++) {
-                multiply(0, x);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int i = x * A_EACH; i < (x + 1) * A_EACH && i < READS; i++) read_one(buf, 1, i);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            keep_here(acc);
-            // step s + 1 has landed when only younger operations are left: the loads of step s + 2, and for two steps after a
-            // tile the stores of its results.  And this wave has read all it wants of the buffer of step s, which is requested
-            // anew behind the barrier.
-            wait_lds();
-            if (behind > 0) wait_memory<B::LOADS + STORES>();
-            else wait_memory<B::LOADS>();
-            __builtin_amdgcn_s_barrier();
-            behind--;
-            buf = buf == 2 ? 0 : buf + 1;  // behind the last step: whatever the buffer holds, not used
-#pragma unroll
-            for (int x = 0; x < PRODUCTS; x++) {
-                multiply(1, x);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int i = x * B_EACH; i < (x + 1) * B_EACH && i < ITEMS; i++) {
-                    if (i < READS) read_one(buf, 0, i);
-                    else if (i == READS) read_scales(buf);
-                    else request(i - READS - 1);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            keep_here(acc);
-            __builtin_amdgcn_sched_barrier(0);  // the reads have had the products' time to arrive
-            take_scales();
+            for (int i = x * A_EACH; i < (x + 1) * A_EACH && i < READS; i++) read_one(buf, 1, i);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        keep_here(acc);
+        // step s + 1 has landed when only younger operations are left: the loads of step s + 2, and for two steps after a tile
+        // the stores of its results.  And this wave has read all it wants of the buffer of step s, which is requested anew
+        // behind the barrier.
+        wait_lds();
+        if (behind > 0) wait_memory<B::LOADS + STORES>();
+        else wait_memory<B::LOADS>();
+        __builtin_amdgcn_s_barrier();
+        behind--;
+        buf = buf == 2 ? 0 : buf + 1;  // behind the last step: whatever the buffer holds, not used
+#pragma unroll
+        for (int x = 0; x < PRODUCTS; x++) {
+            multiply(1, x, false);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = x * B_EACH; i < (x + 1) * B_EACH && i < ITEMS; i++) {
+                if (i < READS) read_one(buf, 0, i);
+                else if (i == READS) read_scales(buf);
+                else request(i - READS - 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        keep_here(acc);
+        __builtin_amdgcn_sched_barrier(0);  // the reads have had the products' time to arrive
+        take_scales();
+    };
+    while (cur.valid) {
+        wait_lds();
+        step(std::true_type());
+#pragma unroll 1
+        for (uint32_t k = 1; k < col_tiles; k++) step(std::false_type());
         behind = finish(cur, acc) ? 2 : 0;
-        cur = next(cursor);
+        // requests are three steps ahead: with four steps a tile or more, the tile turned to last is the one after this
+        if (col_tiles >= 4) cur = ahead;
+        else cur = next(cursor);
     }
     wait_memory<0>();  // loads into LDS do not outlive the block
 }
@@ -510,23 +512,27 @@ __global__ __launch_bounds__(B::WAVES * 64) void mx_pairs_kernel(const Packed a,
     auto finish = [&](const Place& t, f32x16 (&acc)[B::FM][B::FN]) -> bool {
         const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave / B::WC, wc = wave % B::WC;
         const uint32_t last = a.tiles - 1, it = t.i0 + wr * B::FM, jt = t.j0 + wc * B::FN;
+        float li[B::FM], lj[B::FN];  // uniform: scalar loads, all at once
+#pragma unroll
+        for (int i = 0; i < B::FM; i++) li[i] = least[it + i <= last ? it + i : last];
+#pragma unroll
+        for (int j = 0; j < B::FN; j++) lj[j] = least[jt + j <= last ? jt + j : last];
 #pragma unroll
         for (int i = 0; i < B::FM; i++) {
-            const float li = it + i <= last ? least[it + i] * min_cosine : __builtin_inff();
+            if (it + i > last) break;
 #pragma unroll
             for (int j = 0; j < B::FN; j++) {
-                const float lj = jt + j <= last ? least[jt + j] : __builtin_inff();
+                if (jt + j > last) break;
                 float top = acc[i][j][0];
 #pragma unroll
                 for (int k = 1; k < 16; k++) top = fmaxf(top, acc[i][j][k]);
-                if (__ballot(top >= li * lj) == 0) continue;
+                if (__ballot(top >= min_cosine * li[i] * lj[j]) == 0) continue;
                 const uint64_t u = ((uint64_t)it + i) * 32 + lane % 32;
                 const float need = u < n ? min_cosine * length[u] : __builtin_inff();
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     const uint64_t v0 = ((uint64_t)jt + j) * 32 + q * 8 + lane / 32 * 4;
-                    f32x4 len = __builtin_inff();
-                    if (jt + j <= last) len = *reinterpret_cast<const f32x4*>(length + v0);  // filled up to whole tiles
+                    const f32x4 len = *reinterpret_cast<const f32x4*>(length + v0);  // filled up to whole tiles
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const uint64_t v = v0 + k;
