@@ -12,11 +12,12 @@ namespace {
 constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
 
 // ------------------------------------------------------------------------------------------------ embedding lookup
-// out[d] = f_d * sum of table rows.  A wave sums one document: LPR lanes side by side cover a row's columns (8 each, a
-// slab of 512 columns per wave, further slabs are waves of their own), the 64 / LPR lane groups take neighbouring
-// positions.  64 ids are read at once and handed out by lane, then up to eight rows per group are in flight.
+// out[d] = f_d * sum of table rows.  A wave sums one document: `lpr` lanes side by side cover a row's columns (8 each; with NS = 2
+// all 64 lanes take 8 in either half of 1024, and wider rows are shared by waves of their own), the 64 / lpr lane groups take
+// neighbouring positions.  64 ids are read at once, a batch ahead; those that name a row move up to the lowest lanes, so that
+// padding costs nothing behind this point, and are handed out by lane, up to eight rows per group in flight.
 // The table of a static embedding (64000 x 256 in bf16: 33 MB) lives in the last-level cache, so the kernel is bound by
-// the cache's gather rate, not by HBM.
+// the caches' gather rate and its own additions, not by HBM.
 //
 // Documents longer than a piece (2^piece_log2 ids) would leave one wave with all the work: the id axis is cut into pieces, a
 // piece's share of a long document goes to a workspace row in float, and pool_join_kernel adds the shares in order.  A piece
@@ -25,8 +26,9 @@ constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
 struct PoolArgs {
     const void* table;
     uint64_t n_rows, stride;
-    uint32_t dim;
+    uint32_t dim, lpr;
     const void* ids;
+    int id_bytes;
     uint64_t n_ids;
     const uint64_t* offsets;
     uint64_t n_docs;
@@ -37,64 +39,86 @@ struct PoolArgs {
     uint64_t n_pieces;
     float* part;       // [piece][slot][dim]
     uint32_t* part_n;  // [piece][slot] ids that name a row
+    uint64_t* begins;  // [piece] the long document that begins in it, ~0 without one
     void* out;
 };
 
-template <typename T, int U>
-__device__ __forceinline__ void add_rows(const T* __restrict__ table, uint64_t stride, uint32_t row_of_lane, float w_of_lane, bool weighted,
-                                         int first, int step, uint32_t n_cols, f32x8& acc) {
-    typename vec8<T>::raw raw[U];
-    uint32_t r[U];
+// row that position p's id names, or NO_ROW (negative ids become huge: padding as well)
+__device__ __forceinline__ uint32_t named_row(const void* ids, int id_bytes, uint64_t p, uint64_t n_rows) {
+    const uint64_t id = id_bytes == 4 ? (uint64_t)(int64_t)reinterpret_cast<const int32_t*>(ids)[p] : (uint64_t)reinterpret_cast<const int64_t*>(ids)[p];
+    return id < n_rows ? (uint32_t)id : NO_ROW;
+}
+
+// U rows per lane group, `first + u * step` of the 64 that the lanes hold.  ALL: every one of them is named; otherwise NO_ROW is
+// among them, for which row 0 is read and dropped, whatever it holds, NaN included.
+template <typename T, int NS, bool WEIGHTED, bool ALL, int U>
+__device__ __forceinline__ void add_rows(const T* __restrict__ table, uint64_t stride, uint32_t held, float weight, int first, int step, const uint32_t (&n_cols)[NS],
+                                         f32x8 (&acc)[NS]) {
+    typename vec8<T>::raw raw[U][NS];
+    uint32_t at[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        r[u] = __shfl(row_of_lane, first + u * step, 64);
-        raw[u] = load8_raw<T>(table + (uint64_t)(r[u] != NO_ROW ? r[u] : 0) * stride, n_cols);
+        at[u] = __shfl(held, first + u * step, 64);
+        const T* row = table + (uint64_t)(ALL || at[u] != NO_ROW ? at[u] : 0) * stride;
+#pragma unroll
+        for (int n = 0; n < NS; n++) raw[u][n] = load8_raw<T>(row + n * 512, n_cols[n]);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        f32x8 v = __builtin_convertvector(raw[u], f32x8);
-        const float w = weighted ? __shfl(w_of_lane, first + u * step, 64) : 1.0f;
+        const float w = WEIGHTED ? __shfl(weight, first + u * step, 64) : 1.0f;
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const float x = r[u] != NO_ROW ? v[k] : 0.0f;  // padding read row 0: whatever it holds, NaN included, is dropped
-            acc[k] = weighted ? fmaf(x, w, acc[k]) : acc[k] + x;
+        for (int n = 0; n < NS; n++) {
+            f32x8 v = __builtin_convertvector(raw[u][n], f32x8);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float x = ALL || at[u] != NO_ROW ? v[k] : 0.0f;
+                acc[n][k] = WEIGHTED ? fmaf(x, w, acc[n][k]) : acc[n][k] + x;
+            }
         }
     }
 }
 
 // sum of the rows named by ids [beg, end) in this lane's columns; n_named = ids that name a row.  Call with all lanes.
-template <typename T, typename ID, int LPR>
-__device__ __forceinline__ f32x8 sum_span(const PoolArgs& a, uint64_t beg, uint64_t end, uint32_t col, uint32_t& n_named) {
-    constexpr int G = 64 / LPR;
+template <typename T, int NS, bool WEIGHTED>
+__device__ __forceinline__ void sum_span(const PoolArgs& a, uint64_t beg, uint64_t end, uint32_t col, f32x8 (&acc)[NS], uint32_t& n_named) {
+    const int lane = (int)lane_id(), lpr = NS == 2 ? 64 : (int)a.lpr, G = 64 / lpr, g = lane / lpr;
     const T* __restrict__ table = reinterpret_cast<const T*>(a.table) + (col < a.dim ? col : 0);
-    const uint32_t n_cols = col < a.dim ? a.dim - col : 0;
-    const ID* __restrict__ ids = reinterpret_cast<const ID*>(a.ids);
-    const int lane = (int)lane_id(), g = lane / LPR;
-    f32x8 acc = 0.0f;
-    n_named = 0;
-    const bool weighted = a.row_count != nullptr;
-    for (uint64_t p = beg; p < end; p += 64) {
-        uint32_t row = NO_ROW;
-        float w = 0.0f;
-        if (p + lane < end) {
-            const uint64_t id = (uint64_t)(int64_t)ids[p + lane];  // negative ids become huge: padding
-            if (id < a.n_rows) row = (uint32_t)id;
-            if (weighted && row != NO_ROW) w = a.scale / (float)a.row_count[row];
-        }
-        n_named += (uint32_t)__popcll(__ballot(row != NO_ROW));
-        const int n = end - p < 64 ? (int)(end - p) : 64, steps = (n + G - 1) / G;  // steps of G positions, one per group
-        int j = 0;
-        for (; j + 8 <= steps; j += 8) add_rows<T, 8>(table, a.stride, row, w, weighted, j * G + g, G, n_cols, acc);
-        // what is left in batches of 4, 2, 1: at most three more round trips and no row read twice
-        if (j + 4 <= steps) add_rows<T, 4>(table, a.stride, row, w, weighted, j * G + g, G, n_cols, acc), j += 4;
-        if (j + 2 <= steps) add_rows<T, 2>(table, a.stride, row, w, weighted, j * G + g, G, n_cols, acc), j += 2;
-        if (j < steps) add_rows<T, 1>(table, a.stride, row, w, weighted, j * G + g, G, n_cols, acc);
+    uint32_t n_cols[NS];
+#pragma unroll
+    for (int n = 0; n < NS; n++) {
+        n_cols[n] = col + n * 512 < a.dim ? a.dim - col - n * 512 : 0;
+        acc[n] = 0.0f;
     }
+    n_named = 0;
+    uint32_t row = beg + lane < end ? named_row(a.ids, a.id_bytes, beg + lane, a.n_rows) : NO_ROW;
+    for (uint64_t p = beg; p < end; p += 64) {
+        const uint32_t next = p + 64 + lane < end ? named_row(a.ids, a.id_bytes, p + 64 + lane, a.n_rows) : NO_ROW;
+        const uint64_t named = __ballot(row != NO_ROW);
+        const int n = __popcll(named);
+        n_named += (uint32_t)n;
+        float w = 0.0f;
+        if (WEIGHTED && row != NO_ROW) w = a.scale / (float)a.row_count[row];
+        if (n < 64) {  // named lanes to 0 .. n - 1 in their order, the others behind them
+            const uint32_t up = below(named), to = row != NO_ROW ? up : n + lane - up;
+            row = (uint32_t)__builtin_amdgcn_ds_permute((int)to * 4, (int)row);
+            if (WEIGHTED) w = __int_as_float(__builtin_amdgcn_ds_permute((int)to * 4, __float_as_int(w)));
+        }
+        // steps of G rows, one per group: eight at a time, what is left in batches of 4, 2, 1 (at most three more round trips,
+        // no row read twice), and last the groups that get one row more than the others
+        const int steps = n / G;
+        int j = 0;
+        for (; j + 8 <= steps; j += 8) add_rows<T, NS, WEIGHTED, true, 8>(table, a.stride, row, w, j * G + g, G, n_cols, acc);
+        if (j + 4 <= steps) add_rows<T, NS, WEIGHTED, true, 4>(table, a.stride, row, w, j * G + g, G, n_cols, acc), j += 4;
+        if (j + 2 <= steps) add_rows<T, NS, WEIGHTED, true, 2>(table, a.stride, row, w, j * G + g, G, n_cols, acc), j += 2;
+        if (j < steps) add_rows<T, NS, WEIGHTED, true, 1>(table, a.stride, row, w, j * G + g, G, n_cols, acc), j++;
+        if (j * G < n) add_rows<T, NS, WEIGHTED, false, 1>(table, a.stride, row, w, j * G + g, G, n_cols, acc);
+        row = next;
+    }
+    for (int m = lpr; m < 64; m <<= 1)
 #pragma unroll
-    for (int m = LPR; m < 64; m <<= 1)
+        for (int n = 0; n < NS; n++)
 #pragma unroll
-        for (int k = 0; k < 8; k++) acc[k] += __shfl_xor(acc[k], m, 64);
-    return acc;
+            for (int k = 0; k < 8; k++) acc[n][k] += __shfl_xor(acc[n][k], m, 64);
 }
 
 __device__ __forceinline__ float pool_factor(const PoolArgs& a, uint32_t n_named) {
@@ -113,17 +137,38 @@ __device__ __forceinline__ uint64_t doc_at(const uint64_t* __restrict__ offsets,
     return lo ? lo - 1 : n_docs;
 }
 
-template <typename T, typename ID, typename O, int LPR>
+// the same for a whole wave and one position: 64 places are looked at together, three rounds where the above takes sixteen
+__device__ __forceinline__ uint64_t wave_doc_at(const uint64_t* __restrict__ offsets, uint64_t n_docs, uint64_t pos) {
+    const uint32_t lane = lane_id();
+    uint64_t lo = 0, hi = n_docs;
+    while (lo < hi) {
+        const uint64_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step - 1;
+        lo += step * (uint64_t)__popcll(__ballot(at < hi && offsets[at < hi ? at : lo] <= pos));
+        if (step == 1) break;
+        hi = hi < lo + step - 1 ? hi : lo + step - 1;
+    }
+    return lo ? lo - 1 : n_docs;
+}
+
+template <typename O, int NS>
+__device__ __forceinline__ void store_cols(O* __restrict__ row, uint32_t col, uint32_t dim, const f32x8 (&v)[NS], float f) {
+#pragma unroll
+    for (int n = 0; n < NS; n++)
+        if (col + n * 512 < dim) store8<O>(row + col + n * 512, dim - col - n * 512, v[n] * f);
+}
+
+template <typename T, typename O, int NS, bool WEIGHTED>
 __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
-    const uint32_t lane = lane_id(), col = blockIdx.y * 512u + (lane % LPR) * 8u;
-    const bool writes = lane < LPR && col < a.dim;
+    const uint32_t lane = lane_id(), lpr = NS == 2 ? 64 : a.lpr, col = blockIdx.y * (512u * NS) + (lane & (lpr - 1)) * 8u;
     const uint64_t n_work = a.n_pieces + a.n_docs, stride = (uint64_t)gridDim.x * 4;
     const uint64_t piece = 1ull << a.piece_log2;
     for (uint64_t w = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; w < n_work; w += stride) {
         uint32_t n_named;
+        f32x8 acc[NS];
         if (w < a.n_pieces) {  // shares of long documents
             const uint64_t lo = w << a.piece_log2, hi = lo + piece < a.n_ids ? lo + piece : a.n_ids;
-            const uint64_t d0 = doc_at(a.offsets, a.n_docs, lo), d1 = doc_at(a.offsets, a.n_docs, hi - 1);
+            const uint64_t d0 = wave_doc_at(a.offsets, a.n_docs, lo), d1 = wave_doc_at(a.offsets, a.n_docs, hi - 1);
+            uint64_t begins = ~0ull;
 #pragma unroll 1
             for (int slot = 0; slot < 2; slot++) {
                 const uint64_t d = slot ? d1 : d0;
@@ -131,69 +176,80 @@ __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
                 uint64_t beg, end;
                 doc_range(a.offsets, d, a.n_ids, beg, end);
                 if (end - beg <= piece) continue;
+                if (beg >= lo && beg < hi) begins = d;
                 beg = beg > lo ? beg : lo;
                 end = end < hi ? end : hi;
-                f32x8 acc = sum_span<T, ID, LPR>(a, beg, end, col, n_named);
+                sum_span<T, NS, WEIGHTED>(a, beg, end, col, acc, n_named);
                 const uint64_t at = w * 2 + slot;
-                if (writes) store8<float>(a.part + at * a.dim + col, a.dim - col, acc);
+                if (lane < lpr) store_cols<float, NS>(a.part + at * a.dim, col, a.dim, acc, 1.0f);
                 if (lane == 0 && blockIdx.y == 0) a.part_n[at] = n_named;
             }
+            if (lane == 0 && blockIdx.y == 0) a.begins[w] = begins;
         } else {
             const uint64_t d = w - a.n_pieces;
             uint64_t beg, end;
             doc_range(a.offsets, d, a.n_ids, beg, end);
             if (a.n_pieces && end - beg > piece) continue;  // pool_join_kernel writes it
-            f32x8 acc = sum_span<T, ID, LPR>(a, beg, end, col, n_named);
-            if (writes) store8<O>(reinterpret_cast<O*>(a.out) + d * a.dim + col, a.dim - col, acc * pool_factor(a, n_named));
+            sum_span<T, NS, WEIGHTED>(a, beg, end, col, acc, n_named);
+            if (lane < lpr) store_cols<O, NS>(reinterpret_cast<O*>(a.out) + d * a.dim, col, a.dim, acc, pool_factor(a, n_named));
         }
     }
 }
 
-// A wave per document and 512 columns; only long ones have work: the shares of their pieces, in order, eight at a time.
+// A block per piece and 512 columns.  The long document that begins in the piece, if one does, is this block's: each of the four waves adds a quarter of its shares in order, eight at a time, and the quarters are added in
+// order.
 template <typename O>
 __global__ __launch_bounds__(256) void pool_join_kernel(PoolArgs a) {
-    const uint32_t lane = lane_id(), col = blockIdx.y * 512u + lane * 8u;
-    const uint64_t piece = 1ull << a.piece_log2, stride = (uint64_t)gridDim.x * 4;
-    for (uint64_t d = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; d < a.n_docs; d += stride) {
+    __shared__ __attribute__((aligned(32))) float quarter[3][512];
+    const uint32_t lane = lane_id(), wave = threadIdx.x / 64, col = blockIdx.y * 512u + lane * 8u;
+    for (uint64_t first = blockIdx.x; first < a.n_pieces; first += gridDim.x) {
+        const uint64_t d = a.begins[first];
+        if (d >= a.n_docs) continue;  // the same for the whole block
         uint64_t beg, end;
         doc_range(a.offsets, d, a.n_ids, beg, end);
-        if (end - beg <= piece) continue;
-        const uint64_t first = beg >> a.piece_log2, last = (end - 1) >> a.piece_log2;
+        const uint64_t last = (end - 1) >> a.piece_log2;
         // a long document leaves its first piece, so it is slot 0 there only if the piece begins with it
         const uint64_t at0 = first * 2 + (beg > first << a.piece_log2 ? 1 : 0);
         uint32_t n_named = 0;
         for (uint64_t k = first + lane; k <= last; k += 64) n_named += a.part_n[k == first ? at0 : k * 2];
 #pragma unroll
         for (int m = 32; m; m >>= 1) n_named += __shfl_xor(n_named, m, 64);
-        if (col >= a.dim) continue;
-        const float* __restrict__ part = a.part + col;
-        f32x8 acc = load8<float>(part + at0 * a.dim, a.dim - col);
-        uint64_t k = first + 1;
-        for (; k + 8 <= last + 1; k += 8) {
-            f32x8 v[8];
+        f32x8 acc = 0.0f;
+        if (col < a.dim) {
+            const float* __restrict__ part = a.part + col;
+            const uint64_t each = (last - first + 4) / 4;  // shares first + [wave * each, (wave + 1) * each)
+            uint64_t k = first + wave * each;
+            const uint64_t stop = k + each < last + 1 ? k + each : last + 1;
+            if (wave == 0) acc = load8<float>(part + at0 * a.dim, a.dim - col), k++;
+            for (; k + 8 <= stop; k += 8) {
+                f32x8 v[8];
 #pragma unroll
-            for (int u = 0; u < 8; u++) v[u] = load8<float>(part + (k + u) * 2 * a.dim, a.dim - col);
+                for (int u = 0; u < 8; u++) v[u] = load8<float>(part + (k + u) * 2 * a.dim, a.dim - col);
 #pragma unroll
-            for (int u = 0; u < 8; u++) acc += v[u];
+                for (int u = 0; u < 8; u++) acc += v[u];
+            }
+            for (; k < stop; k++) acc += load8<float>(part + k * 2 * a.dim, a.dim - col);
         }
-        for (; k <= last; k++) acc += load8<float>(part + k * 2 * a.dim, a.dim - col);
-        store8<O>(reinterpret_cast<O*>(a.out) + d * a.dim + col, a.dim - col, acc * pool_factor(a, n_named));
+        if (wave) *reinterpret_cast<f32x8*>(&quarter[wave - 1][lane * 8]) = acc;
+        __syncthreads();
+        if (wave == 0 && col < a.dim) {
+#pragma unroll
+            for (int q = 0; q < 3; q++) acc += *reinterpret_cast<const f32x8*>(&quarter[q][lane * 8]);
+            store8<O>(reinterpret_cast<O*>(a.out) + d * a.dim + col, a.dim - col, acc * pool_factor(a, n_named));
+        }
+        __syncthreads();
     }
 }
 
 // One row per id: eight rows per lane group in flight, read and written once -- bound by HBM where the table is large.
-template <typename T, typename ID, int LPR>
-__global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table, uint64_t n_rows, uint64_t row_stride, uint32_t dim,
-                                                     const ID* __restrict__ ids, uint64_t n_ids, float scale, T* __restrict__ out) {
-    constexpr int G = 64 / LPR, U = LPR < 8 ? LPR : 8;  // positions per wave and round: U * G <= 64
-    const uint32_t lane = lane_id(), g = lane / LPR, col = blockIdx.y * 512u + (lane % LPR) * 8u;
+template <typename T>
+__global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table, uint64_t n_rows, uint64_t row_stride, uint32_t dim, uint32_t lpr,
+                                                     const void* __restrict__ ids, int id_bytes, uint64_t n_ids, float scale, T* __restrict__ out) {
+    constexpr uint32_t U = 8;  // U * G positions per wave and round, 64 at most: lpr is 8 to 64
+    const uint32_t G = 64 / lpr, lane = lane_id(), g = lane / lpr, col = blockIdx.y * 512u + (lane & (lpr - 1)) * 8u;
     const uint64_t stride = (uint64_t)gridDim.x * 4 * (U * G);
     for (uint64_t p = ((uint64_t)blockIdx.x * 4 + threadIdx.x / 64) * (U * G); p < n_ids; p += stride) {
-        uint32_t row = NO_ROW;
-        if (lane < U * G && p + lane < n_ids) {
-            const uint64_t id = (uint64_t)(int64_t)ids[p + lane];
-            if (id < n_rows) row = (uint32_t)id;
-        }
+        const uint32_t row = lane < U * G && p + lane < n_ids ? named_row(ids, id_bytes, p + lane, n_rows) : NO_ROW;
         uint32_t r[U];
         typename vec8<T>::raw raw[U];
 #pragma unroll
@@ -239,16 +295,18 @@ __device__ __forceinline__ uint32_t rank_digit(uint32_t digit, bool live, volati
     return rank;
 }
 
-constexpr uint32_t SORT_TILE = 4096, SMALL_SORT = 8192;
+constexpr uint32_t SMALL_SORT = 8192;
+// keys a block: 1024 up to 2^20 keys, so that a quarter of a million still fill the chip; 4096 beyond, for a shorter histogram
+uint32_t sort_tile(uint64_t n) { return n <= (1u << 20) ? 1024 : 4096; }
 
-__global__ __launch_bounds__(256) void sort_count_kernel(const uint32_t* __restrict__ key, uint32_t n, int shift, uint32_t n_tiles,
+__global__ __launch_bounds__(256) void sort_count_kernel(const uint32_t* __restrict__ key, uint32_t n, int shift, uint32_t tile, uint32_t n_tiles,
                                                          uint32_t* __restrict__ hist) {
     __shared__ uint32_t cnt[256];
     cnt[threadIdx.x] = 0;
     __syncthreads();
-    const uint32_t base = blockIdx.x * SORT_TILE;
+    const uint32_t base = blockIdx.x * tile;
 #pragma unroll 4
-    for (uint32_t k = 0; k < SORT_TILE; k += 256) {
+    for (uint32_t k = 0; k < tile; k += 256) {
         const uint32_t i = base + k + threadIdx.x;
         if (i < n) atomicAdd(&cnt[key[i] >> shift & 255u], 1u);
     }
@@ -293,6 +351,7 @@ __global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t* __restrict__ h
     if (threadIdx.x == 0) hist[(uint64_t)256 * n_tiles + blockIdx.x] = carry;
 }
 
+template <int PER>  // keys a thread
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ val, uint32_t n, int shift,
                                                            uint32_t n_tiles, const uint32_t* __restrict__ hist, uint32_t* __restrict__ key_out,
                                                            uint32_t* __restrict__ val_out) {
@@ -300,12 +359,12 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __res
     const uint32_t t = threadIdx.x, wave = t / 64, lane = lane_id();
     for (int w = 0; w < 4; w++) cnt[w][t] = 0;
     __syncthreads();
-    const uint32_t base = blockIdx.x * SORT_TILE + wave * (SORT_TILE / 4) + lane;
-    uint32_t k_[16], rank[16];
+    const uint32_t base = blockIdx.x * (PER * 256) + wave * (PER * 64) + lane;
+    uint32_t k_[PER], rank[PER];
 #pragma unroll
-    for (int r = 0; r < 16; r++) k_[r] = base + r * 64 < n ? key[base + r * 64] : 0;
+    for (int r = 0; r < PER; r++) k_[r] = base + r * 64 < n ? key[base + r * 64] : 0;
 #pragma unroll
-    for (int r = 0; r < 16; r++) rank[r] = rank_digit(k_[r] >> shift & 255u, base + r * 64 < n, cnt[wave]);
+    for (int r = 0; r < PER; r++) rank[r] = rank_digit(k_[r] >> shift & 255u, base + r * 64 < n, cnt[wave]);
     __syncthreads();
     uint32_t all;
     uint32_t at = block_scan256(hist[(uint64_t)256 * n_tiles + t], lds4, &all) + hist[(uint64_t)t * n_tiles + blockIdx.x];
@@ -316,7 +375,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __res
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < 16; r++)
+    for (int r = 0; r < PER; r++)
         if (base + r * 64 < n) {
             const uint32_t to = cnt[wave][k_[r] >> shift & 255u] + rank[r];
             if (to < n) {  // always, unless the keys change while they are sorted
@@ -327,21 +386,27 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __res
 }
 
 // up to SMALL_SORT pairs in one block and one launch: all passes in LDS (8 us where the passes above take 12 launches)
-__global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__ key, uint32_t* __restrict__ val, uint32_t n, int bits) {
+// val_bits > 0: by the value's bits first, then by the key's
+__global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__ key, uint32_t* __restrict__ val, uint32_t n, int val_bits, int bits) {
     __shared__ uint32_t ks[SMALL_SORT], vs[SMALL_SORT], cnt[16][256], lds4[4];
-    const uint32_t t = threadIdx.x, wave = t / 64, lane = lane_id(), base = wave * 512 + lane;
+    const uint32_t t = threadIdx.x, wave = t / 64, lane = lane_id();
+    const uint32_t rounds = (n + 1023) / 1024, base = wave * rounds * 64 + lane;  // of 64 pairs a wave, all sixteen waves at work
     uint32_t k_[8], v_[8], rank[8];
 #pragma unroll
     for (int r = 0; r < 8; r++) {
         const uint32_t i = base + r * 64;
-        k_[r] = i < n ? key[i] : 0;
-        v_[r] = i < n ? val[i] : 0;
+        const bool live = r < (int)rounds && i < n;
+        k_[r] = live ? key[i] : 0;
+        v_[r] = live ? val[i] : 0;
     }
-    for (int shift = 0; shift < bits; shift += 8) {
+    for (int pass = 0, passes = (val_bits + 7) / 8 + (bits + 7) / 8; pass < passes; pass++) {
+        const bool by_val = pass < (val_bits + 7) / 8;
+        const int shift = 8 * (by_val ? pass : pass - (val_bits + 7) / 8);
         for (uint32_t i = t; i < 16 * 256; i += 1024) (&cnt[0][0])[i] = 0;
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < 8; r++) rank[r] = rank_digit(k_[r] >> shift & 255u, base + r * 64 < n, cnt[wave]);
+        for (int r = 0; r < 8; r++)
+            if (r < (int)rounds) rank[r] = rank_digit((by_val ? v_[r] : k_[r]) >> shift & 255u, base + r * 64 < n, cnt[wave]);
         __syncthreads();
         uint32_t own = 0;
         if (t < 256)
@@ -368,8 +433,8 @@ __global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < 8; r++)
-            if (base + r * 64 < n) {
-                const uint32_t to = cnt[wave][k_[r] >> shift & 255u] + rank[r];
+            if (r < (int)rounds && base + r * 64 < n) {
+                const uint32_t to = cnt[wave][(by_val ? v_[r] : k_[r]) >> shift & 255u] + rank[r];
                 ks[to] = k_[r];
                 vs[to] = v_[r];
             }
@@ -377,14 +442,13 @@ __global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__
 #pragma unroll
         for (int r = 0; r < 8; r++) {
             const uint32_t i = base + r * 64;
-            k_[r] = i < n ? ks[i] : 0;
-            v_[r] = i < n ? vs[i] : 0;
+            if (r < (int)rounds && i < n) k_[r] = ks[i], v_[r] = vs[i];
         }
         __syncthreads();
     }
 #pragma unroll
     for (int r = 0; r < 8; r++)
-        if (base + r * 64 < n) {
+        if (r < (int)rounds && base + r * 64 < n) {
             key[base + r * 64] = k_[r];
             val[base + r * 64] = v_[r];
         }
@@ -395,19 +459,20 @@ int bits_of(uint64_t largest) {
     while (b < 64 && largest >> b) b++;
     return b;
 }
-uint64_t sort_hist_words(uint64_t n) { return n <= SMALL_SORT ? 0 : 256 * ((n + SORT_TILE - 1) / SORT_TILE) + 256; }
+uint64_t sort_hist_words(uint64_t n) { return n <= SMALL_SORT ? 0 : 256 * ((n + sort_tile(n) - 1) / sort_tile(n)) + 256; }
 // sorts (key, val) by key, the values of equal keys in their order.  (key2, val2) are scratch of the same length (unused up to
 // SMALL_SORT pairs); the result is in key / val, which change places with key2 / val2 in every pass
 void sort_pairs(hipStream_t s, uint32_t*& key, uint32_t*& val, uint32_t*& key2, uint32_t*& val2, uint64_t n, int bits, uint32_t* hist) {
     if (n <= SMALL_SORT) {
-        hipLaunchKernelGGL(small_sort_kernel, dim3(1), dim3(1024), 0, s, key, val, (uint32_t)n, bits);
+        hipLaunchKernelGGL(small_sort_kernel, dim3(1), dim3(1024), 0, s, key, val, (uint32_t)n, 0, bits);
         return;
     }
-    const uint32_t tiles = (uint32_t)((n + SORT_TILE - 1) / SORT_TILE);
+    const uint32_t tile = sort_tile(n), tiles = (uint32_t)((n + tile - 1) / tile);
+    auto scatter = tile == 1024 ? sort_scatter_kernel<4> : sort_scatter_kernel<16>;
     for (int shift = 0; shift < bits; shift += 8) {
-        hipLaunchKernelGGL(sort_count_kernel, dim3(tiles), dim3(256), 0, s, key, (uint32_t)n, shift, tiles, hist);
+        hipLaunchKernelGGL(sort_count_kernel, dim3(tiles), dim3(256), 0, s, key, (uint32_t)n, shift, tile, tiles, hist);
         hipLaunchKernelGGL(sort_scan_kernel, dim3(256), dim3(256), 0, s, hist, tiles);
-        hipLaunchKernelGGL(sort_scatter_kernel, dim3(tiles), dim3(256), 0, s, key, val, (uint32_t)n, shift, tiles, hist, key2, val2);
+        hipLaunchKernelGGL(scatter, dim3(tiles), dim3(256), 0, s, key, val, (uint32_t)n, shift, tiles, hist, key2, val2);
         std::swap(key, key2);
         std::swap(val, val2);
     }
@@ -417,22 +482,21 @@ void sort_pairs(hipStream_t s, uint32_t*& key, uint32_t*& val, uint32_t*& key2, 
 // key[p] = id, or n_rows for padding and for positions outside every document; val[p] = the row of the gradient that
 // position p's table row took part in.  With count given, the documents' named ids are counted (whole numbers: the order
 // of the atomics does not matter; one atomic per wave where the wave lies in one document).
-template <typename ID>
-__global__ __launch_bounds__(256) void grad_keys_kernel(const ID* __restrict__ ids, uint64_t n_ids, uint64_t n_rows, const uint64_t* __restrict__ offsets,
+__global__ __launch_bounds__(256) void grad_keys_kernel(const void* __restrict__ ids, int id_bytes, uint64_t n_ids, uint64_t n_rows, const uint64_t* __restrict__ offsets,
                                                         uint64_t n_docs, uint32_t* __restrict__ count, uint32_t* __restrict__ key, uint32_t* __restrict__ val) {
     const uint64_t p = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     uint64_t row = p;
     bool named = false;
     if (p < n_ids) {
-        const uint64_t id = (uint64_t)(int64_t)ids[p];
-        named = id < n_rows;
+        const uint32_t id = named_row(ids, id_bytes, p, n_rows);
+        named = id != NO_ROW;
         if (offsets) {
             row = doc_at(offsets, n_docs, p);
             uint64_t beg = 0, end = 0;
             if (row < n_docs) doc_range(offsets, row, n_ids, beg, end);
             if (p < beg || p >= end) named = false;
         }
-        key[p] = named ? (uint32_t)id : (uint32_t)n_rows;
+        key[p] = named ? id : (uint32_t)n_rows;
         val[p] = named ? (uint32_t)row : 0u;
     }
     if (!count) return;
@@ -462,10 +526,10 @@ __global__ __launch_bounds__(256) void grad_starts_kernel(const uint32_t* __rest
 
 // ------------------------------------------------------------------------------------------------ launching the sums
 uint32_t piece_log2_for(uint64_t n_ids) {
-    // about 8192 pieces (two waves for each of the 4096 that the chip holds at sixteen per CU) of 32 to 1024 ids: short
-    // enough to spread one long document over the chip, long enough that the shares stay a fraction of the rows read
+    // A document of all ids takes a wave's time for a piece, then a quarter of its n_ids / piece shares: shortest with pieces of
+    // sqrt(n_ids) / 2.  32 to 1024 ids: fewer would make the shares as many as the rows, more gains nothing
     uint32_t b = 5;
-    while (b < 10 && (n_ids >> b) > 8192) b++;
+    while (b < 10 && (4ull << (2 * b)) < n_ids) b++;
     return b;
 }
 uint64_t n_pieces_for(uint64_t n_ids) {
@@ -474,37 +538,36 @@ uint64_t n_pieces_for(uint64_t n_ids) {
 }
 uint64_t pool_ws_bytes(uint64_t n_ids, uint32_t dim) {
     const uint64_t p = n_pieces_for(n_ids);
-    return p ? round_up(p * 2 * dim * 4, 256) + round_up(p * 2 * 4, 256) : 0;
+    return p ? round_up(p * 2 * dim * 4, 256) + round_up(p * 2 * 4, 256) + round_up(p * 8, 256) : 0;
+}
+void place_parts(PoolArgs& a, uint8_t* ws) {
+    a.part = reinterpret_cast<float*>(ws);
+    a.part_n = reinterpret_cast<uint32_t*>(ws + round_up(a.n_pieces * 2 * a.dim * 4, 256));
+    a.begins = reinterpret_cast<uint64_t*>(ws + round_up(a.n_pieces * 2 * a.dim * 4, 256) + round_up(a.n_pieces * 2 * 4, 256));
 }
 
-template <typename T, typename ID, typename O>
+uint32_t lanes_per_row(uint32_t dim) { return dim > 256 ? 64 : dim > 128 ? 32 : dim > 64 ? 16 : 8; }
+
+template <typename T, typename O, bool WEIGHTED>
 void launch_pool(hipStream_t s, const PoolArgs& a) {
-    const uint32_t slabs = (a.dim + 511) / 512, chunks = (a.dim + 7) / 8;
-    const uint64_t cap = (1u << 20) / slabs + 1;
-    const uint64_t want = (a.n_pieces + a.n_docs + 3) / 4;
+    const uint32_t ns = a.dim > 512 ? 2 : 1, slabs = (a.dim + 512 * ns - 1) / (512 * ns);
+    const uint64_t cap = (1u << 20) / slabs + 1, want = (a.n_pieces + a.n_docs + 3) / 4;
     const dim3 grid((unsigned)(want < cap ? want : cap), slabs), block(256);
-    if (chunks > 32) hipLaunchKernelGGL((pool_kernel<T, ID, O, 64>), grid, block, 0, s, a);
-    else if (chunks > 16) hipLaunchKernelGGL((pool_kernel<T, ID, O, 32>), grid, block, 0, s, a);
-    else if (chunks > 8) hipLaunchKernelGGL((pool_kernel<T, ID, O, 16>), grid, block, 0, s, a);
-    else if (chunks > 4) hipLaunchKernelGGL((pool_kernel<T, ID, O, 8>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((pool_kernel<T, ID, O, 4>), grid, block, 0, s, a);
+    if (ns == 2) hipLaunchKernelGGL((pool_kernel<T, O, 2, WEIGHTED>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((pool_kernel<T, O, 1, WEIGHTED>), grid, block, 0, s, a);
     if (a.n_pieces) {
-        const uint64_t docs = (a.n_docs + 3) / 4;
-        hipLaunchKernelGGL((pool_join_kernel<O>), dim3((unsigned)(docs < cap ? docs : cap), slabs), block, 0, s, a);
+        const uint32_t slabs = (a.dim + 511) / 512;
+        const uint64_t cap = (1u << 20) / slabs + 1;
+        hipLaunchKernelGGL((pool_join_kernel<O>), dim3((unsigned)(a.n_pieces < cap ? a.n_pieces : cap), slabs), dim3(256), 0, s, a);
     }
 }
 
-template <typename T, typename ID>
-void launch_lookup(hipStream_t s, const T* table, uint64_t n_rows, uint64_t stride, uint32_t dim, const ID* ids, uint64_t n_ids, float scale, T* out) {
-    const uint32_t slabs = (dim + 511) / 512, chunks = (dim + 7) / 8;
-    const uint32_t lpr = chunks > 32 ? 64 : chunks > 16 ? 32 : chunks > 8 ? 16 : chunks > 4 ? 8 : 4;
-    const uint64_t per_block = 4ull * (64 / lpr) * (lpr < 8 ? lpr : 8), cap = (1u << 22) / slabs + 1, want = (n_ids + per_block - 1) / per_block;
+template <typename T>
+void launch_lookup(hipStream_t s, const T* table, uint64_t n_rows, uint64_t stride, uint32_t dim, const void* ids, int id_bytes, uint64_t n_ids, float scale, T* out) {
+    const uint32_t slabs = (dim + 511) / 512, lpr = lanes_per_row(dim);
+    const uint64_t per_block = 4ull * (64 / lpr) * 8, cap = (1u << 22) / slabs + 1, want = (n_ids + per_block - 1) / per_block;
     const dim3 grid((unsigned)(want < cap ? want : cap), slabs), block(256);
-    if (lpr == 64) hipLaunchKernelGGL((lookup_kernel<T, ID, 64>), grid, block, 0, s, table, n_rows, stride, dim, ids, n_ids, scale, out);
-    else if (lpr == 32) hipLaunchKernelGGL((lookup_kernel<T, ID, 32>), grid, block, 0, s, table, n_rows, stride, dim, ids, n_ids, scale, out);
-    else if (lpr == 16) hipLaunchKernelGGL((lookup_kernel<T, ID, 16>), grid, block, 0, s, table, n_rows, stride, dim, ids, n_ids, scale, out);
-    else if (lpr == 8) hipLaunchKernelGGL((lookup_kernel<T, ID, 8>), grid, block, 0, s, table, n_rows, stride, dim, ids, n_ids, scale, out);
-    else hipLaunchKernelGGL((lookup_kernel<T, ID, 4>), grid, block, 0, s, table, n_rows, stride, dim, ids, n_ids, scale, out);
+    hipLaunchKernelGGL((lookup_kernel<T>), grid, block, 0, s, table, n_rows, stride, dim, lpr, ids, id_bytes, n_ids, scale, out);
 }
 
 // ------------------------------------------------------------------------------------------------ norm
@@ -765,7 +828,8 @@ dim3 row_grid(uint64_t n, int W) {
 }
 
 // ------------------------------------------------------------------------------------------------ edge cosines
-// Sixteen lanes take an edge, 16 bytes of both rows a step: four edges a wave.  Bound by the gather of two rows per edge.
+// Sixteen lanes take an edge: four edges a wave, 1024 columns of both rows in flight at once.  Bound by the gather of two rows
+// per edge.
 __device__ __forceinline__ u32x4 load_bytes16(const uint8_t* __restrict__ p, uint32_t n) {
     typedef uint32_t any __attribute__((ext_vector_type(4), aligned(1)));
     u32x4 v = 0;
@@ -791,39 +855,41 @@ __global__ __launch_bounds__(256) void edge_cosine_kernel(const uint8_t* __restr
         const uint64_t u = eu[e], v = ev[e];
         const bool ok = u < n_rows && v < n_rows;
         const uint8_t *a = codes + (ok ? u : 0) * stride, *b = codes + (ok ? v : 0) * stride;
-        float ab, aa, bb;
-        if (KIND == MDD_I8) {
-            int iab = 0, iaa = 0, ibb = 0;  // 32768 products of at most 2^14: below 2^30
-            for (uint32_t c = t * 16; c < (ok ? dim : 0); c += 256) {
-                const u32x4 x = load_bytes16(a + c, dim - c), y = load_bytes16(b + c, dim - c);
+        float ab = 0, aa = 0, bb = 0;
+        int iab = 0, iaa = 0, ibb = 0;  // 32768 products of at most 2^14: below 2^30
+        for (uint32_t c0 = t * 16; c0 < (ok ? dim : 0); c0 += 1024) {
+            u32x4 x[4], y[4];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    iab = __builtin_amdgcn_sdot4((int)x[k], (int)y[k], iab, false);
-                    iaa = __builtin_amdgcn_sdot4((int)x[k], (int)x[k], iaa, false);
-                    ibb = __builtin_amdgcn_sdot4((int)y[k], (int)y[k], ibb, false);
-                }
+            for (int s = 0; s < 4; s++) {
+                const uint32_t c = c0 + s * 256;
+                x[s] = 0, y[s] = 0;
+                if (c < dim) x[s] = load_bytes16(a + c, dim - c), y[s] = load_bytes16(b + c, dim - c);
             }
 #pragma unroll
-            for (int m = 8; m; m >>= 1) iab += __shfl_xor(iab, m, 64), iaa += __shfl_xor(iaa, m, 64), ibb += __shfl_xor(ibb, m, 64);
-            ab = (float)iab, aa = (float)iaa, bb = (float)ibb;
-        } else {
-            ab = aa = bb = 0;
-            for (uint32_t c = t * 16; c < (ok ? dim : 0); c += 256) {
-                const u32x4 x = load_bytes16(a + c, dim - c), y = load_bytes16(b + c, dim - c);
+            for (int s = 0; s < 4; s++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    auto x0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[k], false), x1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[k], true);
-                    auto y0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)y[k], false), y1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)y[k], true);
+                    if (KIND == MDD_I8) {
+                        iab = __builtin_amdgcn_sdot4((int)x[s][k], (int)y[s][k], iab, false);
+                        iaa = __builtin_amdgcn_sdot4((int)x[s][k], (int)x[s][k], iaa, false);
+                        ibb = __builtin_amdgcn_sdot4((int)y[s][k], (int)y[s][k], ibb, false);
+                    } else {
+                        auto x0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[s][k], false), x1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[s][k], true);
+                        auto y0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)y[s][k], false), y1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)y[s][k], true);
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        ab = fmaf(x0[i], y0[i], ab), aa = fmaf(x0[i], x0[i], aa), bb = fmaf(y0[i], y0[i], bb);
-                        ab = fmaf(x1[i], y1[i], ab), aa = fmaf(x1[i], x1[i], aa), bb = fmaf(y1[i], y1[i], bb);
+                        for (int i = 0; i < 2; i++) {
+                            ab = fmaf(x0[i], y0[i], ab), aa = fmaf(x0[i], x0[i], aa), bb = fmaf(y0[i], y0[i], bb);
+                            ab = fmaf(x1[i], y1[i], ab), aa = fmaf(x1[i], x1[i], aa), bb = fmaf(y1[i], y1[i], bb);
+                        }
                     }
                 }
-            }
-#pragma unroll
-            for (int m = 8; m; m >>= 1) ab += __shfl_xor(ab, m, 64), aa += __shfl_xor(aa, m, 64), bb += __shfl_xor(bb, m, 64);
         }
+#pragma unroll
+        for (int m = 8; m; m >>= 1) {
+            if (KIND == MDD_I8) iab += __shfl_xor(iab, m, 64), iaa += __shfl_xor(iaa, m, 64), ibb += __shfl_xor(ibb, m, 64);
+            else ab += __shfl_xor(ab, m, 64), aa += __shfl_xor(aa, m, 64), bb += __shfl_xor(bb, m, 64);
+        }
+        if (KIND == MDD_I8) ab = (float)iab, aa = (float)iaa, bb = (float)ibb;
         // a product of the squares stays below 2^63, and a NaN in a row comes through
         if (t == 0) cosines[e] = !ok || aa == 0.0f || bb == 0.0f ? 0.0f : ab / sqrtf(aa * bb);
     }
@@ -875,20 +941,14 @@ int mdd_embed(mdd_ctx* ctx, const void* table, int type, uint64_t n_rows, uint64
         return MDD_OK;
     }
     if (!offsets) {
-        MDD_FOR_TYPE(type, T, {
-            if (id_bytes == 4) launch_lookup<T, int32_t>(ctx->stream, (const T*)table, n_rows, row_stride, dim, (const int32_t*)ids, n_ids, scale, (T*)out);
-            else launch_lookup<T, int64_t>(ctx->stream, (const T*)table, n_rows, row_stride, dim, (const int64_t*)ids, n_ids, scale, (T*)out);
-        });
+        MDD_FOR_TYPE(type, T, launch_lookup<T>(ctx->stream, (const T*)table, n_rows, row_stride, dim, ids, id_bytes, n_ids, scale, (T*)out));
         HIP_TRY(hipGetLastError());
         return MDD_OK;
     }
-    PoolArgs a = {table, n_rows, row_stride, dim, ids, n_ids, offsets, n_docs, mean, scale, nullptr, piece_log2_for(n_ids), n_pieces_for(n_ids), (float*)ws,
-                  nullptr, out};
-    if (a.n_pieces) a.part_n = reinterpret_cast<uint32_t*>((uint8_t*)ws + round_up(a.n_pieces * 2 * dim * 4, 256));
-    MDD_FOR_TYPE(type, T, {
-        if (id_bytes == 4) launch_pool<T, int32_t, T>(ctx->stream, a);
-        else launch_pool<T, int64_t, T>(ctx->stream, a);
-    });
+    PoolArgs a = {table, n_rows, row_stride, dim, lanes_per_row(dim), ids, id_bytes, n_ids, offsets, n_docs, mean, scale, nullptr, piece_log2_for(n_ids), n_pieces_for(n_ids), nullptr,
+                  nullptr, nullptr, out};
+    if (a.n_pieces) place_parts(a, (uint8_t*)ws);
+    MDD_FOR_TYPE(type, T, (launch_pool<T, T, false>(ctx->stream, a)));
     HIP_TRY(hipGetLastError());
     return MDD_OK;
 }
@@ -943,19 +1003,16 @@ int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_s
     uint32_t* count = mean && offsets ? (uint32_t*)(base + at[3]) : nullptr;
     if (count) hipLaunchKernelGGL((fill_kernel<uint32_t>), dim3((unsigned)(n_docs / 256 + 1 < 4096 ? n_docs / 256 + 1 : 4096)), dim3(256), 0, s, count, n_docs, 0u);
     const dim3 per_id(grid_for(n_ids, 256));
-    if (id_bytes == 4)
-        hipLaunchKernelGGL((grad_keys_kernel<int32_t>), per_id, dim3(256), 0, s, (const int32_t*)ids, n_ids, n_rows, offsets, n_docs, count, key, val);
-    else
-        hipLaunchKernelGGL((grad_keys_kernel<int64_t>), per_id, dim3(256), 0, s, (const int64_t*)ids, n_ids, n_rows, offsets, n_docs, count, key, val);
+    hipLaunchKernelGGL(grad_keys_kernel, per_id, dim3(256), 0, s, ids, id_bytes, n_ids, n_rows, offsets, n_docs, count, key, val);
     sort_pairs(s, key, val, key2, val2, n_ids, bits_of(n_rows), (uint32_t*)(base + at[1]));
     hipLaunchKernelGGL(grad_starts_kernel, dim3(grid_for(n_rows + 1, 256)), dim3(256), 0, s, key, (uint32_t)n_ids, n_rows, start);
     // the sums themselves are a lookup: table rows are the documents, the sorted positions their ids, grad the table
-    PoolArgs a = {grad, n_grad, grad_stride, dim, val, n_ids, start, n_rows, 0, scale, count, piece_log2_for(n_ids), n_pieces_for(n_ids),
-                  (float*)(base + at[4]), nullptr, table_grad};
-    if (a.n_pieces) a.part_n = reinterpret_cast<uint32_t*>(base + at[4] + round_up(a.n_pieces * 2 * dim * 4, 256));
+    PoolArgs a = {grad, n_grad, grad_stride, dim, lanes_per_row(dim), val, 4, n_ids, start, n_rows, 0, scale, count, piece_log2_for(n_ids), n_pieces_for(n_ids),
+                  nullptr, nullptr, nullptr, table_grad};
+    if (a.n_pieces) place_parts(a, base + at[4]);
     MDD_FOR_TYPE(type, T, {
-        if (out_type == MDD_F32) launch_pool<T, int32_t, float>(s, a);
-        else launch_pool<T, int32_t, T>(s, a);
+        if (out_type == MDD_F32) count ? launch_pool<T, float, true>(s, a) : launch_pool<T, float, false>(s, a);
+        else count ? launch_pool<T, T, true>(s, a) : launch_pool<T, T, false>(s, a);
     });
     HIP_TRY(hipGetLastError());
     return MDD_OK;
@@ -1087,6 +1144,11 @@ int mdd_sort_edges(mdd_ctx* ctx, uint32_t* edge_u, uint32_t* edge_v, uint64_t n_
     ON_DEVICE(ctx);
     const int bits = bits_of(n_docs ? n_docs - 1 : 0);
     uint32_t *u = edge_u, *v = edge_v, *v2 = (uint32_t*)ws, *u2 = v2 + round_up(n_edges, 64), *hist = u2 + round_up(n_edges, 64);
+    if (n_edges <= SMALL_SORT) {
+        hipLaunchKernelGGL(small_sort_kernel, dim3(1), dim3(1024), 0, ctx->stream, edge_u, edge_v, (uint32_t)n_edges, bits, bits);
+        HIP_TRY(hipGetLastError());
+        return MDD_OK;
+    }
     // by the second column, then stably by the first; the passes of both together are even in number, so the result ends up
     // in the caller's arrays
     sort_pairs(ctx->stream, v, u, v2, u2, n_edges, bits, hist);
