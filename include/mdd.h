@@ -473,7 +473,8 @@ int mdd_jsonl_decode(mdd_ctx* ctx, const uint8_t* raw, uint64_t raw_bytes, uint6
  *   offsets given   document d = ids [offsets[d], offsets[d+1]) as for the packed text (n_docs + 1 ascending entries,
  *                   clamped to n_ids): out[d] = f * sum of its rows, f = scale, or with mean != 0 scale / (its ids that
  *                   name a row).  A document without such an id gives zeros.
- * The order of every sum depends on the sizes alone, so results repeat bit for bit.  n_ids < 2^31. */
+ * The order of every sum depends on the sizes alone, so results repeat bit for bit.  n_ids < 2^31,
+ * row_stride < 2^30. */
 uint64_t mdd_embed_ws_bytes(uint64_t n_ids, uint32_t dim);
 int mdd_embed(mdd_ctx* ctx, const void* table, int type, uint64_t n_rows, uint64_t row_stride, uint32_t dim, const void* ids,
               int id_bytes, uint64_t n_ids, const uint64_t* offsets, uint64_t n_docs, int mean, float scale, void* out,
@@ -481,7 +482,7 @@ int mdd_embed(mdd_ctx* ctx, const void* table, int type, uint64_t n_rows, uint64
 /* Its gradient with respect to the table: table_grad [n_rows, dim] (out_type: MDD_F32 or `type`) is overwritten,
  *   table_grad[v] = sum over the positions p with ids[p] == v of f(p) * grad[row(p)],  row(p) = p or p's document.
  * The positions are sorted by id (stable), so each row is summed in the order of the positions: no floating atomics.
- * n_rows < 2^31, n_docs < 2^31. */
+ * n_rows < 2^31, n_docs < 2^31, grad_stride < 2^30. */
 uint64_t mdd_embed_backward_ws_bytes(uint64_t n_ids, uint64_t n_docs, uint64_t n_rows, uint32_t dim);
 int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_stride, uint32_t dim, const void* ids, int id_bytes,
                        uint64_t n_ids, const uint64_t* offsets, uint64_t n_docs, int mean, float scale, void* table_grad,

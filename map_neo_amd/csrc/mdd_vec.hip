@@ -25,7 +25,8 @@ constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
 // document strictly inside a piece is not long.
 struct PoolArgs {
     const void* table;
-    uint64_t n_rows, stride;
+    uint64_t n_rows;
+    uint32_t row_bytes;  // from a table row to the next
     uint32_t dim, lpr;
     const void* ids;
     int id_bytes;
@@ -49,23 +50,37 @@ __device__ __forceinline__ uint32_t named_row(const void* ids, int id_bytes, uin
     return id < n_rows ? (uint32_t)id : NO_ROW;
 }
 
-// U rows per lane group, `first + u * step` of the 64 that the lanes hold.  ALL: every one of them is named; otherwise NO_ROW is
-// among them, for which row 0 is read and dropped, whatever it holds, NaN included.
-template <typename T, int NS, bool WEIGHTED, bool ALL, int U>
-__device__ __forceinline__ void add_rows(const T* __restrict__ table, uint64_t stride, uint32_t held, float weight, int first, int step, const uint32_t (&n_cols)[NS],
-                                         f32x8 (&acc)[NS]) {
+//
+// A lane's eight columns never reach over the row's end: the last lane starts early enough, and where that makes it overlap its
+// neighbour both compute and store the same numbers.  So every access is one of eight elements, without a branch.  Rows
+// narrower than that (NARROW) take a path of single elements.
+template <bool NARROW>
+__device__ __forceinline__ uint32_t lane_col(uint32_t col, uint32_t dim) {
+    return NARROW ? 0 : col < dim - 8 ? col : dim - 8;
+}
+template <typename T, bool NARROW>
+__device__ __forceinline__ typename vec8<T>::raw load_cols(const T* __restrict__ p, uint32_t dim) {
+    return load8_raw<T>(p, NARROW ? dim : 8);
+}
+
+// U rows per lane group, held by the lanes from byte lane index `first` on in steps of `step`.  ALL: every one of them is
+// named; otherwise NO_ROW is among them, for which row 0 is read and dropped, whatever it holds, NaN included.
+template <typename T, int NS, bool WEIGHTED, bool NARROW, bool ALL, int U>
+__device__ __forceinline__ void add_rows(const PoolArgs& a, const T* __restrict__ (&table)[NS], uint32_t held, float weight, int first, int step, f32x8 (&acc)[NS]) {
     typename vec8<T>::raw raw[U][NS];
     uint32_t at[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        at[u] = __shfl(held, first + u * step, 64);
-        const T* row = table + (uint64_t)(ALL || at[u] != NO_ROW ? at[u] : 0) * stride;
+    for (int u = 0; u < U; u++) at[u] = (uint32_t)__builtin_amdgcn_ds_bpermute(first + u * step, (int)held);
 #pragma unroll
-        for (int n = 0; n < NS; n++) raw[u][n] = load8_raw<T>(row + n * 512, n_cols[n]);
+    for (int u = 0; u < U; u++) {
+        const uint64_t off = (uint64_t)(ALL || at[u] != NO_ROW ? at[u] : 0) * a.row_bytes;
+#pragma unroll
+        for (int n = 0; n < NS; n++) raw[u][n] = load_cols<T, NARROW>(reinterpret_cast<const T*>(reinterpret_cast<const uint8_t*>(table[n]) + off), a.dim);
     }
+    __builtin_amdgcn_sched_barrier(0);  // all loads first: left alone, the compiler takes them one by one to save registers
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const float w = WEIGHTED ? __shfl(weight, first + u * step, 64) : 1.0f;
+        const float w = WEIGHTED ? __int_as_float(__builtin_amdgcn_ds_bpermute(first + u * step, __float_as_int(weight))) : 1.0f;
 #pragma unroll
         for (int n = 0; n < NS; n++) {
             f32x8 v = __builtin_convertvector(raw[u][n], f32x8);
@@ -79,14 +94,13 @@ __device__ __forceinline__ void add_rows(const T* __restrict__ table, uint64_t s
 }
 
 // sum of the rows named by ids [beg, end) in this lane's columns; n_named = ids that name a row.  Call with all lanes.
-template <typename T, int NS, bool WEIGHTED>
-__device__ __forceinline__ void sum_span(const PoolArgs& a, uint64_t beg, uint64_t end, uint32_t col, f32x8 (&acc)[NS], uint32_t& n_named) {
+template <typename T, int NS, bool WEIGHTED, bool NARROW>
+__device__ __forceinline__ void sum_span(const PoolArgs& a, uint64_t beg, uint64_t end, const uint32_t (&col)[NS], f32x8 (&acc)[NS], uint32_t& n_named) {
     const int lane = (int)lane_id(), lpr = NS == 2 ? 64 : (int)a.lpr, G = 64 / lpr, g = lane / lpr;
-    const T* __restrict__ table = reinterpret_cast<const T*>(a.table) + (col < a.dim ? col : 0);
-    uint32_t n_cols[NS];
+    const T* __restrict__ table[NS];
 #pragma unroll
     for (int n = 0; n < NS; n++) {
-        n_cols[n] = col + n * 512 < a.dim ? a.dim - col - n * 512 : 0;
+        table[n] = reinterpret_cast<const T*>(a.table) + col[n];
         acc[n] = 0.0f;
     }
     n_named = 0;
@@ -107,11 +121,13 @@ __device__ __forceinline__ void sum_span(const PoolArgs& a, uint64_t beg, uint64
         // no row read twice), and last the groups that get one row more than the others
         const int steps = n / G;
         int j = 0;
-        for (; j + 8 <= steps; j += 8) add_rows<T, NS, WEIGHTED, true, 8>(table, a.stride, row, w, j * G + g, G, n_cols, acc);
-        if (j + 4 <= steps) add_rows<T, NS, WEIGHTED, true, 4>(table, a.stride, row, w, j * G + g, G, n_cols, acc), j += 4;
-        if (j + 2 <= steps) add_rows<T, NS, WEIGHTED, true, 2>(table, a.stride, row, w, j * G + g, G, n_cols, acc), j += 2;
-        if (j < steps) add_rows<T, NS, WEIGHTED, true, 1>(table, a.stride, row, w, j * G + g, G, n_cols, acc), j++;
-        if (j * G < n) add_rows<T, NS, WEIGHTED, false, 1>(table, a.stride, row, w, j * G + g, G, n_cols, acc);
+        if constexpr (!NARROW) {
+            for (; j + 8 <= steps; j += 8) add_rows<T, NS, WEIGHTED, NARROW, true, 8>(a, table, row, w, (j * G + g) * 4, G * 4, acc);
+            if (j + 4 <= steps) add_rows<T, NS, WEIGHTED, NARROW, true, 4>(a, table, row, w, (j * G + g) * 4, G * 4, acc), j += 4;
+            if (j + 2 <= steps) add_rows<T, NS, WEIGHTED, NARROW, true, 2>(a, table, row, w, (j * G + g) * 4, G * 4, acc), j += 2;
+        }
+        for (; j < steps; j++) add_rows<T, NS, WEIGHTED, NARROW, true, 1>(a, table, row, w, (j * G + g) * 4, G * 4, acc);
+        if (j * G < n) add_rows<T, NS, WEIGHTED, NARROW, false, 1>(a, table, row, w, (j * G + g) * 4, G * 4, acc);
         row = next;
     }
     for (int m = lpr; m < 64; m <<= 1)
@@ -150,16 +166,24 @@ __device__ __forceinline__ uint64_t wave_doc_at(const uint64_t* __restrict__ off
     return lo ? lo - 1 : n_docs;
 }
 
-template <typename O, int NS>
-__device__ __forceinline__ void store_cols(O* __restrict__ row, uint32_t col, uint32_t dim, const f32x8 (&v)[NS], float f) {
+template <typename O, int NS, bool NARROW>
+__device__ __forceinline__ void store_cols(O* __restrict__ row, const uint32_t (&col)[NS], const bool (&in)[NS], uint32_t dim, const f32x8 (&v)[NS], float f) {
 #pragma unroll
     for (int n = 0; n < NS; n++)
-        if (col + n * 512 < dim) store8<O>(row + col + n * 512, dim - col - n * 512, v[n] * f);
+        if (in[n]) store8<O>(row + col[n], NARROW ? dim : 8, v[n] * f);
 }
 
-template <typename T, typename O, int NS, bool WEIGHTED>
+template <typename T, typename O, int NS, bool WEIGHTED, bool NARROW>
 __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
-    const uint32_t lane = lane_id(), lpr = NS == 2 ? 64 : a.lpr, col = blockIdx.y * (512u * NS) + (lane & (lpr - 1)) * 8u;
+    const uint32_t lane = lane_id(), lpr = NS == 2 ? 64 : a.lpr;
+    uint32_t col[NS];
+    bool in[NS];
+#pragma unroll
+    for (int n = 0; n < NS; n++) {
+        const uint32_t c = blockIdx.y * (512u * NS) + n * 512 + (lane & (lpr - 1)) * 8u;
+        col[n] = lane_col<NARROW>(c, a.dim);
+        in[n] = lane < lpr && c < a.dim;
+    }
     const uint64_t n_work = a.n_pieces + a.n_docs, stride = (uint64_t)gridDim.x * 4;
     const uint64_t piece = 1ull << a.piece_log2;
     for (uint64_t w = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; w < n_work; w += stride) {
@@ -179,9 +203,9 @@ __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
                 if (beg >= lo && beg < hi) begins = d;
                 beg = beg > lo ? beg : lo;
                 end = end < hi ? end : hi;
-                sum_span<T, NS, WEIGHTED>(a, beg, end, col, acc, n_named);
+                sum_span<T, NS, WEIGHTED, NARROW>(a, beg, end, col, acc, n_named);
                 const uint64_t at = w * 2 + slot;
-                if (lane < lpr) store_cols<float, NS>(a.part + at * a.dim, col, a.dim, acc, 1.0f);
+                store_cols<float, NS, NARROW>(a.part + at * a.dim, col, in, a.dim, acc, 1.0f);
                 if (lane == 0 && blockIdx.y == 0) a.part_n[at] = n_named;
             }
             if (lane == 0 && blockIdx.y == 0) a.begins[w] = begins;
@@ -190,8 +214,8 @@ __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
             uint64_t beg, end;
             doc_range(a.offsets, d, a.n_ids, beg, end);
             if (a.n_pieces && end - beg > piece) continue;  // pool_join_kernel writes it
-            sum_span<T, NS, WEIGHTED>(a, beg, end, col, acc, n_named);
-            if (lane < lpr) store_cols<O, NS>(reinterpret_cast<O*>(a.out) + d * a.dim, col, a.dim, acc, pool_factor(a, n_named));
+            sum_span<T, NS, WEIGHTED, NARROW>(a, beg, end, col, acc, n_named);
+            store_cols<O, NS, NARROW>(reinterpret_cast<O*>(a.out) + d * a.dim, col, in, a.dim, acc, pool_factor(a, n_named));
         }
     }
 }
@@ -242,29 +266,28 @@ __global__ __launch_bounds__(256) void pool_join_kernel(PoolArgs a) {
 }
 
 // One row per id: eight rows per lane group in flight, read and written once -- bound by HBM where the table is large.
-template <typename T>
-__global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table, uint64_t n_rows, uint64_t row_stride, uint32_t dim, uint32_t lpr,
+template <typename T, bool NARROW>
+__global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table, uint64_t n_rows, uint32_t row_bytes, uint32_t dim, uint32_t lpr,
                                                      const void* __restrict__ ids, int id_bytes, uint64_t n_ids, float scale, T* __restrict__ out) {
     constexpr uint32_t U = 8;  // U * G positions per wave and round, 64 at most: lpr is 8 to 64
-    const uint32_t G = 64 / lpr, lane = lane_id(), g = lane / lpr, col = blockIdx.y * 512u + (lane & (lpr - 1)) * 8u;
+    const uint32_t G = 64 / lpr, lane = lane_id(), g = lane / lpr, c = blockIdx.y * 512u + (lane & (lpr - 1)) * 8u, col = lane_col<NARROW>(c, dim);
     const uint64_t stride = (uint64_t)gridDim.x * 4 * (U * G);
     for (uint64_t p = ((uint64_t)blockIdx.x * 4 + threadIdx.x / 64) * (U * G); p < n_ids; p += stride) {
         const uint32_t row = lane < U * G && p + lane < n_ids ? named_row(ids, id_bytes, p + lane, n_rows) : NO_ROW;
         uint32_t r[U];
         typename vec8<T>::raw raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            r[u] = __shfl(row, u * G + g, 64);
-            raw[u] = 0;
-            if (r[u] != NO_ROW && col < dim) raw[u] = load8_raw<T>(table + r[u] * row_stride + col, dim - col);
-        }
-        if (col < dim) {
+        for (uint32_t u = 0; u < U; u++) r[u] = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(u * G + g) * 4, (int)row);
 #pragma unroll
-            for (int u = 0; u < U; u++)
+        for (uint32_t u = 0; u < U; u++)
+            raw[u] = load_cols<T, NARROW>(reinterpret_cast<const T*>(reinterpret_cast<const uint8_t*>(table + col) + (uint64_t)(r[u] != NO_ROW ? r[u] : 0) * row_bytes), dim);
+        if (c < dim) {
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++)
                 if (p + u * G + g < n_ids) {
                     f32x8 v = __builtin_convertvector(raw[u], f32x8) * scale;
-                    if (r[u] == NO_ROW) v = 0.0f;  // also where the scale is no number
-                    store8<T>(out + (p + u * G + g) * dim + col, dim - col, v);
+                    if (r[u] == NO_ROW) v = 0.0f;  // whatever row 0 and the scale hold
+                    store8<T>(out + (p + u * G + g) * dim + col, NARROW ? dim : 8, v);
                 }
         }
     }
@@ -553,8 +576,9 @@ void launch_pool(hipStream_t s, const PoolArgs& a) {
     const uint32_t ns = a.dim > 512 ? 2 : 1, slabs = (a.dim + 512 * ns - 1) / (512 * ns);
     const uint64_t cap = (1u << 20) / slabs + 1, want = (a.n_pieces + a.n_docs + 3) / 4;
     const dim3 grid((unsigned)(want < cap ? want : cap), slabs), block(256);
-    if (ns == 2) hipLaunchKernelGGL((pool_kernel<T, O, 2, WEIGHTED>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((pool_kernel<T, O, 1, WEIGHTED>), grid, block, 0, s, a);
+    if (a.dim < 8) hipLaunchKernelGGL((pool_kernel<T, O, 1, WEIGHTED, true>), grid, block, 0, s, a);
+    else if (ns == 2) hipLaunchKernelGGL((pool_kernel<T, O, 2, WEIGHTED, false>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((pool_kernel<T, O, 1, WEIGHTED, false>), grid, block, 0, s, a);
     if (a.n_pieces) {
         const uint32_t slabs = (a.dim + 511) / 512;
         const uint64_t cap = (1u << 20) / slabs + 1;
@@ -567,7 +591,8 @@ void launch_lookup(hipStream_t s, const T* table, uint64_t n_rows, uint64_t stri
     const uint32_t slabs = (dim + 511) / 512, lpr = lanes_per_row(dim);
     const uint64_t per_block = 4ull * (64 / lpr) * 8, cap = (1u << 22) / slabs + 1, want = (n_ids + per_block - 1) / per_block;
     const dim3 grid((unsigned)(want < cap ? want : cap), slabs), block(256);
-    hipLaunchKernelGGL((lookup_kernel<T>), grid, block, 0, s, table, n_rows, stride, dim, lpr, ids, id_bytes, n_ids, scale, out);
+    auto kernel = dim < 8 ? lookup_kernel<T, true> : lookup_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, s, table, n_rows, (uint32_t)(stride * sizeof(T)), dim, lpr, ids, id_bytes, n_ids, scale, out);
 }
 
 // ------------------------------------------------------------------------------------------------ norm
@@ -928,6 +953,7 @@ int mdd_embed(mdd_ctx* ctx, const void* table, int type, uint64_t n_rows, uint64
     REQUIRE(out && aligned_to(out, type_bytes(type)), "%s: out is NULL or not aligned to its elements", who);
     REQUIRE(n_ids == 0 || (ids && aligned_to(ids, id_bytes)), "%s: ids is NULL or not aligned", who);
     if (n_rows) CHECKED(check_matrix(who, "table", table, type, row_stride, dim));
+    REQUIRE(row_stride < (1u << 30), "%s: row stride of 2^30 elements or more", who);
     const uint64_t need = offsets && n_rows ? pool_ws_bytes(n_ids, dim) : 0;
     REQUIRE(need == 0 || (ws && aligned_to(ws, 256) && ws_bytes >= need), "%s: workspace of %llu bytes, 256-byte aligned, needed", who,
             (unsigned long long)need);
@@ -945,7 +971,7 @@ int mdd_embed(mdd_ctx* ctx, const void* table, int type, uint64_t n_rows, uint64
         HIP_TRY(hipGetLastError());
         return MDD_OK;
     }
-    PoolArgs a = {table, n_rows, row_stride, dim, lanes_per_row(dim), ids, id_bytes, n_ids, offsets, n_docs, mean, scale, nullptr, piece_log2_for(n_ids), n_pieces_for(n_ids), nullptr,
+    PoolArgs a = {table, n_rows, (uint32_t)(row_stride * type_bytes(type)), dim, lanes_per_row(dim), ids, id_bytes, n_ids, offsets, n_docs, mean, scale, nullptr, piece_log2_for(n_ids), n_pieces_for(n_ids), nullptr,
                   nullptr, nullptr, out};
     if (a.n_pieces) place_parts(a, (uint8_t*)ws);
     MDD_FOR_TYPE(type, T, (launch_pool<T, T, false>(ctx->stream, a)));
@@ -983,6 +1009,7 @@ int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_s
     if (!offsets) n_docs = 0;
     const uint64_t n_grad = offsets ? n_docs : n_ids;
     if (n_grad) CHECKED(check_matrix(who, "grad", grad, type, grad_stride, dim));
+    REQUIRE(grad_stride < (1u << 30), "%s: row stride of 2^30 elements or more", who);
     uint64_t at[5];
     const uint64_t need = n_ids && n_grad ? backward_parts(n_ids, n_docs, n_rows, dim, at) : 0;
     REQUIRE(need == 0 || (ws && aligned_to(ws, 256) && ws_bytes >= need), "%s: workspace of %llu bytes, 256-byte aligned, needed", who,
@@ -1007,7 +1034,7 @@ int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_s
     sort_pairs(s, key, val, key2, val2, n_ids, bits_of(n_rows), (uint32_t*)(base + at[1]));
     hipLaunchKernelGGL(grad_starts_kernel, dim3(grid_for(n_rows + 1, 256)), dim3(256), 0, s, key, (uint32_t)n_ids, n_rows, start);
     // the sums themselves are a lookup: table rows are the documents, the sorted positions their ids, grad the table
-    PoolArgs a = {grad, n_grad, grad_stride, dim, lanes_per_row(dim), val, 4, n_ids, start, n_rows, 0, scale, count, piece_log2_for(n_ids), n_pieces_for(n_ids),
+    PoolArgs a = {grad, n_grad, (uint32_t)(grad_stride * type_bytes(type)), dim, lanes_per_row(dim), val, 4, n_ids, start, n_rows, 0, scale, count, piece_log2_for(n_ids), n_pieces_for(n_ids),
                   nullptr, nullptr, nullptr, table_grad};
     if (a.n_pieces) place_parts(a, base + at[4]);
     MDD_FOR_TYPE(type, T, {

@@ -33,7 +33,7 @@ EMBED = dict(ctx=CTX, table=P, type=F32, n_rows=10, stride=64, dim=64, ids=P, id
 @pytest.mark.parametrize("change,needle", [
     (dict(ctx=None), "ctx is NULL"), (dict(dim=0), "dim=0"), (dict(dim=32769), "dim=32769"), (dict(type=3), "element type"), (dict(id_bytes=2), "id_bytes"),
     (dict(n_ids=2 ** 31), "2^31"), (dict(n_rows=2 ** 32 - 1), "2^32"), (dict(out=None), "out is NULL"), (dict(out=ODD), "aligned"), (dict(ids=None), "ids"),
-    (dict(ids=P + 2), "ids"), (dict(table=None), "table is NULL"), (dict(table=ODD), "aligned"), (dict(stride=63), "stride"), (dict(ws=None), "workspace"),
+    (dict(ids=P + 2), "ids"), (dict(table=None), "table is NULL"), (dict(table=ODD), "aligned"), (dict(stride=63), "stride"), (dict(stride=2 ** 30), "2^30"), (dict(ws=None), "workspace"),
     (dict(ws=P + 128), "workspace"), (dict(ws_bytes=100), "workspace")])
 def test_embed(change, needle):
     _refused(_call("mdd_embed", EMBED, **change), needle)
@@ -46,7 +46,7 @@ BACK = dict(ctx=CTX, grad=P, type=BF16, stride=64, dim=64, ids=P, id_bytes=8, n_
 @pytest.mark.parametrize("change,needle", [
     (dict(ctx=None), "ctx is NULL"), (dict(dim=0), "dim=0"), (dict(type=9), "element type"), (dict(out_type=2), "out_type"), (dict(id_bytes=1), "id_bytes"),
     (dict(n_ids=2 ** 31), "2^31"), (dict(n_docs=2 ** 31), "2^31"), (dict(n_rows=2 ** 31), "2^31"), (dict(out=None), "table_grad"), (dict(out=P + 2), "table_grad"),
-    (dict(ids=P + 4), "ids"), (dict(grad=None), "grad is NULL"), (dict(stride=1), "stride"), (dict(ws=None), "workspace"), (dict(ws_bytes=8), "workspace")])
+    (dict(ids=P + 4), "ids"), (dict(grad=None), "grad is NULL"), (dict(stride=1), "stride"), (dict(stride=2 ** 31), "2^30"), (dict(ws=None), "workspace"), (dict(ws_bytes=8), "workspace")])
 def test_embed_backward(change, needle):
     _refused(_call("mdd_embed_backward", BACK, **change), needle)
 
