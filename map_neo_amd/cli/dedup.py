@@ -54,6 +54,15 @@ def build_parser() -> argparse.ArgumentParser:
                         "ceil(min_jaccard * num_perm) components before the union-find; one-GPU path only.  Only the STAR edges of a bucket "
                         "are checked (each document against the smallest document of its bucket), not all pairs: two documents "
                         "that are similar to each other but not to that document are split, unlike pairwise LSH verification")
+    p.add_argument("--min_cosine", type=float, default=None,
+                   help="extension: documents whose vectors have a cosine of at least this are duplicates too (map_neo_amd.dedup."
+                        "vector_edges); needs --embeddings, or --embedding_table with --token_ids and --token_offsets; one-GPU path only")
+    p.add_argument("--embeddings", default=None,
+                   help=".npy, float32 or float16 [rows, dim]: a vector for every row of the input, in the order of the files and of the "
+                        "rows that are JSON objects in them (what n_rows of summary.json counts)")
+    p.add_argument("--embedding_table", default=None, help=".npy, float32 or float16 [vocabulary, dim]: a document's vector is the mean over its token ids")
+    p.add_argument("--token_ids", default=None, help=".npy, int32 or int64: the token ids of all rows back to back (ids outside the table are padding)")
+    p.add_argument("--token_offsets", default=None, help=".npy, int64 [rows + 1]: row k has the ids [token_offsets[k], token_offsets[k + 1])")
     p.add_argument("--device", type=int, default=0)
     p.add_argument("--workers", type=int, default=min(16, os.cpu_count() or 1))
     p.add_argument("--checkpoint_dir", default=None,
@@ -114,6 +123,50 @@ def _write_shard(task):
     return kept
 
 
+def _check_vector_args(args, distributed):
+    table = (args.embedding_table, args.token_ids, args.token_offsets)
+    given = bool(args.embeddings) + all(table)
+    if any(table) and not all(table):
+        raise SystemExit("--embedding_table, --token_ids and --token_offsets go together")
+    if (args.min_cosine is not None) != (given == 1) or given > 1:
+        raise SystemExit("--min_cosine needs either --embeddings or --embedding_table with --token_ids and --token_offsets, and they need it")
+    if args.min_cosine is None:
+        return
+    if not 0.0 < args.min_cosine <= 1.0:
+        raise SystemExit("--min_cosine must be in (0, 1]")
+    if distributed or args.checkpoint_dir or args.resume_from:
+        raise SystemExit("--min_cosine: single-process runs without --checkpoint_dir / --resume_from only")
+
+
+def _load_npy(path, dtypes, ndim):
+    a = np.load(path, mmap_mode="r", allow_pickle=False)
+    if a.ndim != ndim or a.dtype not in dtypes:
+        raise SystemExit("%s holds %s of %d dimensions, not %s of %d" % (path, a.dtype, a.ndim, " or ".join(np.dtype(t).name for t in dtypes), ndim))
+    return a
+
+
+def document_vectors(eng, args, rows, n_rows):
+    """device matrix [len(rows), dim]: the vectors of the input rows `rows` (of n_rows in all)"""
+    import torch
+    if args.embeddings:
+        emb = _load_npy(args.embeddings, (np.float32, np.float16), 2)
+        if emb.shape[0] != n_rows:
+            raise SystemExit("%s holds %d rows, the input %d" % (args.embeddings, emb.shape[0], n_rows))
+        out = torch.empty((len(rows), emb.shape[1]), dtype=torch.float32 if emb.dtype == np.float32 else torch.float16, device=eng.device)
+        for k in range(0, len(rows), 1 << 16):                   # gathered on the host a block at a time: the file may not fit its memory
+            block = np.ascontiguousarray(emb[rows[k: k + (1 << 16)]])
+            out[k: k + len(block)] = torch.from_numpy(block).to(eng.device)
+        return out
+    table = _load_npy(args.embedding_table, (np.float32, np.float16), 2)
+    ids, offs = _load_npy(args.token_ids, (np.int32, np.int64), 1), _load_npy(args.token_offsets, (np.int64,), 1)
+    if offs.size != n_rows + 1:
+        raise SystemExit("%s holds %d entries, not one more than the %d input rows" % (args.token_offsets, offs.size, n_rows))
+    if offs.size and (offs[0] < 0 or offs[-1] > ids.size or (np.diff(offs) < 0).any()):
+        raise SystemExit("%s does not ascend within the %d entries of %s" % (args.token_offsets, ids.size, args.token_ids))
+    up = lambda a: torch.from_numpy(np.array(a)).to(eng.device)
+    return eng.embed(up(table), up(ids), up(offs), mode="mean")[up(rows)]
+
+
 def run(args, engine_factory=None) -> dict:
     """Single process: one GPU.  Under torchrun (WORLD_SIZE > 1, or --distributed): one process per GPU, every rank
     ingests a contiguous block of the shards, band records are exchanged by all-to-all, the union-find is
@@ -136,6 +189,9 @@ def run(args, engine_factory=None) -> dict:
         raise SystemExit("--checkpoint_dir / --resume_from: single-process runs only")
     if resume and not ckpt_dir:
         raise SystemExit("--resume_from needs --checkpoint_dir")
+    min_cosine = getattr(args, "min_cosine", None)
+    if hasattr(args, "min_cosine"):
+        _check_vector_args(args, distributed)
     if files and all(f.lower().endswith((".parquet", ".pq")) for f in files):
         # Arrow decodes without the GIL and hands its buffers over without a copy: threads, not processes
         from multiprocessing.pool import ThreadPool
@@ -168,6 +224,7 @@ def run(args, engine_factory=None) -> dict:
                 else:
                     dist.init_process_group("gloo")
         sigs, all_ids, cand_ids, any_synth = [], [], [], False
+        cand_rows = []                                    # with vectors: input rows of the hashed documents
 
         def padded(text):
             return to_padded_device(eng, text)
@@ -175,6 +232,8 @@ def run(args, engine_factory=None) -> dict:
         for r in parsed:
             ids, cand = r["ids"], r["cand"]
             any_synth |= r["synthetic"]
+            if min_cosine is not None:
+                cand_rows.append(np.asarray(cand, dtype=np.int64) + len(all_ids))
             all_ids.extend(ids)
             if len(cand) == 0:
                 continue
@@ -215,7 +274,10 @@ def run(args, engine_factory=None) -> dict:
                 eng.components_finish(lab)
                 labels = as_u32(lab).reshape(n)
             else:
-                out = cluster_local(eng, sig, args.bands, args.rows, min_jaccard=args.min_jaccard)
+                vectors = None
+                if min_cosine is not None:
+                    vectors = document_vectors(eng, args, np.concatenate(cand_rows or [np.zeros(0, np.int64)]), len(all_ids))
+                out = cluster_local(eng, sig, args.bands, args.rows, min_jaccard=args.min_jaccard, vectors=vectors, min_cosine=min_cosine)
                 labels = as_u32(out["labels"]).reshape(n)
                 if ckpt_dir:
                     edges = np.ascontiguousarray(np.stack([as_u32(out["edge_u"]), as_u32(out["edge_v"])], axis=1))

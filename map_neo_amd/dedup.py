@@ -51,12 +51,35 @@ def verified_edges(be, sig: torch.Tensor, eu: torch.Tensor, ev: torch.Tensor, mi
     return eu[keep], ev[keep]
 
 
+# How far below the threshold the 4-bit screen of vector_edges looks.  A row's 4-bit form is off by about an eighth of its
+# length in a random direction, which takes about 0.015 off the cosine of two near rows with a spread of a few thousandths.
+SCREEN_MARGIN = 0.05
+
+
+def vector_edges(be, vectors: torch.Tensor, min_cosine: float, margin: float = SCREEN_MARGIN):
+    """Near-duplicate pairs by document vectors [n, dim]: every pair whose 4-bit rows reach min_cosine - margin is checked on
+    the 8-bit rows, and kept if its cosine there (off by less than 2^-7) is >= min_cosine.  Returns (u, v), u > v, ordered.  An
+    extension: the reference compares documents by their shingles only.  Vectors of zeros, and with a NaN, pair with nothing."""
+    if not 0.0 < float(min_cosine) <= 1.0:
+        raise ValueError("min_cosine must be in (0, 1]")
+    codes, _, _ = be.rms_norm_q8(vectors)
+    eu, ev = be.mx_pairs(be.mx_quantize(vectors), max(float(min_cosine) - margin, 0.01))
+    keep = be.edge_cosines(codes, eu, ev) >= float(min_cosine)
+    return eu[keep], ev[keep]
+
+
 def cluster_local(be, sig: torch.Tensor, bands: int = BANDS, rows: int = ROWS, key_bits: int = 64,
-                  want_buckets: bool = False, timer: Optional[StageTimer] = None, min_jaccard: Optional[float] = None):
+                  want_buckets: bool = False, timer: Optional[StageTimer] = None, min_jaccard: Optional[float] = None,
+                  vectors: Optional[torch.Tensor] = None, min_cosine: Optional[float] = None):
     """Band records -> buckets/edges -> union-find -> removed mask for signatures already in HBM
     (EN:133-145 / ZH-2..ZH-4).  Document index = row of `sig`.  min_jaccard (default None = the reference's behaviour)
-    drops candidate edges (document, smallest document of its bucket) whose estimated Jaccard similarity is lower."""
+    drops candidate edges (document, smallest document of its bucket) whose estimated Jaccard similarity is lower.  vectors
+    [n, dim] with min_cosine (default None) add the pairs of vector_edges."""
     n, num_perm = sig.shape
+    if (vectors is None) != (min_cosine is None):
+        raise ValueError("vectors and min_cosine go together")
+    if vectors is not None and vectors.shape[0] != n:
+        raise ValueError("vectors has %d rows for %d documents" % (vectors.shape[0], n))
     mark = timer.mark if timer is not None else (lambda name: None)
     key, meta = be.band_keys(sig, bands, rows, 0, key_bits)
     mark("band_keys")
@@ -65,6 +88,10 @@ def cluster_local(be, sig: torch.Tensor, bands: int = BANDS, rows: int = ROWS, k
     if min_jaccard is not None:
         eu, ev = verified_edges(be, sig, eu, ev, min_jaccard)
         mark("verify")
+    if vectors is not None:
+        vu, vv = vector_edges(be, vectors, min_cosine)
+        eu, ev = torch.cat([eu, vu]), torch.cat([ev, vv])
+        mark("vector_edges")
     labels = be.components_init(n)
     be.components_union(labels, eu, ev)
     be.components_finish(labels)
@@ -78,7 +105,8 @@ def cluster_local(be, sig: torch.Tensor, bands: int = BANDS, rows: int = ROWS, k
 def dedup_local(be, text: torch.Tensor, offsets: torch.Tensor, num_perm: int = NUM_PERM, width: int = WIDTH,
                 unit: str = "char", bands: int = BANDS, rows: int = ROWS, seed: int = SEED,
                 text_bytes: Optional[int] = None, key_bits: int = 64, want_buckets: bool = False,
-                timer: Optional[StageTimer] = None, min_jaccard: Optional[float] = None):
+                timer: Optional[StageTimer] = None, min_jaccard: Optional[float] = None,
+                vectors: Optional[torch.Tensor] = None, min_cosine: Optional[float] = None):
     """One-GPU path.  Returns a dict of device tensors: sig [n,K], edge_u/edge_v, labels [n]
     (label = smallest doc index of the component), removed [n] uint8, n_removed (device
     int64[1]), n_collisions (host int)."""
@@ -86,7 +114,7 @@ def dedup_local(be, text: torch.Tensor, offsets: torch.Tensor, num_perm: int = N
     mark("start")
     sig = be.signatures(text, offsets, num_perm, width, unit, seed, text_bytes=text_bytes)
     mark("signatures")
-    return cluster_local(be, sig, bands, rows, key_bits, want_buckets, timer, min_jaccard)
+    return cluster_local(be, sig, bands, rows, key_bits, want_buckets, timer, min_jaccard, vectors, min_cosine)
 
 
 def signatures_streamed(be, blocks, n_docs: int, num_perm=NUM_PERM, width: int = WIDTH, unit: str = "char", seed: int = SEED,
