@@ -40,13 +40,17 @@ def _tensors(x):
             yield from _tensors(y)
 
 
+# the current stream as a number: a tenth of a microsecond where torch.cuda.current_stream, which makes an object, takes two
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _ordered(fn):
     """runs fn on the engine's stream; under another current stream that one waits for the results, and they for it"""
     @functools.wraps(fn)
     def call(self, *args, **kw):
-        cur = torch.cuda.current_stream(self.device)
-        if cur == self.stream:
+        if _raw_stream(self.device_index) == self.stream.cuda_stream:
             return fn(self, *args, **kw)
+        cur = torch.cuda.current_stream(self.device)
         self.stream.wait_stream(cur)
         with torch.cuda.stream(self.stream):
             out = fn(self, *args, **kw)
@@ -65,27 +69,46 @@ def _need(ok, what):
         raise _lib.MddError(what)
 
 
+def _refuse(what):
+    raise _lib.MddError(what)
+
+
 class VectorOps:
     """mixed into minhash.Engine"""
 
     # ------------------------------------------------------------------ checks
+    # (messages are made only when they are raised: a call is a dozen microseconds, of which these checks would be three)
     def _matrix(self, t, name, dtype=None, rows=None, cols=None):
-        _need(isinstance(t, torch.Tensor) and t.device == self.device, f"{name} must be a tensor on {self.device}")
-        _need(t.dim() == 2, f"{name} must be a matrix, not {t.dim()}-dimensional")
-        _need(t.dtype in _TYPE if dtype is None else t.dtype == dtype, f"{name} has type {t.dtype}" + (f", not {dtype}" if dtype else ""))
+        """(address, row stride) of a matrix, None for an empty one"""
+        if not isinstance(t, torch.Tensor) or t.device != self.device:
+            _refuse(f"{name} must be a tensor on {self.device}")
+        if t.dim() != 2:
+            _refuse(f"{name} must be a matrix, not {t.dim()}-dimensional")
+        if t.dtype not in _TYPE if dtype is None else t.dtype != dtype:
+            _refuse(f"{name} has type {t.dtype}" + (f", not {dtype}" if dtype else ""))
         n, d = t.shape
-        _need(1 <= d <= MAX_DIM, f"{name} has {d} columns: 1 to {MAX_DIM} are supported")
-        _need(rows is None or n == rows, f"{name} has {n} rows, not {rows}")
-        _need(cols is None or d == cols, f"{name} has {d} columns, not {cols}")
-        _need(n == 0 or ((d == 1 or t.stride(1) == 1) and (n == 1 or t.stride(0) >= d)), f"{name} must have unit stride inside its rows")
-        return (t.data_ptr() if t.numel() else None), (t.stride(0) if n > 1 else d)
+        if not 1 <= d <= MAX_DIM:
+            _refuse(f"{name} has {d} columns: 1 to {MAX_DIM} are supported")
+        if rows is not None and n != rows:
+            _refuse(f"{name} has {n} rows, not {rows}")
+        if cols is not None and d != cols:
+            _refuse(f"{name} has {d} columns, not {cols}")
+        stride, inner = t.stride()
+        if n > 0 and ((inner != 1 and d > 1) or (stride < d and n > 1)):
+            _refuse(f"{name} must have unit stride inside its rows")
+        return (t.data_ptr() if n else None), (stride if n > 1 else d)
 
     def _vector(self, t, name, dtypes, size=None):
-        _need(isinstance(t, torch.Tensor) and t.device == self.device, f"{name} must be a tensor on {self.device}")
-        _need(t.dim() == 1 and t.is_contiguous(), f"{name} must be a contiguous vector")
-        _need(t.dtype in dtypes, f"{name} has type {t.dtype}")
-        _need(size is None or t.numel() == size, f"{name} has {t.numel()} entries, not {size}")
-        return t.data_ptr() if t.numel() else None
+        if not isinstance(t, torch.Tensor) or t.device != self.device:
+            _refuse(f"{name} must be a tensor on {self.device}")
+        if t.dim() != 1 or not t.is_contiguous():
+            _refuse(f"{name} must be a contiguous vector")
+        if t.dtype not in dtypes:
+            _refuse(f"{name} has type {t.dtype}")
+        n = t.numel()
+        if size is not None and n != size:
+            _refuse(f"{name} has {n} entries, not {size}")
+        return t.data_ptr() if n else None
 
     def _work(self, n_bytes):
         if not n_bytes:
@@ -94,7 +117,8 @@ class VectorOps:
         return ws.data_ptr(), n_bytes, ws
 
     def _ids(self, ids, offsets, mode):
-        _need(mode in ("mean", "sum"), f"mode {mode!r} is neither 'mean' nor 'sum'")
+        if mode not in ("mean", "sum"):
+            _refuse(f"mode {mode!r} is neither 'mean' nor 'sum'")
         p = self._vector(ids, "ids", (torch.int32, torch.int64))
         o, docs = None, 0
         if offsets is not None:
@@ -126,8 +150,10 @@ class VectorOps:
         the gradient's type, zeros where no id points.  Summed in the order of the positions: repeats bit for bit."""
         gp, gs = self._matrix(grad, "grad")
         ip, ib, n_ids, op, docs = self._ids(ids, offsets, mode)
-        _need(grad.shape[0] == (docs if op else n_ids), f"grad has {grad.shape[0]} rows, not {docs if op else n_ids}")
-        _need(dtype in (torch.float32, grad.dtype), f"dtype {dtype} is neither float32 nor the gradient's")
+        if grad.shape[0] != (docs if op else n_ids):
+            _refuse(f"grad has {grad.shape[0]} rows, not {docs if op else n_ids}")
+        if dtype not in (torch.float32, grad.dtype):
+            _refuse(f"dtype {dtype} is neither float32 nor the gradient's")
         _need(n_rows >= 0, "n_rows is negative")
         dim = grad.shape[1]
         out = torch.empty((n_rows, dim), dtype=dtype, device=self.device)
@@ -162,7 +188,8 @@ class VectorOps:
                     kind: str = "int8"):
         """rms_norm with y in 8 bits and a float32 scale per row (y = codes * scale): kind "int8" or "e4m3".  Returns (codes,
         scales, h, or None without a residual).  Codes are those of exact arithmetic."""
-        _need(kind in _Q8, f"kind {kind!r} is neither 'int8' nor 'e4m3'")
+        if kind not in _Q8:
+            _refuse(f"kind {kind!r} is neither 'int8' nor 'e4m3'")
         xp, xs, rp, rs, wp, n, dim = self._norm_args(x, weight, residual)
         codes = torch.empty((n, dim), dtype=_Q8[kind][1], device=self.device)
         scales = torch.empty(n, dtype=torch.float32, device=self.device)
@@ -218,12 +245,14 @@ class VectorOps:
 
     # ------------------------------------------------------------------ microscaled 4-bit matrices
     def _packed(self, m, name):
-        _need(isinstance(m, MxMatrix), f"{name} must be an MxMatrix")
+        if not isinstance(m, MxMatrix):
+            _refuse(f"{name} must be an MxMatrix")
         rt, ct = (m.rows + 31) // 32, (m.cols + 127) // 128
-        _need(m.rows >= 0 and 1 <= m.cols <= MAX_DIM, f"{name} is {m.rows} x {m.cols}: 1 to {MAX_DIM} columns are supported")
+        if m.rows < 0 or not 1 <= m.cols <= MAX_DIM:
+            _refuse(f"{name} is {m.rows} x {m.cols}: 1 to {MAX_DIM} columns are supported")
         for t, size in ((m.codes, rt * ct * 2048), (m.scales, rt * ct * 128)):
-            _need(isinstance(t, torch.Tensor) and t.device == self.device and t.dtype == torch.uint8 and t.is_contiguous() and t.numel() == size,
-                  f"{name}: codes and scales must be contiguous uint8 tensors on {self.device} of {rt * ct * 2048} and {rt * ct * 128} bytes")
+            if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != size:
+                _refuse(f"{name}: codes and scales must be contiguous uint8 tensors on {self.device} of {rt * ct * 2048} and {rt * ct * 128} bytes")
         return (m.codes.data_ptr(), m.scales.data_ptr()) if m.rows else (None, None)
 
     @_ordered
@@ -243,8 +272,10 @@ class VectorOps:
         """alpha * A B^T [a.rows, b.rows] in float32 or bfloat16: every row of A against every row of B."""
         ac, as_ = self._packed(a, "a")
         bc, bs = self._packed(b, "b")
-        _need(a.cols == b.cols, f"a has {a.cols} columns and b {b.cols}")
-        _need(dtype in (torch.float32, torch.bfloat16), f"dtype {dtype} is neither float32 nor bfloat16")
+        if a.cols != b.cols:
+            _refuse(f"a has {a.cols} columns and b {b.cols}")
+        if dtype not in (torch.float32, torch.bfloat16):
+            _refuse(f"dtype {dtype} is neither float32 nor bfloat16")
         out = torch.empty((a.rows, b.rows), dtype=dtype, device=self.device)
         if out.numel():
             _lib.check(self.L.mdd_mx_matmul(self.ctx, ac, as_, a.rows, bc, bs, b.rows, a.cols, float(alpha), out.data_ptr(), _TYPE[dtype], b.rows),
@@ -265,7 +296,8 @@ class VectorOps:
             _lib.check(self.L.mdd_mx_pairs(self.ctx, mc, ms, m.rows, m.cols, float(min_cosine), eu.data_ptr(), ev.data_ptr(), cap, cnt.data_ptr(),
                                            wp, wb), "mdd_mx_pairs")
             n = int(cnt.item())
-            _need(n <= max_pairs, f"{n} pairs reach {min_cosine}: more than max_pairs={max_pairs}")
+            if n > max_pairs:
+                _refuse(f"{n} pairs reach {min_cosine}: more than max_pairs={max_pairs}")
             if n <= cap:
                 break
             cap = n
