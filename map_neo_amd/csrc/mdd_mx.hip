@@ -426,7 +426,7 @@ __global__ __launch_bounds__(B::WAVES * 64) void mx_matmul_kernel(const Packed a
                     const uint64_t row = (uint64_t)(t.i0 + wr * B::FM + i) * 32 + rr, col = (uint64_t)(t.j0 + wc * B::FN + j0) * 32 + cc * PE;
                     O* to = c + row * cs + col;
                     if (inside) {
-                        *reinterpret_cast<piece_any*>(to) = o;
+                        __builtin_nontemporal_store(o, reinterpret_cast<piece_any*>(to));
                     } else if (row < m && col < n) {
                         if (n - col >= PE) {
                             *reinterpret_cast<piece_any*>(to) = o;

@@ -79,15 +79,10 @@ __device__ __forceinline__ void store8(T* __restrict__ p, uint32_t n, f32x8 v) {
     }
 }
 
-// sum / maximum over the 64 lanes of a wave, the same in every lane; a butterfly, so the order is fixed
+// sum over the 64 lanes of a wave, the same in every lane; a butterfly, so the order is fixed
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, 64);
-    return v;
-}
-__device__ __forceinline__ double wave_max(double v) {
-#pragma unroll
-    for (int m = 32; m; m >>= 1) v = fmax(v, __shfl_xor(v, m, 64));
     return v;
 }
 

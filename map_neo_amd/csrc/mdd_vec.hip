@@ -610,17 +610,20 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
     __syncthreads();
     return s;
 }
-template <int W>
-__device__ __forceinline__ double row_max(double v, double* lds) {
-    v = wave_max(v);
+template <int W, typename F>
+__device__ __forceinline__ F row_max(F v, F* lds) {
+#pragma unroll
+    for (int m = 32; m; m >>= 1) {
+        const F o = __shfl_xor(v, m, 64);
+        v = v > o ? v : o;
+    }
     if (W == 1) return v;
     if (lane_id() == 0) lds[threadIdx.x / 64] = v;
     __syncthreads();
-    double s = lds[0];
 #pragma unroll
-    for (int w = 1; w < W; w++) s = fmax(s, lds[w]);
+    for (int w = 0; w < W; w++) v = v > lds[w] ? v : lds[w];
     __syncthreads();
-    return s;
+    return v;
 }
 
 template <typename T, int NC, int W>
@@ -659,20 +662,24 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_kernel(const T* __r
 }
 
 // The nearest 8-bit value to z = y * top / big.  zf is z rounded to 32 bits, at most 2^-24 of its size off, which is below
-// 1e-5 of a step; only next to a midpoint is z itself formed, a correctly rounded quotient in 64 bits -- rarely, so the codes
-// are those of exact arithmetic and do not depend on how the row was summed, without a division per element.
+// 1e-5 of a step; only next to a midpoint (`tie`) does z itself decide, a correctly rounded quotient in 64 bits -- for one
+// element in some ten thousands.  So the codes are those of exact arithmetic and do not depend on how the row was summed,
+// without a division per element.
 template <int KIND>
-__device__ __forceinline__ float nearest8(float zf, double y, double top, double big) {
+__device__ __forceinline__ float nearest8(float zf, bool& tie) {
     float step = 1.0f;
     if (KIND == MDD_E4M3) {
         const int e = (int)(__float_as_uint(zf) >> 23 & 255u) - 127;
         step = __uint_as_float((uint32_t)((e > -6 ? e : -6) - 3 + 127) << 23);
     }
     const float u = zf / step, q = rintf(u);  // the step is a power of two: exact
-    if (fabsf(fabsf(u - q) - 0.5f) > 2e-5f) return q * step;
-    const double z = y * top / big;
+    tie = fabsf(fabsf(u - q) - 0.5f) <= 2e-5f;
+    return q * step;
+}
+template <int KIND>
+__device__ __forceinline__ float nearest8_exact(double z) {
     if (KIND == MDD_E4M3) {  // the step of z itself: zf may lie across a power of two
-        double s = exp2(fmax(floor(log2(fmax(fabs(z), 0.015625))), -6.0) - 3.0);
+        const double s = exp2(fmax(floor(log2(fmax(fabs(z), 0.015625))), -6.0) - 3.0);
         return (float)(rint(z / s) * s);
     }
     return (float)rint(z);
@@ -724,8 +731,17 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* 
             uint32_t pack[2] = {0, 0};
             if (fine && big > 0) {
                 float q[8];
+                bool tie[8], any = false;
 #pragma unroll
-                for (int k = 0; k < 8; k++) q[k] = nearest8<KIND>((float)(y[c][k] * inv), y[c][k], (double)top, big);
+                for (int k = 0; k < 8; k++) {
+                    q[k] = nearest8<KIND>((float)(y[c][k] * inv), tie[k]);
+                    any |= tie[k];
+                }
+                if (any) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (tie[k]) q[k] = nearest8_exact<KIND>(y[c][k] * (double)top / big);
+                }
 #pragma unroll
                 for (int k = 0; k < 8; k += 4) {
                     if (KIND == MDD_I8) {
@@ -833,7 +849,7 @@ __global__ __launch_bounds__(1024) void weight_grad_kernel(const float* __restri
 
 uint32_t backward_blocks(uint64_t n, uint32_t dim) {
     const uint64_t want = dim <= 2048 ? (n + 3) / 4 : n;
-    return (uint32_t)(want < 512 ? want : 512);  // two blocks a CU
+    return (uint32_t)(want < 1024 ? want : 1024);  // four blocks a CU
 }
 
 // picks NC and W of a row kernel; body(NC, W) as integral constants
