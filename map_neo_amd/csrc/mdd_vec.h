@@ -62,6 +62,12 @@ __device__ __forceinline__ typename vec8<T>::raw load8_raw(const T* __restrict__
     }
     return v;
 }
+// For data that is read, or written, once and whole: past the caches, which keep what is used again
+template <typename T>
+__device__ __forceinline__ f32x8 load8_once(const T* __restrict__ p, uint32_t n) {
+    if (n >= 8) return __builtin_convertvector(__builtin_nontemporal_load(reinterpret_cast<const typename vec8<T>::raw_any*>(p)), f32x8);
+    return __builtin_convertvector(load8_raw<T>(p, n), f32x8);
+}
 template <typename T>
 __device__ __forceinline__ f32x8 load8(const T* __restrict__ p, uint32_t n) {
     return __builtin_convertvector(load8_raw<T>(p, n), f32x8);
@@ -76,6 +82,16 @@ __device__ __forceinline__ void store8(T* __restrict__ p, uint32_t n, f32x8 v) {
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++)
             if (k < n) p[k] = r[k];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8_once(T* __restrict__ p, uint32_t n, f32x8 v) {
+    if (n >= 8) {
+        typename vec8<T>::raw r = __builtin_convertvector(v, typename vec8<T>::raw);
+        __builtin_nontemporal_store(r, reinterpret_cast<typename vec8<T>::raw_any*>(p));
+    } else {
+        store8<T>(p, n, v);
     }
 }
 

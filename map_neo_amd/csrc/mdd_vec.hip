@@ -704,10 +704,10 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* 
             const uint32_t col = (c * TPR + t) * 8;
             f32x8 v = 0.0f, o = 0.0f, w = 1.0f;
             if (col < dim) {
-                v = load8<T>(x + row * xs + col, dim - col);
-                if (res) o = load8<T>(res + row * rs + col, dim - col);
+                v = load8_once<T>(x + row * xs + col, dim - col);
+                if (res) o = load8_once<T>(res + row * rs + col, dim - col);
                 if (weight) w = load8<T>(weight + col, dim - col);
-                if (sum_out) store8<T>(sum_out + row * dim + col, dim - col, v + o);
+                if (sum_out) store8_once<T>(sum_out + row * dim + col, dim - col, v + o);
             }
 #pragma unroll
             for (int k = 0; k < 8; k++) {
@@ -756,7 +756,7 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* 
             uint8_t* to = codes + row * dim + col;
             if (dim - col >= 8) {
                 typedef uint32_t pair_any __attribute__((ext_vector_type(2), aligned(1)));
-                *reinterpret_cast<pair_any*>(to) = pair_any{pack[0], pack[1]};
+                __builtin_nontemporal_store(pair_any{pack[0], pack[1]}, reinterpret_cast<pair_any*>(to));
             } else {
 #pragma unroll
                 for (uint32_t k = 0; k < 8; k++)
