@@ -1,6 +1,10 @@
 """CPU suite: what the document-vector entry points refuse.  Every check of arguments comes before the first HIP call, so a
 zeroed block of memory may stand for the context and made-up addresses for buffers: nothing is dereferenced."""
 import ctypes as C
+import os
+import re
+import shutil
+import subprocess
 from types import SimpleNamespace
 
 import pytest
@@ -129,6 +133,21 @@ def test_workspace_sizes():
     assert L.mdd_sort_edges_ws_bytes(8192) == 0 and L.mdd_sort_edges_ws_bytes(8193) >= 2 * 8193 * 4
     assert L.mdd_mx_pairs_ws_bytes(33) >= 64 * 4
     assert L.mdd_rms_norm_backward_ws_bytes(10 ** 6, 100) >= 512 * 400
+
+
+def test_library_holds_no_packed_float_instructions(tmp_path):
+    """v_pk_add_f32, v_pk_mul_f32 and v_pk_fma_f32 have given wrong results on this hardware: none in any kernel"""
+    tool = "/opt/rocm/llvm/bin/llvm-objdump"
+    if not os.path.exists(tool):
+        pytest.skip("no llvm-objdump")
+    shutil.copy(mlib.SO_PATH, tmp_path / "lib.so")
+    subprocess.run([tool, "--offloading", "lib.so"], cwd=tmp_path, check=True, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
+    objects = [f for f in os.listdir(tmp_path) if "gfx950" in f]
+    assert objects
+    for f in objects:
+        asm = subprocess.run([tool, "-d", f], cwd=tmp_path, check=True, stdout=subprocess.PIPE).stdout
+        assert b"s_endpgm" in asm
+        assert not re.search(rb"v_pk_(add|mul|fma)_f32", asm), f
 
 
 # ------------------------------------------------------------------------------------------------ the Python methods
