@@ -490,6 +490,7 @@ int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_s
 
 /* Root-mean-square norm.  h = x + residual (residual may be NULL: h = x), r = 1 / sqrt(mean(h^2) + eps), weight [dim] of
  * x's type (NULL: ones).  dim <= MDD_VEC_MAX_DIM.
+ *   (the squares of a row have to add up to a 32-bit number: beyond 10^19 r is 0)
  *   norm      y = h * r * weight;  sum_out (may be NULL) = h, rounded to the type;  rstd (may be NULL) = r, float per row
  *   norm_q8   the same with y in 8 bits (kind MDD_I8 or MDD_E4M3): with top = 127 or 448 and big = the row's largest
  *             |h * weight|, code = the nearest 8-bit value to h * weight * top / big, ties to even, decided as in exact
@@ -528,9 +529,11 @@ int mdd_sort_edges(mdd_ctx* ctx, uint32_t* edge_u, uint32_t* edge_v, uint64_t n_
  *   matmul   c [m, n] (MDD_F32 or MDD_BF16, c_stride) = alpha * A * B^T,  A [m, dim], B [n, dim] packed
  *   pairs    every u > v with cos(A_u, A_v) >= min_cosine (0 < min_cosine <= 1; cosine of the 4-bit values), appended to edge_u /
  *            edge_v in no fixed order, at most edge_cap of them; *n_edges (device u64, set by the call) counts all of them.
+ *            The comparison is one of 32-bit numbers: a pair within 2^-20 of min_cosine may fall on either side.
  *            Rows of zeros and rows with a NaN have no pairs.  Rows of similar length are fastest.  m <= MDD_MX_MAX_PAIR_ROWS
  *            (2^22: 10^13 pairs; larger sets are compared block by block with matmul). */
 #define MDD_MX_MAX_PAIR_ROWS 4194304
+#define MDD_MX_MAX_ROWS 2147483392u /* 2^31 - 256: quantize, matmul */
 #define MDD_MX_TILE_ROWS 32
 #define MDD_MX_TILE_COLS 128
 #define MDD_MX_CODE_BYTES(rows, dim) ((((uint64_t)(rows) + 31) / 32) * (((uint64_t)(dim) + 127) / 128) * 2048)

@@ -583,7 +583,7 @@ int mdd_mx_quantize(mdd_ctx* ctx, const void* x, int type, uint64_t x_stride, ui
     REQUIRE(ctx, "%s: ctx is NULL", who);
     REQUIRE(dim >= 1 && dim <= MDD_VEC_MAX_DIM, "%s: dim=%u outside [1,%d]", who, dim, MDD_VEC_MAX_DIM);
     REQUIRE(type_bytes(type), "%s: unknown element type %d", who, type);
-    REQUIRE(n_rows < (1ull << 31), "%s: 2^31 or more rows", who);
+    REQUIRE(n_rows <= MDD_MX_MAX_ROWS, "%s: more than 2^31 - 256 rows", who);
     if (n_rows == 0) return MDD_OK;
     REQUIRE(x && aligned_to(x, type_bytes(type)), "%s: x is NULL or not aligned to its elements", who);
     REQUIRE(x_stride >= dim, "%s: row stride %llu below dim %u", who, (unsigned long long)x_stride, dim);
@@ -606,7 +606,7 @@ int mdd_mx_matmul(mdd_ctx* ctx, const uint8_t* a_codes, const uint8_t* a_scales,
     REQUIRE(ctx, "%s: ctx is NULL", who);
     REQUIRE(dim >= 1 && dim <= MDD_VEC_MAX_DIM, "%s: dim=%u outside [1,%d]", who, dim, MDD_VEC_MAX_DIM);
     REQUIRE(c_type == MDD_F32 || c_type == MDD_BF16, "%s: c_type %d is neither MDD_F32 nor MDD_BF16", who, c_type);
-    REQUIRE(m < (1ull << 31) && n < (1ull << 31), "%s: 2^31 or more rows", who);
+    REQUIRE(m <= MDD_MX_MAX_ROWS && n <= MDD_MX_MAX_ROWS, "%s: more than 2^31 - 256 rows", who);
     if (m == 0 || n == 0) return MDD_OK;
     int rc = check_packed(who, "A", a_codes, a_scales);
     if (!rc) rc = check_packed(who, "B", b_codes, b_scales);

@@ -722,7 +722,7 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* 
         big = row_max<W>(big, ldsd);
         const float r = 1.0f / sqrtf(row_sum<W>(ss, lds) / (float)dim + eps);
         const bool fine = big < __builtin_inf();
-        if (t == 0) scales[row] = fine ? (float)big * r / top : __builtin_nanf("");
+        if (t == 0) scales[row] = !fine ? __builtin_nanf("") : big > 0 ? (float)big * r / top : 0.0f;  // (r is infinite for zeros without eps)
         const double inv = big > 0 ? (double)top / big : 0.0;
 #pragma unroll
         for (int c = 0; c < NC; c++) {

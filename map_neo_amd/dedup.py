@@ -64,7 +64,7 @@ def vector_edges(be, vectors: torch.Tensor, min_cosine: float, margin: float = S
         raise ValueError("min_cosine must be in (0, 1]")
     codes, _, _ = be.rms_norm_q8(vectors)
     eu, ev = be.mx_pairs(be.mx_quantize(vectors), max(float(min_cosine) - margin, 0.01))
-    keep = be.edge_cosines(codes, eu, ev) >= float(min_cosine)
+    keep = be.edge_cosines(codes, eu, ev) >= float(min_cosine) - 2.0 ** -20      # equal rows may come out a few 2^-24 below 1
     return eu[keep], ev[keep]
 
 

@@ -252,6 +252,8 @@ def test_rms_norm_q8_special_rows(engine, kind):
     q, s = R.q8(x, None, None, float(np.float32(1e-6)), kind)
     assert torch.equal(codes.float().double().cpu(), q)
     assert torch.isnan(scales[2:4]).all() and scales[1] == 0 and (codes[1:4].float() == 0).all()
+    zero, s0, _ = engine.rms_norm_q8(x[1:2].cuda(), kind=kind, eps=0.0)
+    assert (zero.float() == 0).all() and s0.item() == 0
     ok = [0, 1, 4, 5, 6, 7]
     _close(scales[ok], s[ok], 120 * R.U32 * s[ok].abs())
 

@@ -73,6 +73,9 @@ def test_vector_edges_keeps_what_reaches_the_threshold(backend, dtype):
     u, v = D.vector_edges(backend, x.to(backend.device), 0.85)
     assert (41, 31) in list(zip(u.cpu().tolist(), v.cpu().tolist()))
     assert D.vector_edges(backend, x[:0].to(backend.device), 0.9)[0].numel() == 0
+    x[60:63] = x[59]
+    u, v = D.vector_edges(backend, x.to(backend.device), 1.0)
+    assert list(zip(u.cpu().tolist(), v.cpu().tolist())) == [(60, 59), (61, 59), (61, 60), (62, 59), (62, 60), (62, 61)]
     for bad in (0.0, 1.1, float("nan")):
         with pytest.raises(ValueError):
             D.vector_edges(backend, x.to(backend.device), bad)

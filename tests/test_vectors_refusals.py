@@ -113,7 +113,7 @@ def test_mx_quantize(change, needle):
 
 
 @pytest.mark.parametrize("change,needle", [
-    (dict(ctx=None), "ctx is NULL"), (dict(dim=0), "dim=0"), (dict(c_type=2), "c_type"), (dict(m=2 ** 31), "2^31"), (dict(n=2 ** 31), "2^31"), (dict(ac=None), "A is NULL"),
+    (dict(ctx=None), "ctx is NULL"), (dict(dim=0), "dim=0"), (dict(c_type=2), "c_type"), (dict(m=2 ** 31 - 255), "2^31"), (dict(n=2 ** 31), "2^31"), (dict(ac=None), "A is NULL"),
     (dict(bs=P + 2), "16-byte"), (dict(c=None), "c is NULL"), (dict(c=P + 2), "aligned"), (dict(cs=5), "c_stride"), (dict(m=2 ** 30, n=2 ** 30, cs=2 ** 30), "2^31 tiles")])
 def test_mx_matmul(change, needle):
     _refused(_call("mdd_mx_matmul", MUL, **change), needle)
