@@ -408,9 +408,49 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __res
         }
 }
 
+// What the gradient sorts.  key = id, or n_rows for padding and for positions outside every document; val = the row of the
+// gradient that the position's table row took part in.  With count given, the documents' named ids are counted (whole
+// numbers: the order of the atomics does not matter; one atomic per wave where the wave lies in one document).
+struct GradIds {
+    const void* ids;
+    int id_bytes;
+    uint64_t n_ids, n_rows;
+    const uint64_t* offsets;
+    uint64_t n_docs;
+    uint32_t* count;
+};
+__device__ __forceinline__ void grad_key(const GradIds& g, uint64_t p, uint32_t& key, uint32_t& val) {  // call with all lanes
+    uint64_t row = p;
+    uint32_t id = NO_ROW;
+    bool named = false;
+    if (p < g.n_ids) {
+        id = named_row(g.ids, g.id_bytes, p, g.n_rows);
+        named = id != NO_ROW;
+        if (g.offsets) {
+            row = doc_at(g.offsets, g.n_docs, p);
+            uint64_t beg = 0, end = 0;
+            if (row < g.n_docs) doc_range(g.offsets, row, g.n_ids, beg, end);
+            if (p < beg || p >= end) named = false;
+        }
+    }
+    key = named ? id : (uint32_t)g.n_rows;
+    val = named ? (uint32_t)row : 0u;
+    if (!g.count) return;
+    const uint64_t live = __ballot(named);
+    if (!live) return;
+    const int leader = __ffsll((unsigned long long)live) - 1;
+    const uint32_t first = __shfl((uint32_t)row, leader, 64);
+    if (__ballot(named && (uint32_t)row != first) == 0) {
+        if ((int)lane_id() == leader) atomicAdd(&g.count[first], (uint32_t)__popcll(live));
+    } else if (named) {
+        atomicAdd(&g.count[row], 1u);
+    }
+}
+
 // up to SMALL_SORT pairs in one block and one launch: all passes in LDS (8 us where the passes above take 12 launches)
-// val_bits > 0: by the value's bits first, then by the key's
-__global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__ key, uint32_t* __restrict__ val, uint32_t n, int val_bits, int bits) {
+// val_bits > 0: by the value's bits first, then by the key's.  MAKE: the pairs are the gradient's, made on the way in
+template <bool MAKE>
+__global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__ key, uint32_t* __restrict__ val, uint32_t n, int val_bits, int bits, GradIds g) {
     __shared__ uint32_t ks[SMALL_SORT], vs[SMALL_SORT], cnt[16][256], lds4[4];
     const uint32_t t = threadIdx.x, wave = t / 64, lane = lane_id();
     const uint32_t rounds = (n + 1023) / 1024, base = wave * rounds * 64 + lane;  // of 64 pairs a wave, all sixteen waves at work
@@ -418,9 +458,11 @@ __global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__
 #pragma unroll
     for (int r = 0; r < 8; r++) {
         const uint32_t i = base + r * 64;
-        const bool live = r < (int)rounds && i < n;
-        k_[r] = live ? key[i] : 0;
-        v_[r] = live ? val[i] : 0;
+        k_[r] = v_[r] = 0;
+        if (r < (int)rounds) {
+            if (MAKE) grad_key(g, i, k_[r], v_[r]);
+            else if (i < n) k_[r] = key[i], v_[r] = val[i];
+        }
     }
     for (int pass = 0, passes = (val_bits + 7) / 8 + (bits + 7) / 8; pass < passes; pass++) {
         const bool by_val = pass < (val_bits + 7) / 8;
@@ -483,13 +525,9 @@ int bits_of(uint64_t largest) {
     return b;
 }
 uint64_t sort_hist_words(uint64_t n) { return n <= SMALL_SORT ? 0 : 256 * ((n + sort_tile(n) - 1) / sort_tile(n)) + 256; }
-// sorts (key, val) by key, the values of equal keys in their order.  (key2, val2) are scratch of the same length (unused up to
-// SMALL_SORT pairs); the result is in key / val, which change places with key2 / val2 in every pass
+// More than SMALL_SORT pairs: sorts (key, val) by key, the values of equal keys in their order.  (key2, val2) are scratch of the
+// same length; the result is in key / val, which change places with key2 / val2 in every pass
 void sort_pairs(hipStream_t s, uint32_t*& key, uint32_t*& val, uint32_t*& key2, uint32_t*& val2, uint64_t n, int bits, uint32_t* hist) {
-    if (n <= SMALL_SORT) {
-        hipLaunchKernelGGL(small_sort_kernel, dim3(1), dim3(1024), 0, s, key, val, (uint32_t)n, 0, bits);
-        return;
-    }
     const uint32_t tile = sort_tile(n), tiles = (uint32_t)((n + tile - 1) / tile);
     auto scatter = tile == 1024 ? sort_scatter_kernel<4> : sort_scatter_kernel<16>;
     for (int shift = 0; shift < bits; shift += 8) {
@@ -502,36 +540,12 @@ void sort_pairs(hipStream_t s, uint32_t*& key, uint32_t*& val, uint32_t*& key2, 
 }
 
 // ------------------------------------------------------------------------------------------------ gradient of the lookup
-// key[p] = id, or n_rows for padding and for positions outside every document; val[p] = the row of the gradient that
-// position p's table row took part in.  With count given, the documents' named ids are counted (whole numbers: the order
-// of the atomics does not matter; one atomic per wave where the wave lies in one document).
-__global__ __launch_bounds__(256) void grad_keys_kernel(const void* __restrict__ ids, int id_bytes, uint64_t n_ids, uint64_t n_rows, const uint64_t* __restrict__ offsets,
-                                                        uint64_t n_docs, uint32_t* __restrict__ count, uint32_t* __restrict__ key, uint32_t* __restrict__ val) {
+// one thread a position, for more than small_sort_kernel takes
+__global__ __launch_bounds__(256) void grad_keys_kernel(GradIds g, uint32_t* __restrict__ key, uint32_t* __restrict__ val) {
     const uint64_t p = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    uint64_t row = p;
-    bool named = false;
-    if (p < n_ids) {
-        const uint32_t id = named_row(ids, id_bytes, p, n_rows);
-        named = id != NO_ROW;
-        if (offsets) {
-            row = doc_at(offsets, n_docs, p);
-            uint64_t beg = 0, end = 0;
-            if (row < n_docs) doc_range(offsets, row, n_ids, beg, end);
-            if (p < beg || p >= end) named = false;
-        }
-        key[p] = named ? id : (uint32_t)n_rows;
-        val[p] = named ? (uint32_t)row : 0u;
-    }
-    if (!count) return;
-    const uint64_t live = __ballot(named);
-    if (!live) return;
-    const int leader = __ffsll((unsigned long long)live) - 1;
-    const uint32_t first = __shfl((uint32_t)row, leader, 64);
-    if (__ballot(named && (uint32_t)row != first) == 0) {
-        if ((int)lane_id() == leader) atomicAdd(&count[first], (uint32_t)__popcll(live));
-    } else if (named) {
-        atomicAdd(&count[row], 1u);
-    }
+    uint32_t k, v;
+    grad_key(g, p, k, v);
+    if (p < g.n_ids) key[p] = k, val[p] = v;
 }
 
 // start[v] = first sorted position with a key >= v, v = 0 .. n_rows
@@ -1045,9 +1059,18 @@ int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_s
     uint64_t* start = (uint64_t*)(base + at[2]);
     uint32_t* count = mean && offsets ? (uint32_t*)(base + at[3]) : nullptr;
     if (count) hipLaunchKernelGGL((fill_kernel<uint32_t>), dim3((unsigned)(n_docs / 256 + 1 < 4096 ? n_docs / 256 + 1 : 4096)), dim3(256), 0, s, count, n_docs, 0u);
+    const GradIds g = {ids, id_bytes, n_ids, n_rows, offsets, n_docs, count};
+    const int bits = bits_of(n_rows);
     const dim3 per_id(grid_for(n_ids, 256));
-    hipLaunchKernelGGL(grad_keys_kernel, per_id, dim3(256), 0, s, ids, id_bytes, n_ids, n_rows, offsets, n_docs, count, key, val);
-    sort_pairs(s, key, val, key2, val2, n_ids, bits_of(n_rows), (uint32_t*)(base + at[1]));
+    if (n_ids <= SMALL_SORT && (!offsets || n_ids <= 1024)) {
+        // one launch less; but finding the document of each position is slow work for a single block (8000 ids in 80 documents:
+        // a gradient of 105 us made on the way in, 64 with a launch of their own)
+        hipLaunchKernelGGL(small_sort_kernel<true>, dim3(1), dim3(1024), 0, s, key, val, (uint32_t)n_ids, 0, bits, g);
+    } else {
+        hipLaunchKernelGGL(grad_keys_kernel, per_id, dim3(256), 0, s, g, key, val);
+        if (n_ids <= SMALL_SORT) hipLaunchKernelGGL(small_sort_kernel<false>, dim3(1), dim3(1024), 0, s, key, val, (uint32_t)n_ids, 0, bits, g);
+        else sort_pairs(s, key, val, key2, val2, n_ids, bits, (uint32_t*)(base + at[1]));
+    }
     hipLaunchKernelGGL(grad_starts_kernel, dim3(grid_for(n_rows + 1, 256)), dim3(256), 0, s, key, (uint32_t)n_ids, n_rows, start);
     // the sums themselves are a lookup: table rows are the documents, the sorted positions their ids, grad the table
     PoolArgs a = {grad, n_grad, (uint32_t)(grad_stride * type_bytes(type)), dim, lanes_per_row(dim), val, 4, n_ids, start, n_rows, 0, scale, count, piece_log2_for(n_ids), n_pieces_for(n_ids),
@@ -1188,7 +1211,7 @@ int mdd_sort_edges(mdd_ctx* ctx, uint32_t* edge_u, uint32_t* edge_v, uint64_t n_
     const int bits = bits_of(n_docs ? n_docs - 1 : 0);
     uint32_t *u = edge_u, *v = edge_v, *v2 = (uint32_t*)ws, *u2 = v2 + round_up(n_edges, 64), *hist = u2 + round_up(n_edges, 64);
     if (n_edges <= SMALL_SORT) {
-        hipLaunchKernelGGL(small_sort_kernel, dim3(1), dim3(1024), 0, ctx->stream, edge_u, edge_v, (uint32_t)n_edges, bits, bits);
+        hipLaunchKernelGGL(small_sort_kernel<false>, dim3(1), dim3(1024), 0, ctx->stream, edge_u, edge_v, (uint32_t)n_edges, bits, bits, GradIds());
         HIP_TRY(hipGetLastError());
         return MDD_OK;
     }
