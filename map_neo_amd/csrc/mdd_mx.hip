@@ -226,15 +226,18 @@ struct Place {
     bool valid;
 };
 __device__ __forceinline__ Place place_at(uint32_t i0, uint32_t j0) { return {(uint32_t)__builtin_amdgcn_readfirstlane(i0), (uint32_t)__builtin_amdgcn_readfirstlane(j0), true}; }
+struct Cursor {  // of a block's walk through the list: the round that comes next, and the band of the last tile
+    uint32_t first = 0, band = 0;
+};
 constexpr uint64_t MAX_TILES = 1ull << 31;  // of a list
 
-// next(cursor) is the block's next tile, from cursor 0 on (valid = false: the list is done).  finish(place, acc) takes a tile's
-// results; it returns whether it has issued at least STORES memory operations.
-template <typename B, int STORES, typename F, typename G>
-__device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32_t col_tiles, uint8_t* lds, F&& next, G&& finish) {
+// next(cursor) is the block's next tile (valid = false: the list is done).  begin(place) is called before a tile's steps and
+// finish(place, acc) takes its results; it returns whether it has issued at least STORES memory operations.
+template <typename B, int STORES, typename F, typename I, typename G>
+__device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32_t col_tiles, uint8_t* lds, F&& next, I&& begin, G&& finish) {
     constexpr int FM = B::FM, FN = B::FN;
     const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave / B::WC, wc = wave % B::WC;
-    uint32_t req_cursor = 0, cursor = 0;
+    Cursor req_cursor, cursor;
     Place req = next(req_cursor), cur = next(cursor);
     if (!cur.valid) return;
     uint32_t req_k = 0, req_buf = 0;
@@ -356,6 +359,7 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
         take_scales();
     };
     while (cur.valid) {
+        begin(cur);
         wait_lds();
         step(std::true_type());
 #pragma unroll 1
@@ -391,12 +395,13 @@ __global__ __launch_bounds__(B::WAVES * 64) void mx_matmul_kernel(const Packed a
     constexpr int STORES = B::FM * B::FN / JO * 4;
     static_assert(B::LOADS + STORES <= 63, "the wait counter holds six bits");
     const uint32_t gm = (a.tiles + B::TA - 1) / B::TA, gn = (b.tiles + B::TB - 1) / B::TB, total = gm * gn;
-    auto next = [&](uint32_t& cursor) -> Place {
-        const uint32_t l = list_place(cursor, total);
-        cursor += gridDim.x;  // total and the grid are below 2^31: no wrap
+    auto next = [&](Cursor& c) -> Place {
+        const uint32_t l = list_place(c.first, total);
+        c.first += gridDim.x;  // total and the grid are below 2^31: no wrap
         if (l >= total) return {0, 0, false};
-        const uint32_t band = l / (8 * gn), rows = gm - band * 8 < 8 ? gm - band * 8 : 8, in = l - band * 8 * gn, col = in / rows;
-        return place_at((band * 8 + in - col * rows) * B::TA, col * B::TB);
+        while (l - c.band * 8 * gn >= 8 * gn) c.band++;  // l only grows
+        const uint32_t in = l - c.band * 8 * gn, rows = gm - c.band * 8 < 8 ? gm - c.band * 8 : 8, col = rows == 8 ? in / 8 : in / rows;
+        return place_at((c.band * 8 + in - col * rows) * B::TA, col * B::TB);
     };
     auto finish = [&](const Place& t, f32x16 (&acc)[B::FM][B::FN]) -> bool {
         typedef O piece __attribute__((ext_vector_type(16 / sizeof(O))));
@@ -426,7 +431,7 @@ __global__ __launch_bounds__(B::WAVES * 64) void mx_matmul_kernel(const Packed a
                     const uint64_t row = (uint64_t)(t.i0 + wr * B::FM + i) * 32 + rr, col = (uint64_t)(t.j0 + wc * B::FN + j0) * 32 + cc * PE;
                     O* to = c + row * cs + col;
                     if (inside) {
-                        __builtin_nontemporal_store(o, reinterpret_cast<piece_any*>(to));
+                        *reinterpret_cast<piece_any*>(to) = o;
                     } else if (row < m && col < n) {
                         if (n - col >= PE) {
                             *reinterpret_cast<piece_any*>(to) = o;
@@ -440,7 +445,7 @@ __global__ __launch_bounds__(B::WAVES * 64) void mx_matmul_kernel(const Packed a
             }
         return inside;
     };
-    mx_stream<B, STORES>(a, b, col_tiles, lds, next, finish);
+    mx_stream<B, STORES>(a, b, col_tiles, lds, next, [](const Place&) {}, finish);
 }
 
 // ------------------------------------------------------------------------------------------------ near pairs
@@ -496,27 +501,28 @@ __global__ __launch_bounds__(B::WAVES * 64) void mx_pairs_kernel(const Packed a,
     static_assert(B::TA == B::TB, "square blocks: the diagonal ones hold both sides");
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const uint32_t g = (a.tiles + B::TA - 1) / B::TA, bands = (g + 7) / 8, total = 32 * bands * (bands + 1);
-    auto next = [&](uint32_t& cursor) -> Place {
+    auto next = [&](Cursor& c) -> Place {
         for (;;) {
-            const uint32_t l = list_place(cursor, total);
-            cursor += gridDim.x;
+            const uint32_t l = list_place(c.first, total);
+            c.first += gridDim.x;
             if (l >= total) return {0, 0, false};
-            // band: eight block rows, 8 (band + 1) block columns, after 32 band (band + 1) places
-            uint32_t band = (uint32_t)((__builtin_sqrtf(1.0f + (float)l / 8.0f) - 1.0f) * 0.5f);
-            while (32 * band * (band + 1) > l) band--;
-            while (32 * (band + 1) * (band + 2) <= l) band++;
-            const uint32_t in = l - 32 * band * (band + 1), bi = band * 8 + in % 8, bj = in / 8;
+            // band: eight block rows, 8 (band + 1) block columns, after 32 band (band + 1) places; l only grows
+            while (32 * (c.band + 1) * (c.band + 2) <= l) c.band++;
+            const uint32_t in = l - 32 * c.band * (c.band + 1), bi = c.band * 8 + in % 8, bj = in / 8;
             if (bi < g && bj <= bi) return place_at(bi * B::TA, bj * B::TB);
         }
     };
-    auto finish = [&](const Place& t, f32x16 (&acc)[B::FM][B::FN]) -> bool {
-        const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave / B::WC, wc = wave % B::WC;
-        const uint32_t last = a.tiles - 1, it = t.i0 + wr * B::FM, jt = t.j0 + wc * B::FN;
-        float li[B::FM], lj[B::FN];  // uniform: scalar loads, all at once
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave / B::WC, wc = wave % B::WC, last = a.tiles - 1;
+    float li[B::FM], lj[B::FN];  // least lengths of the wave's row tiles: scalar loads, on their way during the steps
+    auto begin = [&](const Place& t) {
+        const uint32_t it = t.i0 + wr * B::FM, jt = t.j0 + wc * B::FN;
 #pragma unroll
         for (int i = 0; i < B::FM; i++) li[i] = least[it + i <= last ? it + i : last];
 #pragma unroll
         for (int j = 0; j < B::FN; j++) lj[j] = least[jt + j <= last ? jt + j : last];
+    };
+    auto finish = [&](const Place& t, f32x16 (&acc)[B::FM][B::FN]) -> bool {
+        const uint32_t lane = lane_id(), it = t.i0 + wr * B::FM, jt = t.j0 + wc * B::FN;
 #pragma unroll
         for (int i = 0; i < B::FM; i++) {
             if (it + i > last) break;
@@ -554,7 +560,7 @@ __global__ __launch_bounds__(B::WAVES * 64) void mx_pairs_kernel(const Packed a,
         }
         return false;
     };
-    mx_stream<B, 0>(a, a, col_tiles, lds, next, finish);
+    mx_stream<B, 0>(a, a, col_tiles, lds, next, begin, finish);
 }
 
 // Large blocks read half as much from L2 per product, small ones fill the chip with fewer tiles: whichever needs less time
