@@ -220,48 +220,51 @@ __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
     }
 }
 
-// A block per piece and 512 columns.  The long document that begins in the piece, if one does, is this block's: each of the four waves adds a quarter of its shares in order, eight at a time, and the quarters are added in
+// A block per eight pieces and 512 columns.  The long documents that begin in them are this block's: each of the four waves adds a quarter of its shares in order, eight at a time, and the quarters are added in
 // order.
 template <typename O>
 __global__ __launch_bounds__(256) void pool_join_kernel(PoolArgs a) {
     __shared__ __attribute__((aligned(32))) float quarter[3][512];
     const uint32_t lane = lane_id(), wave = threadIdx.x / 64, col = blockIdx.y * 512u + lane * 8u;
-    for (uint64_t first = blockIdx.x; first < a.n_pieces; first += gridDim.x) {
-        const uint64_t d = a.begins[first];
-        if (d >= a.n_docs) continue;  // the same for the whole block
-        uint64_t beg, end;
-        doc_range(a.offsets, d, a.n_ids, beg, end);
-        const uint64_t last = (end - 1) >> a.piece_log2;
-        // a long document leaves its first piece, so it is slot 0 there only if the piece begins with it
-        const uint64_t at0 = first * 2 + (beg > first << a.piece_log2 ? 1 : 0);
-        uint32_t n_named = 0;
-        for (uint64_t k = first + lane; k <= last; k += 64) n_named += a.part_n[k == first ? at0 : k * 2];
+    for (uint64_t base = (uint64_t)blockIdx.x * 8; base < a.n_pieces; base += (uint64_t)gridDim.x * 8) {
+        const uint64_t mine = lane < 8 && base + lane < a.n_pieces ? a.begins[base + lane] : ~0ull;
+        for (uint64_t left = __ballot(mine < a.n_docs); left; left &= left - 1) {  // the same for the whole block
+            const int at = __ffsll((unsigned long long)left) - 1;
+            const uint64_t first = base + at, d = __shfl(mine, at, 64);
+            uint64_t beg, end;
+            doc_range(a.offsets, d, a.n_ids, beg, end);
+            const uint64_t last = (end - 1) >> a.piece_log2;
+            // a long document leaves its first piece, so it is slot 0 there only if the piece begins with it
+            const uint64_t at0 = first * 2 + (beg > first << a.piece_log2 ? 1 : 0);
+            uint32_t n_named = 0;
+            for (uint64_t k = first + lane; k <= last; k += 64) n_named += a.part_n[k == first ? at0 : k * 2];
 #pragma unroll
-        for (int m = 32; m; m >>= 1) n_named += __shfl_xor(n_named, m, 64);
-        f32x8 acc = 0.0f;
-        if (col < a.dim) {
-            const float* __restrict__ part = a.part + col;
-            const uint64_t each = (last - first + 4) / 4;  // shares first + [wave * each, (wave + 1) * each)
-            uint64_t k = first + wave * each;
-            const uint64_t stop = k + each < last + 1 ? k + each : last + 1;
-            if (wave == 0) acc = load8<float>(part + at0 * a.dim, a.dim - col), k++;
-            for (; k + 8 <= stop; k += 8) {
-                f32x8 v[8];
+            for (int m = 32; m; m >>= 1) n_named += __shfl_xor(n_named, m, 64);
+            f32x8 acc = 0.0f;
+            if (col < a.dim) {
+                const float* __restrict__ part = a.part + col;
+                const uint64_t each = (last - first + 4) / 4;  // shares first + [wave * each, (wave + 1) * each)
+                uint64_t k = first + wave * each;
+                const uint64_t stop = k + each < last + 1 ? k + each : last + 1;
+                if (wave == 0) acc = load8<float>(part + at0 * a.dim, a.dim - col), k++;
+                for (; k + 8 <= stop; k += 8) {
+                    f32x8 v[8];
 #pragma unroll
-                for (int u = 0; u < 8; u++) v[u] = load8<float>(part + (k + u) * 2 * a.dim, a.dim - col);
+                    for (int u = 0; u < 8; u++) v[u] = load8<float>(part + (k + u) * 2 * a.dim, a.dim - col);
 #pragma unroll
-                for (int u = 0; u < 8; u++) acc += v[u];
+                    for (int u = 0; u < 8; u++) acc += v[u];
+                }
+                for (; k < stop; k++) acc += load8<float>(part + k * 2 * a.dim, a.dim - col);
             }
-            for (; k < stop; k++) acc += load8<float>(part + k * 2 * a.dim, a.dim - col);
-        }
-        if (wave) *reinterpret_cast<f32x8*>(&quarter[wave - 1][lane * 8]) = acc;
-        __syncthreads();
-        if (wave == 0 && col < a.dim) {
+            if (wave) *reinterpret_cast<f32x8*>(&quarter[wave - 1][lane * 8]) = acc;
+            __syncthreads();
+            if (wave == 0 && col < a.dim) {
 #pragma unroll
-            for (int q = 0; q < 3; q++) acc += *reinterpret_cast<const f32x8*>(&quarter[q][lane * 8]);
-            store8<O>(reinterpret_cast<O*>(a.out) + d * a.dim + col, a.dim - col, acc * pool_factor(a, n_named));
+                for (int q = 0; q < 3; q++) acc += *reinterpret_cast<const f32x8*>(&quarter[q][lane * 8]);
+                store8<O>(reinterpret_cast<O*>(a.out) + d * a.dim + col, a.dim - col, acc * pool_factor(a, n_named));
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -596,7 +599,7 @@ void launch_pool(hipStream_t s, const PoolArgs& a) {
     if (a.n_pieces) {
         const uint32_t slabs = (a.dim + 511) / 512;
         const uint64_t cap = (1u << 20) / slabs + 1;
-        hipLaunchKernelGGL((pool_join_kernel<O>), dim3((unsigned)(a.n_pieces < cap ? a.n_pieces : cap), slabs), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((pool_join_kernel<O>), dim3((unsigned)((a.n_pieces + 7) / 8 < cap ? (a.n_pieces + 7) / 8 : cap), slabs), dim3(256), 0, s, a);
     }
 }
 
