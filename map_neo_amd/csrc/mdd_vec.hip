@@ -119,7 +119,7 @@ __device__ __forceinline__ void sum_span(const PoolArgs& a, uint64_t beg, uint64
         }
         // steps of G rows, one per group: eight at a time, what is left in batches of 4, 2, 1 (at most three more round trips,
         // no row read twice), and last the groups that get one row more than the others
-        const int steps = n / G;
+        const int steps = n >> __builtin_ctz(G);
         int j = 0;
         if constexpr (!NARROW) {
             for (; j + 8 <= steps; j += 8) add_rows<T, NS, WEIGHTED, NARROW, true, 8>(a, table, row, w, (j * G + g) * 4, G * 4, acc);
