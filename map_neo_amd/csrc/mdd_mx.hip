@@ -14,14 +14,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr uint32_t TILE = 2048, STILE = 128;  // bytes of a 32 x 128 tile: codes, scales
 
 // ------------------------------------------------------------------------------------------------ quantisation
-// code of |a| on the grid 0 .5 1 1.5 2 3 4 6: below 1 the grid is even (steps of .5); from 1 on it is a float with one
-// fraction bit, so rounding the bits to that place (ties to even) and rebasing the exponent gives the code
-__device__ __forceinline__ uint32_t e2m1(float a) {
-    const uint32_t u = __float_as_uint(a);
-    const uint32_t hi = ((u + 0x1FFFFFu + (u >> 22 & 1u)) >> 22) - 252u;
-    return a < 1.0f ? (uint32_t)rintf(a + a) : (hi < 7u ? hi : 7u);
-}
-
 // A thread takes a block of 32 columns of a row; four threads side by side take a tile's four blocks, 32 rows a tile.
 // Bound by HBM: the matrix is read once, a bit more than half a byte per element is written.
 template <typename T>
@@ -48,16 +40,15 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
         // biased exponent of the largest, less 2; subnormal and zero blocks stop at 2^-127
         const int e = (int)(big >> 23) - 127 - 2, sc = e > -127 ? e : -127;
         const bool bad = big >= 0x7F800000u;
-        const float inv = __uint_as_float((uint32_t)(127 - sc) << 23);  // sc is -127 .. 125: 2^2 .. 2^254 of the exponent field
+        const float scale = sc > -127 ? __uint_as_float((uint32_t)(sc + 127) << 23) : 0x1p-127f;
         u32x4 p = 0;
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             uint32_t w = 0;
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const uint32_t sign = __float_as_uint(v[c][k]) >> 31;
-                w |= (e2m1(fabsf(v[c][k]) * inv) | sign << 3) << (4 * k);
-            }
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[c][0], v[c][1], scale, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[c][2], v[c][3], scale, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[c][4], v[c][5], scale, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[c][6], v[c][7], scale, 3);
             p[c] = bad ? 0u : w;
         }
         *reinterpret_cast<u32x4*>(codes + tile * TILE + kb * 512 + r * 16) = p;

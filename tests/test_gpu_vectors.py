@@ -309,8 +309,9 @@ def test_mx_quantize(engine, dtype, n, dim):
         x[n // 2, 32: 64] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9]).repeat(4).to(dtype)      # every midpoint, and beyond 6
         x[n - 1, 64] = float("inf")
         x[n - 1, 33] = float("nan")
-    if dtype == torch.float32 and dim >= 32:
-        x[n - 1, :32] = 2.0 ** -140                               # subnormal: the scale stops at 2^-127
+    if dtype != torch.float16 and dim >= 32:                     # near and below the smallest normal number: the scale stops at 2^-127
+        x[n - 1, :32] = (2.0 ** torch.linspace(-128, -123, 32)).to(dtype) * torch.tensor([1.0, -1.0]).repeat(16).to(dtype)
+        x[n // 3, :32] = 2.0 ** -130
     m = engine.mx_quantize(x.cuda())
     codes, sb = R.mx_unpack(m.codes, m.scales, n, dim)
     want, wb = R.mx_codes(x)
