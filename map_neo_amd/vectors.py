@@ -285,9 +285,10 @@ class VectorOps:
     @_ordered
     def mx_pairs(self, m: MxMatrix, min_cosine: float, max_pairs: int = 1 << 28):
         """Every pair of rows u > v whose 4-bit values have a cosine >= min_cosine, ordered by (u, v): int32 tensors (u, v).  The
-        n x n matrix is never stored.  One synchronisation, for the number of pairs; a second pass when there are more than eight
+        n x n matrix is never stored.  Rows of zeros, with a NaN, or of a length outside [2^-60, 2^60] have no pairs.  One synchronisation, for the number of pairs; a second pass when there are more than eight
         per row.  More than max_pairs raise MddError."""
         mc, ms = self._packed(m, "m")
+        _need(max_pairs >= 0, "max_pairs is negative")
         cnt = torch.empty(1, dtype=torch.int64, device=self.device)
         wp, wb, ws = self._work(self.L.mdd_mx_pairs_ws_bytes(m.rows))
         cap = min(int(max_pairs), max(4096, 8 * m.rows))

@@ -219,6 +219,19 @@ def test_rms_norm_gradient_against_differences(engine):
         assert abs((f(x, up) - f(x, dn)) / (2 * e) - dw[j].item()) < 1e-5
 
 
+@pytest.mark.parametrize("kind,top", [("int8", 127), ("e4m3", 448)])
+def test_q8_scale_of_products_above_32_bits(engine, kind, top):
+    """h * weight leaves the range of float, its quotient by the row's norm and the largest code does not"""
+    x = torch.zeros(2, 64)
+    x[0, 3], x[1] = 4, 4
+    w = torch.full((64,), 3e38)
+    codes, scales, _ = engine.rms_norm_q8(x.cuda(), w.cuda(), eps=0.0, kind=kind)
+    r = 1 / (x.double() ** 2).mean(1).sqrt()
+    want = 4 * w[0].double() * r / top                           # rstd: a sum of 64 squares, root, quotient; two roundings here
+    assert ((scales.double().cpu() - want).abs() <= want * 2.0 ** -24 * 16).all()
+    assert (codes.float().cpu() == torch.where(x > 0, float(top), 0.0)).all()
+
+
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim,n", DIMS)
@@ -381,6 +394,22 @@ def test_mx_pairs(engine, n, dim):
     assert n < 2 or np.abs(c[np.tril_indices(n, -1)] - 0.9).min() > 1e-4      # the data leaves no pair at the threshold
     wu, wv = np.nonzero(np.tril(c >= 0.9, -1))
     assert (eu.cpu().numpy() == wu).all() and (ev.cpu().numpy() == wv).all() and (n < 100 or len(wu) > 0)
+
+
+@pytest.mark.parametrize("power", [-120, -75, -61, -56, 56, 61, 75, 120])
+def test_mx_pairs_long_and_short_rows(engine, power):
+    """32 equal rows of `power` and 32 rows each along an axis of its own, where a product of lengths may leave the range of
+    a 32-bit number: pairs among the equal rows only, and none where the length is outside [2^-60, 2^60]"""
+    x = torch.zeros(96, 64)
+    x[:32, :4] = 2.0 ** (power - 1)                              # length 2^power
+    x[torch.arange(32, 64), torch.arange(4, 36)] = 2.0 ** power
+    x[64:, 40:44] = 0.5                                          # length 1
+    eu, ev = engine.mx_pairs(engine.mx_quantize(x.cuda()), 0.9)
+    wu, wv = np.nonzero(np.tril(np.ones((32, 32)), -1))
+    mid = wu + 64, wv + 64
+    if -60 <= power <= 60:
+        mid = np.concatenate([wu, mid[0]]), np.concatenate([wv, mid[1]])
+    assert (eu.cpu().numpy() == mid[0]).all() and (ev.cpu().numpy() == mid[1]).all()
 
 
 def test_mx_pairs_all_alike(engine):

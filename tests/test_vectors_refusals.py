@@ -178,7 +178,8 @@ M, I32 = torch.zeros(4, 8), torch.zeros(3, dtype=torch.int32)
     (lambda: E.rms_norm_q8(M, kind="int4"), "kind"), (lambda: E.rms_norm_backward(M, M, M[0]), "entries"), (lambda: E.rms_norm_backward(M.half(), M, M[:, 0].clone()), "type"),
     (lambda: E.edge_cosines(M, I32, I32), "int8"), (lambda: E.edge_cosines(M.to(torch.int8), I32, I32[:2]), "entries"), (lambda: E.sort_edges(I32, I32.long(), 5), "type"),
     (lambda: E.mx_matmul(M, M), "MxMatrix"), (lambda: E.mx_matmul(V.MxMatrix(M, M, 4, 8), None), "contiguous uint8"),
-    (lambda: E.mx_pairs(V.MxMatrix(I32, I32, 1, 0), 0.9), "columns are supported")])
+    (lambda: E.mx_pairs(V.MxMatrix(I32, I32, 1, 0), 0.9), "columns are supported"),
+    (lambda: E.mx_pairs(V.MxMatrix(I32[:0].byte(), I32[:0].byte(), 0, 4), 0.9, max_pairs=-1), "max_pairs is negative")])
 def test_python_refusals(call, needle):
     with pytest.raises(mlib.MddError, match=needle):
         call()
