@@ -367,13 +367,9 @@ __device__ __forceinline__ void mx_stream(const Packed a, const Packed b, uint32
     wait_memory<0>();  // loads into LDS do not outlive the block
 }
 
-// Work order.  Blocks go to the eight XCDs in turn, so XCD x gets a run of consecutive tiles of the list, and the list walks
-// eight block rows at a time down the columns: the 32 blocks that an XCD runs together share 8 + 4 tiles out of its L2.
-__device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t n) {
-    const uint32_t per = n / 8;  // the last n % 8 keep their place
-    return b < per * 8 ? (b % 8) * per + b / 8 : b;
-}
-// position in the list of this block's round that begins at `first`; `total` when there is none
+// Work order.  An XCD gets a run of consecutive tiles of the list, and the list walks eight block rows at a time down the
+// columns: the 32 blocks that an XCD runs together share 8 + 4 tiles out of its L2.
+// Position in the list of this block's round that begins at `first`; `total` when there is none
 __device__ __forceinline__ uint32_t list_place(uint32_t first, uint32_t total) {
     if (first >= total || blockIdx.x >= total - first) return total;
     return first + xcd_order(blockIdx.x, total - first < gridDim.x ? total - first : gridDim.x);

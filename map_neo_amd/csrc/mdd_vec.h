@@ -102,6 +102,12 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
+// Blocks go to the eight XCDs in turn: place of block b of n in a list of which each XCD then takes a run of neighbours
+__device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t n) {
+    const uint32_t per = n / 8;  // the last n % 8 keep their place
+    return b < per * 8 ? (b % 8) * per + b / 8 : b;
+}
+
 // runs body(T()) for the element type `t`
 #define MDD_FOR_TYPE(t, T, ...)                                   \
     do {                                                          \

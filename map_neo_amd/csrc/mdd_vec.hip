@@ -30,6 +30,7 @@ struct PoolArgs {
     uint64_t n_rows;
     uint32_t row_bytes;  // from a table row to the next
     uint32_t dim, lpr;
+    uint32_t slabs;  // of 256 columns, shared out by block (column_slabs); 1: all columns
     const void* ids;
     int id_bytes;
     uint64_t n_ids;
@@ -80,6 +81,25 @@ __device__ __forceinline__ void add_rows(const PoolArgs& a, const T* __restrict_
         for (int n = 0; n < NS; n++) raw[u][n] = load_cols<T, NARROW>(reinterpret_cast<const T*>(reinterpret_cast<const uint8_t*>(table[n]) + off), a.dim);
     }
     __builtin_amdgcn_sched_barrier(0);  // all loads first: left alone, the compiler takes them one by one to save registers
+    if constexpr (std::is_same_v<T, __bf16> && !WEIGHTED && ALL && !NARROW && U >= 2) {
+        // Two rows at once: their elements of a column side by side, times one and one, added to the sum -- an instruction per
+        // element where a conversion and an addition are two.  The sum has at most the error of two additions, subnormal numbers
+        // included (its form for fp16 drops those and is not used).  40000 documents of 480 x 256: 516 -> 488 us.
+        typedef __bf16 two __attribute__((ext_vector_type(2)));
+        const two ones = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+        for (int u = 0; u < U; u += 2)
+#pragma unroll
+            for (int n = 0; n < NS; n++) {
+                const u32x4 x = __builtin_bit_cast(u32x4, raw[u][n]), y = __builtin_bit_cast(u32x4, raw[u + 1][n]);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    acc[n][2 * k] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(two, __builtin_amdgcn_perm(y[k], x[k], 0x05040100u)), ones, acc[n][2 * k], false);
+                    acc[n][2 * k + 1] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(two, __builtin_amdgcn_perm(y[k], x[k], 0x07060302u)), ones, acc[n][2 * k + 1], false);
+                }
+            }
+        return;
+    }
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const float w = WEIGHTED ? __int_as_float(__builtin_amdgcn_ds_bpermute(first + u * step, __float_as_int(weight))) : 1.0f;
@@ -178,17 +198,26 @@ __device__ __forceinline__ void store_cols(O* __restrict__ row, const uint32_t (
 template <typename T, typename O, int NS, bool WEIGHTED, bool NARROW>
 __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
     const uint32_t lane = lane_id(), lpr = NS == 2 ? 64 : a.lpr;
+    uint32_t block = blockIdx.x, blocks = gridDim.x, slab = blockIdx.y;
+    if (NS == 1 && a.slabs > 1) {
+        // one slab after the other down the list of blocks, an eighth of which each XCD takes in a row; and a slab's work in steps
+        // of eight, so that each XCD has its part of the pieces, which come first and are the most work
+        const uint32_t at = xcd_order(block, blocks);
+        blocks /= a.slabs, slab = at / blocks, block = at - slab * blocks;
+        const uint32_t run = blocks / 8;
+        if (block < run * 8) block = block % run * 8 + block / run;
+    }
     uint32_t col[NS];
     bool in[NS];
 #pragma unroll
     for (int n = 0; n < NS; n++) {
-        const uint32_t c = blockIdx.y * (512u * NS) + n * 512 + (lane & (lpr - 1)) * 8u;
+        const uint32_t c = slab * (NS == 1 && a.slabs > 1 ? 256u : 512u * NS) + n * 512 + (lane & (lpr - 1)) * 8u;
         col[n] = lane_col<NARROW>(c, a.dim);
         in[n] = lane < lpr && c < a.dim;
     }
-    const uint64_t n_work = a.n_pieces + a.n_docs, stride = (uint64_t)gridDim.x * 4;
+    const uint64_t n_work = a.n_pieces + a.n_docs, stride = (uint64_t)blocks * 4;
     const uint64_t piece = 1ull << a.piece_log2;
-    for (uint64_t w = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; w < n_work; w += stride) {
+    for (uint64_t w = (uint64_t)block * 4 + threadIdx.x / 64; w < n_work; w += stride) {
         uint32_t n_named;
         f32x8 acc[NS];
         if (w < a.n_pieces) {  // shares of long documents
@@ -208,9 +237,9 @@ __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
                 sum_span<T, NS, WEIGHTED, NARROW>(a, beg, end, col, acc, n_named);
                 const uint64_t at = w * 2 + slot;
                 store_cols<float, NS, NARROW>(a.part + at * a.dim, col, in, a.dim, acc, 1.0f);
-                if (lane == 0 && blockIdx.y == 0) a.part_n[at] = n_named;
+                if (lane == 0 && slab == 0) a.part_n[at] = n_named;
             }
-            if (lane == 0 && blockIdx.y == 0) a.begins[w] = begins;
+            if (lane == 0 && slab == 0) a.begins[w] = begins;
         } else {
             const uint64_t d = w - a.n_pieces;
             uint64_t beg, end;
@@ -591,11 +620,24 @@ void place_parts(PoolArgs& a, uint8_t* ws) {
 
 uint32_t lanes_per_row(uint32_t dim) { return dim > 256 ? 64 : dim > 128 ? 32 : dim > 64 ? 16 : 8; }
 
+// Every XCD has an L2 of 4 MB of its own.  With a row's columns shared out among them, 256 a slab, an L2 keeps its slab of the
+// table instead of a little of everything: 10000 documents of 480 ids, 64000 x 1024 in bf16, 630 -> 488 us; 30000 of 64 ids, 64000 x 768
+// in fp32, 441 -> 338.  Not where a slab would be mostly empty, where the table fits or its rows are not named again, or
+// where sums are so short that reading their ids once a slab costs more (10 ids a document: 315 us whole, 487 in slabs; at 32
+// ids 259 and 253).  Slabs of 128 columns: 40000 documents of 480 x 256 531 us instead of 497.
+uint32_t column_slabs(const PoolArgs& a) {
+    const uint32_t n = (a.dim + 255) / 256;
+    if (n < 2 || n * 256 > a.dim + a.dim / 8 || a.n_rows * a.row_bytes <= (4u << 20) || a.n_ids < 2 * a.n_rows || a.n_ids < 32 * a.n_docs) return 1;
+    return n;
+}
+
 template <typename T, typename O, bool WEIGHTED>
-void launch_pool(hipStream_t s, const PoolArgs& a) {
-    const uint32_t ns = a.dim > 512 ? 2 : 1, slabs = (a.dim + 512 * ns - 1) / (512 * ns);
-    const uint64_t cap = (1u << 20) / slabs + 1, want = (a.n_pieces + a.n_docs + 3) / 4;
-    const dim3 grid((unsigned)(want < cap ? want : cap), slabs), block(256);
+void launch_pool(hipStream_t s, PoolArgs a) {
+    a.slabs = column_slabs(a);
+    if (a.slabs > 1) a.lpr = 32;
+    const uint32_t ns = a.dim > 512 && a.slabs == 1 ? 2 : 1, slabs = a.slabs > 1 ? a.slabs : (a.dim + 512 * ns - 1) / (512 * ns);
+    const uint64_t cap = (1u << 20) / slabs + 1, want = (a.n_pieces + a.n_docs + 3) / 4, blocks = want < cap ? want : cap;
+    const dim3 grid((unsigned)(a.slabs > 1 ? blocks * slabs : blocks), a.slabs > 1 ? 1 : slabs), block(256);
     if (a.dim < 8) hipLaunchKernelGGL((pool_kernel<T, O, 1, WEIGHTED, true>), grid, block, 0, s, a);
     else if (ns == 2) hipLaunchKernelGGL((pool_kernel<T, O, 2, WEIGHTED, false>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((pool_kernel<T, O, 1, WEIGHTED, false>), grid, block, 0, s, a);
@@ -1011,7 +1053,7 @@ int mdd_embed(mdd_ctx* ctx, const void* table, int type, uint64_t n_rows, uint64
         HIP_TRY(hipGetLastError());
         return MDD_OK;
     }
-    PoolArgs a = {table, n_rows, (uint32_t)(row_stride * type_bytes(type)), dim, lanes_per_row(dim), ids, id_bytes, n_ids, offsets, n_docs, mean, scale, nullptr, piece_log2_for(n_ids), n_pieces_for(n_ids), nullptr,
+    PoolArgs a = {table, n_rows, (uint32_t)(row_stride * type_bytes(type)), dim, lanes_per_row(dim), 1, ids, id_bytes, n_ids, offsets, n_docs, mean, scale, nullptr, piece_log2_for(n_ids), n_pieces_for(n_ids), nullptr,
                   nullptr, nullptr, out};
     if (a.n_pieces) place_parts(a, (uint8_t*)ws);
     MDD_FOR_TYPE(type, T, (launch_pool<T, T, false>(ctx->stream, a)));
@@ -1084,7 +1126,7 @@ int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_s
     hipLaunchKernelGGL(grad_starts_kernel, dim3(grid_for(n_rows + 1, 256)), dim3(256), 0, s, key, (uint32_t)n_ids, n_rows, start);
     // the sums themselves are a lookup: table rows are the documents, the sorted positions their ids, grad the table.
     // 262144 x 1024 in bf16 into 64000 rows: 205 us for 800 MB read and written, 245 us with the sort
-    PoolArgs a = {grad, n_grad, (uint32_t)(grad_stride * type_bytes(type)), dim, lanes_per_row(dim), val, 4, n_ids, start, n_rows, 0, scale, count, piece_log2_for(n_ids), n_pieces_for(n_ids),
+    PoolArgs a = {grad, n_grad, (uint32_t)(grad_stride * type_bytes(type)), dim, lanes_per_row(dim), 1, val, 4, n_ids, start, n_rows, 0, scale, count, piece_log2_for(n_ids), n_pieces_for(n_ids),
                   nullptr, nullptr, nullptr, table_grad};
     if (a.n_pieces) place_parts(a, base + at[4]);
     MDD_FOR_TYPE(type, T, {
