@@ -482,7 +482,9 @@ __device__ __forceinline__ void grad_key(const GradIds& g, uint64_t p, uint32_t&
     }
 }
 
-// up to SMALL_SORT pairs in one block and one launch: all passes in LDS (8 us where the passes above take 12 launches)
+// Up to SMALL_SORT pairs in one block and one launch, all passes in LDS: 450 edges 10 us, 6750 30 (four passes each).  Counting for each
+// edge on all CUs how many are before it takes 16 for 6750, but a workspace and a launch more: 8 us less of 474 a search for near
+// pairs, and 3 more of 54 for the small one.
 // val_bits > 0: by the value's bits first, then by the key's.  MAKE: the pairs are the gradient's, made on the way in
 template <bool MAKE>
 __global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__ key, uint32_t* __restrict__ val, uint32_t n, int val_bits, int bits, GradIds g) {

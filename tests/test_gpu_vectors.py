@@ -296,7 +296,7 @@ def test_edge_cosines(engine, kind, dim):
     assert engine.edge_cosines(rows.cuda(), eu[:0].cuda(), ev[:0].cuda()).numel() == 0
 
 
-@pytest.mark.parametrize("n,docs", [(0, 5), (1, 5), (2, 2), (4000, 3), (8192, 70000), (8193, 300), (50001, 256), (100000, 2 ** 20), (30000, 2 ** 31)])
+@pytest.mark.parametrize("n,docs", [(0, 5), (1, 5), (2, 2), (63, 7), (65, 2 ** 32 - 1), (1025, 40), (4000, 3), (8191, 90), (8192, 70000), (8193, 300), (50001, 256), (100000, 2 ** 20), (30000, 2 ** 31)])
 def test_sort_edges(engine, n, docs):
     """one block and many; an odd and an even number of passes; equal edges"""
     g = np.random.default_rng(n)
@@ -394,6 +394,15 @@ def test_mx_pairs(engine, n, dim):
     assert n < 2 or np.abs(c[np.tril_indices(n, -1)] - 0.9).min() > 1e-4      # the data leaves no pair at the threshold
     wu, wv = np.nonzero(np.tril(c >= 0.9, -1))
     assert (eu.cpu().numpy() == wu).all() and (ev.cpu().numpy() == wv).all() and (n < 100 or len(wu) > 0)
+
+
+@pytest.mark.parametrize("n", [2, 3, 64, 91, 92, 128, 129])
+def test_mx_pairs_order(engine, n):
+    """few enough pairs to come out in order, in the first pass or (91 rows: 4095 pairs) the second, and one more row"""
+    m = engine.mx_quantize(torch.ones(n, 40).cuda())
+    eu, ev = engine.mx_pairs(m, 0.5)
+    wu, wv = np.nonzero(np.tril(np.ones((n, n)), -1))
+    assert (eu.cpu().numpy() == wu).all() and (ev.cpu().numpy() == wv).all()
 
 
 @pytest.mark.parametrize("power", [-120, -75, -61, -56, 56, 61, 75, 120])
