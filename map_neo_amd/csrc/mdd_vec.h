@@ -95,6 +95,19 @@ __device__ __forceinline__ void store8_once(T* __restrict__ p, uint32_t n, f32x8
     }
 }
 
+// What a call moves beyond the last-level cache goes past it (ONCE): below that the next kernel finds it there
+constexpr uint64_t LAST_LEVEL = 256u << 20;
+template <typename T, bool ONCE>
+__device__ __forceinline__ f32x8 load8_or_once(const T* __restrict__ p, uint32_t n) {
+    if constexpr (ONCE) return load8_once<T>(p, n);
+    else return load8<T>(p, n);
+}
+template <typename T, bool ONCE>
+__device__ __forceinline__ void store8_or_once(T* __restrict__ p, uint32_t n, f32x8 v) {
+    if constexpr (ONCE) store8_once<T>(p, n, v);
+    else store8<T>(p, n, v);
+}
+
 // sum over the 64 lanes of a wave, the same in every lane; a butterfly, so the order is fixed
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

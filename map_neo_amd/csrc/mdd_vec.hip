@@ -61,14 +61,15 @@ template <bool NARROW>
 __device__ __forceinline__ uint32_t lane_col(uint32_t col, uint32_t dim) {
     return NARROW ? 0 : col < dim - 8 ? col : dim - 8;
 }
-template <typename T, bool NARROW>
+template <typename T, bool NARROW, bool ONCE = false>
 __device__ __forceinline__ typename vec8<T>::raw load_cols(const T* __restrict__ p, uint32_t dim) {
-    return load8_raw<T>(p, NARROW ? dim : 8);
+    if constexpr (ONCE && !NARROW) return __builtin_nontemporal_load(reinterpret_cast<const typename vec8<T>::raw_any*>(p));
+    else return load8_raw<T>(p, NARROW ? dim : 8);
 }
 
 // U rows per lane group, held by the lanes from byte lane index `first` on in steps of `step`.  ALL: every one of them is
 // named; otherwise NO_ROW is among them, for which row 0 is read and dropped, whatever it holds, NaN included.
-template <typename T, int NS, bool WEIGHTED, bool NARROW, bool ALL, int U>
+template <typename T, int NS, bool WEIGHTED, bool NARROW, bool ONCE, bool ALL, int U>
 __device__ __forceinline__ void add_rows(const PoolArgs& a, const T* __restrict__ (&table)[NS], uint32_t held, float weight, int first, int step, f32x8 (&acc)[NS]) {
     typename vec8<T>::raw raw[U][NS];
     uint32_t at[U];
@@ -78,7 +79,7 @@ __device__ __forceinline__ void add_rows(const PoolArgs& a, const T* __restrict_
     for (int u = 0; u < U; u++) {
         const uint64_t off = (uint64_t)(ALL || at[u] != NO_ROW ? at[u] : 0) * a.row_bytes;
 #pragma unroll
-        for (int n = 0; n < NS; n++) raw[u][n] = load_cols<T, NARROW>(reinterpret_cast<const T*>(reinterpret_cast<const uint8_t*>(table[n]) + off), a.dim);
+        for (int n = 0; n < NS; n++) raw[u][n] = load_cols<T, NARROW, ONCE>(reinterpret_cast<const T*>(reinterpret_cast<const uint8_t*>(table[n]) + off), a.dim);
     }
     __builtin_amdgcn_sched_barrier(0);  // all loads first: left alone, the compiler takes them one by one to save registers
     if constexpr (std::is_same_v<T, __bf16> && !WEIGHTED && ALL && !NARROW && U >= 2) {
@@ -116,7 +117,7 @@ __device__ __forceinline__ void add_rows(const PoolArgs& a, const T* __restrict_
 }
 
 // sum of the rows named by ids [beg, end) in this lane's columns; n_named = ids that name a row.  Call with all lanes.
-template <typename T, int NS, bool WEIGHTED, bool NARROW>
+template <typename T, int NS, bool WEIGHTED, bool NARROW, bool ONCE>
 __device__ __forceinline__ void sum_span(const PoolArgs& a, uint64_t beg, uint64_t end, const uint32_t (&col)[NS], f32x8 (&acc)[NS], uint32_t& n_named) {
     const int lane = (int)lane_id(), lpr = NS == 2 ? 64 : (int)a.lpr, G = 64 / lpr, g = lane / lpr;
     const T* __restrict__ table[NS];
@@ -144,12 +145,12 @@ __device__ __forceinline__ void sum_span(const PoolArgs& a, uint64_t beg, uint64
         const int steps = n >> __builtin_ctz(G);
         int j = 0;
         if constexpr (!NARROW) {
-            for (; j + 8 <= steps; j += 8) add_rows<T, NS, WEIGHTED, NARROW, true, 8>(a, table, row, w, (j * G + g) * 4, G * 4, acc);
-            if (j + 4 <= steps) add_rows<T, NS, WEIGHTED, NARROW, true, 4>(a, table, row, w, (j * G + g) * 4, G * 4, acc), j += 4;
-            if (j + 2 <= steps) add_rows<T, NS, WEIGHTED, NARROW, true, 2>(a, table, row, w, (j * G + g) * 4, G * 4, acc), j += 2;
+            for (; j + 8 <= steps; j += 8) add_rows<T, NS, WEIGHTED, NARROW, ONCE, true, 8>(a, table, row, w, (j * G + g) * 4, G * 4, acc);
+            if (j + 4 <= steps) add_rows<T, NS, WEIGHTED, NARROW, ONCE, true, 4>(a, table, row, w, (j * G + g) * 4, G * 4, acc), j += 4;
+            if (j + 2 <= steps) add_rows<T, NS, WEIGHTED, NARROW, ONCE, true, 2>(a, table, row, w, (j * G + g) * 4, G * 4, acc), j += 2;
         }
-        for (; j < steps; j++) add_rows<T, NS, WEIGHTED, NARROW, true, 1>(a, table, row, w, (j * G + g) * 4, G * 4, acc);
-        if (j * G < n) add_rows<T, NS, WEIGHTED, NARROW, false, 1>(a, table, row, w, (j * G + g) * 4, G * 4, acc);
+        for (; j < steps; j++) add_rows<T, NS, WEIGHTED, NARROW, ONCE, true, 1>(a, table, row, w, (j * G + g) * 4, G * 4, acc);
+        if (j * G < n) add_rows<T, NS, WEIGHTED, NARROW, ONCE, false, 1>(a, table, row, w, (j * G + g) * 4, G * 4, acc);
         row = next;
     }
     for (int m = lpr; m < 64; m <<= 1)
@@ -195,7 +196,7 @@ __device__ __forceinline__ void store_cols(O* __restrict__ row, const uint32_t (
         if (in[n]) store8<O>(row + col[n], NARROW ? dim : 8, v[n] * f);
 }
 
-template <typename T, typename O, int NS, bool WEIGHTED, bool NARROW>
+template <typename T, typename O, int NS, bool WEIGHTED, bool NARROW, bool ONCE>
 __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
     const uint32_t lane = lane_id(), lpr = NS == 2 ? 64 : a.lpr;
     uint32_t block = blockIdx.x, blocks = gridDim.x, slab = blockIdx.y;
@@ -234,7 +235,7 @@ __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
                 if (beg >= lo && beg < hi) begins = d;
                 beg = beg > lo ? beg : lo;
                 end = end < hi ? end : hi;
-                sum_span<T, NS, WEIGHTED, NARROW>(a, beg, end, col, acc, n_named);
+                sum_span<T, NS, WEIGHTED, NARROW, ONCE>(a, beg, end, col, acc, n_named);
                 const uint64_t at = w * 2 + slot;
                 store_cols<float, NS, NARROW>(a.part + at * a.dim, col, in, a.dim, acc, 1.0f);
                 if (lane == 0 && slab == 0) a.part_n[at] = n_named;
@@ -245,7 +246,7 @@ __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
             uint64_t beg, end;
             doc_range(a.offsets, d, a.n_ids, beg, end);
             if (a.n_pieces && end - beg > piece) continue;  // pool_join_kernel writes it
-            sum_span<T, NS, WEIGHTED, NARROW>(a, beg, end, col, acc, n_named);
+            sum_span<T, NS, WEIGHTED, NARROW, ONCE>(a, beg, end, col, acc, n_named);
             store_cols<O, NS, NARROW>(reinterpret_cast<O*>(a.out) + d * a.dim, col, in, a.dim, acc, pool_factor(a, n_named));
         }
     }
@@ -300,8 +301,9 @@ __global__ __launch_bounds__(256) void pool_join_kernel(PoolArgs a) {
 }
 
 // One row per id: eight rows per lane group in flight, read and written once -- bound by HBM: 262144 rows of 1024 in bf16 (131 MB
-// of table, 537 MB of result) in 146 us, 4.6 TB/s.
-template <typename T, bool NARROW>
+// of table, 537 MB of result) in 106 us, 6.3 TB/s, 161 with the result written through the caches; results that fit them stay
+// there (262144 x 256 in 30 us).
+template <typename T, bool NARROW, bool ONCE>
 __global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table, uint64_t n_rows, uint32_t row_bytes, uint32_t dim, uint32_t lpr,
                                                      const void* __restrict__ ids, int id_bytes, uint64_t n_ids, float scale, T* __restrict__ out) {
     constexpr uint32_t U = 8;  // U * G positions per wave and round, 64 at most: lpr is 8 to 64
@@ -322,7 +324,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ table
                 if (p + u * G + g < n_ids) {
                     f32x8 v = __builtin_convertvector(raw[u], f32x8) * scale;
                     if (r[u] == NO_ROW) v = 0.0f;  // whatever row 0 and the scale hold
-                    store8<T>(out + (p + u * G + g) * dim + col, NARROW ? dim : 8, v);
+                    store8_or_once<T, ONCE>(out + (p + u * G + g) * dim + col, NARROW ? dim : 8, v);
                 }
         }
     }
@@ -482,10 +484,10 @@ __device__ __forceinline__ void grad_key(const GradIds& g, uint64_t p, uint32_t&
     }
 }
 
-// Up to SMALL_SORT pairs in one block and one launch, all passes in LDS: 450 edges 10 us, 6750 30 (four passes each).  Counting for each
-// edge on all CUs how many are before it takes 16 for 6750, but a workspace and a launch more: 8 us less of 474 a search for near
-// pairs, and 3 more of 54 for the small one.
-// val_bits > 0: by the value's bits first, then by the key's.  MAKE: the pairs are the gradient's, made on the way in
+// Up to SMALL_SORT pairs in one block and one launch, all passes in LDS: 450 edges 10 us, 6750 30 (four passes each). Counting
+// for each edge on all CUs how many are before it takes 16 for 6750, but a workspace and a launch more: 8 us less of 474 a
+// search for near pairs, and 3 more of 54 for the small one. val_bits > 0: by the value's bits first, then by the key's. MAKE:
+// the pairs are the gradient's, made on the way in
 template <bool MAKE>
 __global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__ key, uint32_t* __restrict__ val, uint32_t n, int val_bits, int bits, GradIds g) {
     __shared__ uint32_t ks[SMALL_SORT], vs[SMALL_SORT], cnt[16][256], lds4[4];
@@ -623,26 +625,26 @@ void place_parts(PoolArgs& a, uint8_t* ws) {
 uint32_t lanes_per_row(uint32_t dim) { return dim > 256 ? 64 : dim > 128 ? 32 : dim > 64 ? 16 : 8; }
 
 // Every XCD has an L2 of 4 MB of its own.  With a row's columns shared out among them, 256 a slab, an L2 keeps its slab of the
-// table instead of a little of everything: 10000 documents of 480 ids, 64000 x 1024 in bf16, 630 -> 488 us; 30000 of 64 ids, 64000 x 768
-// in fp32, 441 -> 338.  Not where a slab would be mostly empty, where the table fits or its rows are not named again, or
-// where sums are so short that reading their ids once a slab costs more (10 ids a document: 315 us whole, 487 in slabs; at 32
-// ids 259 and 253).  Slabs of 128 columns: 40000 documents of 480 x 256 531 us instead of 497.
+// table instead of a little of everything: 10000 documents of 480 ids, 64000 x 1024 in bf16, 630 -> 488 us; 30000 of 64 ids,
+// 64000 x 768 in fp32, 441 -> 338. Not where a slab would be mostly empty, where the table fits or its rows are not named
+// again, or where sums are so short that reading their ids once a slab costs more (10 ids a document: 315 us whole, 487 in
+// slabs; at 32 ids 259 and 253). Slabs of 128 columns: 40000 documents of 480 x 256 531 us instead of 497.
 uint32_t column_slabs(const PoolArgs& a) {
     const uint32_t n = (a.dim + 255) / 256;
     if (n < 2 || n * 256 > a.dim + a.dim / 8 || a.n_rows * a.row_bytes <= (4u << 20) || a.n_ids < 2 * a.n_rows || a.n_ids < 32 * a.n_docs) return 1;
     return n;
 }
 
-template <typename T, typename O, bool WEIGHTED>
+template <typename T, typename O, bool WEIGHTED, bool ONCE>
 void launch_pool(hipStream_t s, PoolArgs a) {
     a.slabs = column_slabs(a);
     if (a.slabs > 1) a.lpr = 32;
     const uint32_t ns = a.dim > 512 && a.slabs == 1 ? 2 : 1, slabs = a.slabs > 1 ? a.slabs : (a.dim + 512 * ns - 1) / (512 * ns);
     const uint64_t cap = (1u << 20) / slabs + 1, want = (a.n_pieces + a.n_docs + 3) / 4, blocks = want < cap ? want : cap;
     const dim3 grid((unsigned)(a.slabs > 1 ? blocks * slabs : blocks), a.slabs > 1 ? 1 : slabs), block(256);
-    if (a.dim < 8) hipLaunchKernelGGL((pool_kernel<T, O, 1, WEIGHTED, true>), grid, block, 0, s, a);
-    else if (ns == 2) hipLaunchKernelGGL((pool_kernel<T, O, 2, WEIGHTED, false>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((pool_kernel<T, O, 1, WEIGHTED, false>), grid, block, 0, s, a);
+    if (a.dim < 8) hipLaunchKernelGGL((pool_kernel<T, O, 1, WEIGHTED, true, false>), grid, block, 0, s, a);
+    else if (ns == 2) hipLaunchKernelGGL((pool_kernel<T, O, 2, WEIGHTED, false, ONCE>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((pool_kernel<T, O, 1, WEIGHTED, false, ONCE>), grid, block, 0, s, a);
     if (a.n_pieces) {
         const uint32_t slabs = (a.dim + 511) / 512;
         const uint64_t cap = (1u << 20) / slabs + 1;
@@ -655,15 +657,16 @@ void launch_lookup(hipStream_t s, const T* table, uint64_t n_rows, uint64_t stri
     const uint32_t slabs = (dim + 511) / 512, lpr = lanes_per_row(dim);
     const uint64_t per_block = 4ull * (64 / lpr) * 8, cap = (1u << 22) / slabs + 1, want = (n_ids + per_block - 1) / per_block;
     const dim3 grid((unsigned)(want < cap ? want : cap), slabs), block(256);
-    auto kernel = dim < 8 ? lookup_kernel<T, true> : lookup_kernel<T, false>;
+    auto kernel = dim < 8 ? lookup_kernel<T, true, false> : n_ids * dim * sizeof(T) <= LAST_LEVEL ? lookup_kernel<T, false, false> : lookup_kernel<T, false, true>;
     hipLaunchKernelGGL(kernel, grid, block, 0, s, table, n_rows, (uint32_t)(stride * sizeof(T)), dim, lpr, ids, id_bytes, n_ids, scale, out);
 }
 
 // ------------------------------------------------------------------------------------------------ norm
 // A row is held in registers, 8 * NC columns a lane, by W waves: one up to 2048 columns (no barrier; four rows a block),
 // four up to 8192, sixteen beyond.  x is read once and everything written once: bound by HBM.  20001 x 1000 in fp16 with
-// residual 30 us (5.3 TB/s, part of it from the last-level cache); into 8 bits 262144 x 768 in bf16 with residual 331 us, 4.3
-// TB/s, where the arithmetic in 64 bits takes four fifths of the same time.
+// residual 30 us (5.3 TB/s, part of it from the last-level cache); 262144 x 768 in bf16 with residual 275 us past the caches, 290
+// through them, 8000 x 4096 41 us through and 46 past.  Into 8 bits 262144 x 768 with residual 316 us, 4.5 TB/s, where the
+// arithmetic in 64 bits takes four fifths of the same time.
 template <int W>
 __device__ __forceinline__ float row_sum(float v, float* lds) {
     v = wave_sum(v);
@@ -692,7 +695,7 @@ __device__ __forceinline__ F row_max(F v, F* lds) {
     return v;
 }
 
-template <typename T, int NC, int W>
+template <typename T, int NC, int W, bool ONCE>
 __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_kernel(const T* __restrict__ x, uint64_t xs, const T* __restrict__ res, uint64_t rs,
                                                                     const T* __restrict__ weight, float eps, uint64_t n, uint32_t dim, T* __restrict__ y,
                                                                     T* __restrict__ sum_out, float* __restrict__ rstd) {
@@ -707,9 +710,9 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_kernel(const T* __r
             const uint32_t col = (c * TPR + t) * 8;
             h[c] = 0.0f;
             if (col < dim) {
-                h[c] = load8<T>(x + row * xs + col, dim - col);
-                if (res) h[c] += load8<T>(res + row * rs + col, dim - col);
-                if (sum_out) store8<T>(sum_out + row * dim + col, dim - col, h[c]);
+                h[c] = load8_or_once<T, ONCE>(x + row * xs + col, dim - col);
+                if (res) h[c] += load8_or_once<T, ONCE>(res + row * rs + col, dim - col);
+                if (sum_out) store8_or_once<T, ONCE>(sum_out + row * dim + col, dim - col, h[c]);
             }
 #pragma unroll
             for (int k = 0; k < 8; k++) ss = fmaf(h[c][k], h[c][k], ss);
@@ -722,7 +725,7 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_kernel(const T* __r
             if (col >= dim) continue;
             f32x8 v = h[c] * r;
             if (weight) v *= load8<T>(weight + col, dim - col);
-            store8<T>(y + row * dim + col, dim - col, v);
+            store8_or_once<T, ONCE>(y + row * dim + col, dim - col, v);
         }
     }
 }
@@ -751,7 +754,7 @@ __device__ __forceinline__ float nearest8_exact(double z) {
     return (float)rint(z);
 }
 
-template <typename T, int NC, int W, int KIND>
+template <typename T, int NC, int W, int KIND, bool ONCE>
 __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* __restrict__ x, uint64_t xs, const T* __restrict__ res, uint64_t rs,
                                                                        const T* __restrict__ weight, float eps, uint64_t n, uint32_t dim,
                                                                        uint8_t* __restrict__ codes, float* __restrict__ scales, T* __restrict__ sum_out) {
@@ -770,10 +773,10 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* 
             const uint32_t col = (c * TPR + t) * 8;
             f32x8 v = 0.0f, o = 0.0f, w = 1.0f;
             if (col < dim) {
-                v = load8_once<T>(x + row * xs + col, dim - col);
-                if (res) o = load8_once<T>(res + row * rs + col, dim - col);
+                v = load8_or_once<T, ONCE>(x + row * xs + col, dim - col);
+                if (res) o = load8_or_once<T, ONCE>(res + row * rs + col, dim - col);
                 if (weight) w = load8<T>(weight + col, dim - col);
-                if (sum_out) store8_once<T>(sum_out + row * dim + col, dim - col, v + o);
+                if (sum_out) store8_or_once<T, ONCE>(sum_out + row * dim + col, dim - col, v + o);
             }
 #pragma unroll
             for (int k = 0; k < 8; k++) {
@@ -822,7 +825,9 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* 
             uint8_t* to = codes + row * dim + col;
             if (dim - col >= 8) {
                 typedef uint32_t pair_any __attribute__((ext_vector_type(2), aligned(1)));
-                __builtin_nontemporal_store(pair_any{pack[0], pack[1]}, reinterpret_cast<pair_any*>(to));
+                const pair_any v = {pack[0], pack[1]};
+                if (ONCE) __builtin_nontemporal_store(v, reinterpret_cast<pair_any*>(to));
+                else *reinterpret_cast<pair_any*>(to) = v;
             } else {
 #pragma unroll
                 for (uint32_t k = 0; k < 8; k++)
@@ -1058,7 +1063,7 @@ int mdd_embed(mdd_ctx* ctx, const void* table, int type, uint64_t n_rows, uint64
     PoolArgs a = {table, n_rows, (uint32_t)(row_stride * type_bytes(type)), dim, lanes_per_row(dim), 1, ids, id_bytes, n_ids, offsets, n_docs, mean, scale, nullptr, piece_log2_for(n_ids), n_pieces_for(n_ids), nullptr,
                   nullptr, nullptr, out};
     if (a.n_pieces) place_parts(a, (uint8_t*)ws);
-    MDD_FOR_TYPE(type, T, (launch_pool<T, T, false>(ctx->stream, a)));
+    MDD_FOR_TYPE(type, T, (launch_pool<T, T, false, false>(ctx->stream, a)));
     HIP_TRY(hipGetLastError());
     return MDD_OK;
 }
@@ -1127,13 +1132,19 @@ int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_s
     }
     hipLaunchKernelGGL(grad_starts_kernel, dim3(grid_for(n_rows + 1, 256)), dim3(256), 0, s, key, (uint32_t)n_ids, n_rows, start);
     // the sums themselves are a lookup: table rows are the documents, the sorted positions their ids, grad the table.
-    // 262144 x 1024 in bf16 into 64000 rows: 205 us for 800 MB read and written, 245 us with the sort
+    // 262144 x 1024 in bf16 into 64000 rows, 800 MB read and written: 199 us with the sort, 219 through the caches; gradients
+    // that fit the last-level cache come out of it (262144 x 256: 82 us, 98 past it)
+    const bool once = !offsets && n_grad * dim * type_bytes(type) > LAST_LEVEL;  // with documents a row is read for each of its ids
     PoolArgs a = {grad, n_grad, (uint32_t)(grad_stride * type_bytes(type)), dim, lanes_per_row(dim), 1, val, 4, n_ids, start, n_rows, 0, scale, count, piece_log2_for(n_ids), n_pieces_for(n_ids),
                   nullptr, nullptr, nullptr, table_grad};
     if (a.n_pieces) place_parts(a, base + at[4]);
     MDD_FOR_TYPE(type, T, {
-        if (out_type == MDD_F32) count ? launch_pool<T, float, true>(s, a) : launch_pool<T, float, false>(s, a);
-        else count ? launch_pool<T, T, true>(s, a) : launch_pool<T, T, false>(s, a);
+        auto run = [&](auto* out) {
+            typedef std::remove_pointer_t<decltype(out)> O;
+            count ? launch_pool<T, O, true, false>(s, a) : once ? launch_pool<T, O, false, true>(s, a) : launch_pool<T, O, false, false>(s, a);
+        };
+        if (out_type == MDD_F32) run((float*)nullptr);
+        else run((T*)nullptr);
     });
     HIP_TRY(hipGetLastError());
     return MDD_OK;
@@ -1153,10 +1164,12 @@ int mdd_rms_norm(mdd_ctx* ctx, const void* x, int type, uint64_t x_stride, const
     CHECKED(check_matrix(who, "y", y, type, dim, dim));
     REQUIRE(!sum_out || aligned_to(sum_out, type_bytes(type)), "%s: sum_out is not aligned to its elements", who);
     REQUIRE(!rstd || aligned_to(rstd, 4), "%s: rstd is not aligned", who);
+    const bool once = n_rows * dim * type_bytes(type) * (2 + (residual != nullptr) + (sum_out != nullptr)) > LAST_LEVEL;
     ON_DEVICE(ctx);
     MDD_FOR_TYPE(type, T, {
         for_width(dim, [&](auto nc, auto w) {
-            hipLaunchKernelGGL((norm_kernel<T, nc.value, w.value>), row_grid(n_rows, w.value), dim3(w.value == 16 ? 1024 : 256), 0, ctx->stream,
+            auto kernel = once ? norm_kernel<T, nc.value, w.value, true> : norm_kernel<T, nc.value, w.value, false>;
+            hipLaunchKernelGGL(kernel, row_grid(n_rows, w.value), dim3(w.value == 16 ? 1024 : 256), 0, ctx->stream,
                                (const T*)x, x_stride, (const T*)residual, residual_stride, (const T*)weight, eps, n_rows, dim, (T*)y, (T*)sum_out, rstd);
         });
     });
@@ -1178,10 +1191,12 @@ int mdd_rms_norm_q8(mdd_ctx* ctx, const void* x, int type, uint64_t x_stride, co
     if (weight) CHECKED(check_matrix(who, "weight", weight, type, dim, dim));
     REQUIRE(codes && scales && aligned_to(scales, 4), "%s: NULL buffer, or scales not aligned", who);
     REQUIRE(!sum_out || aligned_to(sum_out, type_bytes(type)), "%s: sum_out is not aligned to its elements", who);
+    const bool once = n_rows * dim * (type_bytes(type) * (1 + (residual != nullptr) + (sum_out != nullptr)) + 1) > LAST_LEVEL;
     ON_DEVICE(ctx);
     MDD_FOR_TYPE(type, T, {
         for_width(dim, [&](auto nc, auto w) {
-            auto kernel = kind == MDD_I8 ? norm_q8_kernel<T, nc.value, w.value, MDD_I8> : norm_q8_kernel<T, nc.value, w.value, MDD_E4M3>;
+            auto kernel = kind == MDD_I8 ? (once ? norm_q8_kernel<T, nc.value, w.value, MDD_I8, true> : norm_q8_kernel<T, nc.value, w.value, MDD_I8, false>)
+                                         : (once ? norm_q8_kernel<T, nc.value, w.value, MDD_E4M3, true> : norm_q8_kernel<T, nc.value, w.value, MDD_E4M3, false>);
             hipLaunchKernelGGL(kernel, row_grid(n_rows, w.value), dim3(w.value == 16 ? 1024 : 256), 0, ctx->stream, (const T*)x, x_stride,
                                (const T*)residual, residual_stride, (const T*)weight, eps, n_rows, dim, (uint8_t*)codes, scales, (T*)sum_out);
         });

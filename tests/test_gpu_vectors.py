@@ -67,6 +67,48 @@ def test_embed_documents(engine, dtype, mode, dim, lens):
     _close(got, want, R.half(dtype, want.abs()) + (cnt[:, None].double() + 4) * R.U32 * mag)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [512, 768, 1000])
+def test_embed_documents_of_a_large_table(engine, dtype, dim):
+    """a table beyond an L2 whose rows are named again: columns in slabs of 256, the last one short; one document longer than a
+    piece, empty ones, infinities and a NaN in single columns; and from rows further apart than their width"""
+    g = torch.Generator().manual_seed(dim)
+    lens = [0, 4000] + torch.randint(0, 90, (200,), generator=g).tolist() + [0, 1]
+    v = sum(lens) // 2
+    wide = torch.randn(v, dim + 8, generator=g).to(dtype)
+    wide[7, 3], wide[8, 259], wide[9, dim - 1] = float("inf"), float("nan"), -float("inf")
+    table, ids = wide[:, :dim], _ids(sum(lens), v, g)
+    assert v * dim * wide.element_size() > 4 << 20 and ids.numel() >= 32 * len(lens)
+    offs = _ragged(lens, "cuda")
+    got = engine.embed(table.contiguous().cuda(), ids.cuda(), offs, scale=0.5)
+    want, mag, cnt = R.embed(table, ids, offs, 0.5, "mean")
+    odd = ~want.isfinite()
+    g64 = got.double().cpu()
+    assert odd.any() and (g64[odd].isnan() == want[odd].isnan()).all() and (g64[odd & ~want.isnan()] == want[odd & ~want.isnan()]).all()
+    tol = R.half(dtype, want.abs()) + (cnt[:, None].double() + 4) * R.U32 * mag
+    _close(got.cpu().masked_fill(odd, 0), want.masked_fill(odd, 0), tol.masked_fill(odd, 0))
+    assert torch.equal(engine.embed(wide.cuda()[:, :dim], ids.cuda(), offs, scale=0.5).view(torch.uint8), got.view(torch.uint8))
+
+
+def test_calls_beyond_the_last_level_cache(engine):
+    """results of more than 256 MiB go past the caches: the same numbers as in two halves, which do not"""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n, dim = 70002, 1000
+    table = torch.randn(500, dim, generator=g, device="cuda")
+    ids = torch.randint(-1, 501, (n,), generator=g, device="cuda", dtype=torch.int32)
+    got = engine.embed(table, ids)
+    assert got.numel() * 4 > 1 << 28 and torch.equal(got, torch.cat([engine.embed(table, ids[: n // 2]), engine.embed(table, ids[n // 2:])]))
+    # every position a document of its own is the same gradient in the same order, read through the caches
+    each = torch.arange(n + 1, device="cuda")
+    assert torch.equal(engine.embed_backward(got, ids, 500), engine.embed_backward(got, ids, 500, each, mode="sum"))
+    x, r, w = got[: n // 2], got[n // 2:], torch.randn(dim, generator=g, device="cuda")
+    whole, parts = engine.rms_norm(x, w, r), [engine.rms_norm(a, w, b) for a, b in zip(x.chunk(3), r.chunk(3))]
+    assert all(torch.equal(whole[k], torch.cat([q[k] for q in parts])) for k in range(3))
+    for kind in ("int8", "e4m3"):
+        whole, parts = engine.rms_norm_q8(x, w, r, kind=kind), [engine.rms_norm_q8(a, w, b, kind=kind) for a, b in zip(x.chunk(4), r.chunk(4))]
+        assert all(torch.equal(whole[k].view(torch.uint8), torch.cat([q[k].view(torch.uint8) for q in parts])) for k in range(3))
+
+
 def test_embed_one_long_document_and_many_short(engine):
     """pieces of 32 to 1024 ids: one document of 300000 ids among short ones, a document of padding only"""
     g = torch.Generator().manual_seed(5)
