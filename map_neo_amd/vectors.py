@@ -137,7 +137,7 @@ class VectorOps:
         tp, ts = self._matrix(table, "table")
         ip, ib, n_ids, op, docs = self._ids(ids, offsets, mode)
         v, dim = table.shape
-        out = torch.empty((docs if op else n_ids, dim), dtype=table.dtype, device=self.device)
+        out = torch.empty(docs if op else n_ids, dim, dtype=table.dtype, device=self.device)
         wp, wb, ws = self._work(self.L.mdd_embed_ws_bytes(n_ids, dim) if op else 0)
         _lib.check(self.L.mdd_embed(self.ctx, tp, _TYPE[table.dtype], v, ts, dim, ip, ib, n_ids, op, docs, int(mode == "mean"), float(scale),
                                     out.data_ptr() if out.numel() else None, wp, wb), "mdd_embed")
@@ -156,7 +156,7 @@ class VectorOps:
             _refuse(f"dtype {dtype} is neither float32 nor the gradient's")
         _need(n_rows >= 0, "n_rows is negative")
         dim = grad.shape[1]
-        out = torch.empty((n_rows, dim), dtype=dtype, device=self.device)
+        out = torch.empty(n_rows, dim, dtype=dtype, device=self.device)
         wp, wb, ws = self._work(self.L.mdd_embed_backward_ws_bytes(n_ids, docs, n_rows, dim))
         _lib.check(self.L.mdd_embed_backward(self.ctx, gp, _TYPE[grad.dtype], gs, dim, ip, ib, n_ids, op, docs, int(mode == "mean"), float(scale),
                                              out.data_ptr() if out.numel() else None, _TYPE[dtype], n_rows, wp, wb), "mdd_embed_backward")
@@ -175,7 +175,7 @@ class VectorOps:
         """h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight.  Returns (y, h rounded to x's type -- x itself without a
         residual --, 1 / sqrt(...) as float32 [n]): what rms_norm_backward wants."""
         xp, xs, rp, rs, wp, n, dim = self._norm_args(x, weight, residual)
-        y = torch.empty((n, dim), dtype=x.dtype, device=self.device)
+        y = torch.empty(n, dim, dtype=x.dtype, device=self.device)
         total = x if residual is None else torch.empty_like(y)
         rstd = torch.empty(n, dtype=torch.float32, device=self.device)
         if n:
@@ -191,9 +191,9 @@ class VectorOps:
         if kind not in _Q8:
             _refuse(f"kind {kind!r} is neither 'int8' nor 'e4m3'")
         xp, xs, rp, rs, wp, n, dim = self._norm_args(x, weight, residual)
-        codes = torch.empty((n, dim), dtype=_Q8[kind][1], device=self.device)
+        codes = torch.empty(n, dim, dtype=_Q8[kind][1], device=self.device)
         scales = torch.empty(n, dtype=torch.float32, device=self.device)
-        total = None if residual is None else torch.empty((n, dim), dtype=x.dtype, device=self.device)
+        total = None if residual is None else torch.empty(n, dim, dtype=x.dtype, device=self.device)
         if n:
             _lib.check(self.L.mdd_rms_norm_q8(self.ctx, xp, _TYPE[x.dtype], xs, rp, rs, wp, float(eps), n, dim, _Q8[kind][0], codes.data_ptr(),
                                               scales.data_ptr(), None if total is None else total.data_ptr()), "mdd_rms_norm_q8")
@@ -210,7 +210,7 @@ class VectorOps:
         sp, ss = (None, 0) if grad_sum is None else self._matrix(grad_sum, "grad_sum", total.dtype, n, dim)
         wp = None if weight is None else self._vector(weight, "weight", (total.dtype,), dim)
         rp = self._vector(rstd, "rstd", (torch.float32,), n)
-        dx = torch.empty((n, dim), dtype=total.dtype, device=self.device)
+        dx = torch.empty(n, dim, dtype=total.dtype, device=self.device)
         dw = None if weight is None else torch.empty(dim, dtype=torch.float32, device=self.device)
         kp, kb, ws = self._work(0 if dw is None else self.L.mdd_rms_norm_backward_ws_bytes(n, dim))
         _lib.check(self.L.mdd_rms_norm_backward(self.ctx, gp, _TYPE[total.dtype], gs, hp, hs, sp, ss, wp, rp, n, dim, dx.data_ptr() if n else None,
@@ -261,8 +261,8 @@ class VectorOps:
         xp, xs = self._matrix(x, "x")
         n, dim = x.shape
         rt, ct = (n + 31) // 32, (dim + 127) // 128
-        m = MxMatrix(torch.empty((rt, ct, 4, 32, 16), dtype=torch.uint8, device=self.device),
-                     torch.empty((rt, ct, 2, 32, 2), dtype=torch.uint8, device=self.device), n, dim)
+        m = MxMatrix(torch.empty(rt, ct, 4, 32, 16, dtype=torch.uint8, device=self.device),
+                     torch.empty(rt, ct, 2, 32, 2, dtype=torch.uint8, device=self.device), n, dim)
         if n:
             _lib.check(self.L.mdd_mx_quantize(self.ctx, xp, _TYPE[x.dtype], xs, n, dim, m.codes.data_ptr(), m.scales.data_ptr()), "mdd_mx_quantize")
         return m
@@ -276,7 +276,7 @@ class VectorOps:
             _refuse(f"a has {a.cols} columns and b {b.cols}")
         if dtype not in (torch.float32, torch.bfloat16):
             _refuse(f"dtype {dtype} is neither float32 nor bfloat16")
-        out = torch.empty((a.rows, b.rows), dtype=dtype, device=self.device)
+        out = torch.empty(a.rows, b.rows, dtype=dtype, device=self.device)
         if out.numel():
             _lib.check(self.L.mdd_mx_matmul(self.ctx, ac, as_, a.rows, bc, bs, b.rows, a.cols, float(alpha), out.data_ptr(), _TYPE[dtype], b.rows),
                        "mdd_mx_matmul")
@@ -293,13 +293,14 @@ class VectorOps:
         wp, wb, ws = self._work(self.L.mdd_mx_pairs_ws_bytes(m.rows))
         cap = min(int(max_pairs), max(4096, 8 * m.rows))
         while True:
-            eu, ev = (torch.empty(cap, dtype=torch.int32, device=self.device) for _ in range(2))
-            _lib.check(self.L.mdd_mx_pairs(self.ctx, mc, ms, m.rows, m.cols, float(min_cosine), eu.data_ptr(), ev.data_ptr(), cap, cnt.data_ptr(),
-                                           wp, wb), "mdd_mx_pairs")
+            edges = torch.empty(2 * cap, dtype=torch.int32, device=self.device)
+            at = edges.data_ptr()
+            _lib.check(self.L.mdd_mx_pairs(self.ctx, mc, ms, m.rows, m.cols, float(min_cosine), at, at + 4 * cap, cap, cnt.data_ptr(), wp, wb),
+                       "mdd_mx_pairs")
             n = int(cnt.item())
             if n > max_pairs:
                 _refuse(f"{n} pairs reach {min_cosine}: more than max_pairs={max_pairs}")
             if n <= cap:
                 break
             cap = n
-        return self.sort_edges(eu[:n], ev[:n], m.rows)
+        return self.sort_edges(edges[:n], edges[cap: cap + n], m.rows)
