@@ -111,9 +111,10 @@ __device__ __forceinline__ void store_quad(O* __restrict__ p, uint32_t n, float 
     }
 }
 
-// Few rows of A (FM row tiles): every wave streams one row tile of B from memory, the A fragments come out of the caches.
-// Bound by reading B: one row against 262144 x 1024 in 24 us, 142 MB at 5.9 TB/s (the last-level cache holds half). SPLIT waves
-// share a tile's columns where there are too few tiles to fill the chip; their sums are joined in LDS in wave order.
+// Few rows of A, or few of both: every wave streams one row tile of B from memory and multiplies it with FM row tiles of A (of a
+// group of four by blockIdx.y), whose fragments come out of the caches.  Bound by reading B: one row against 262144 x 1024 in
+// 24 us, 142 MB at 5.9 TB/s (the last-level cache holds half).  SPLIT waves share a tile's columns where there are too few tiles
+// to fill the chip; their sums are joined in LDS in wave order.
 template <typename O, int FM, int SPLIT>
 __global__ __launch_bounds__(256) void mx_skinny_kernel(const uint8_t* __restrict__ ac, const uint8_t* __restrict__ as, uint64_t m, uint32_t a_tiles,
                                                         const uint8_t* __restrict__ bc, const uint8_t* __restrict__ bs, uint64_t n, uint64_t b_tiles,
@@ -122,12 +123,13 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(const uint8_t* __restric
     __shared__ float join[SPLIT > 1 ? (SPLIT - 1) * FM * 16 * 64 : 1];
     const uint32_t lane = lane_id(), wave = threadIdx.x / 64, part = wave % SPLIT;
     const uint64_t tile = (uint64_t)blockIdx.x * (4 / SPLIT) + wave / SPLIT;
+    const uint64_t first = (uint64_t)blockIdx.y * FM, here = a_tiles - first;  // row tiles of A: from which on, and how many there are
     f32x16 acc[FM];
 #pragma unroll
     for (int f = 0; f < FM; f++) acc[f] = 0.0f;
     if (tile < b_tiles) {
         const uint8_t *bp = bc + tile * col_tiles * TILE + lane * 16, *sp = bs + tile * col_tiles * STILE + lane * 2;
-        const uint8_t *ap = ac + lane * 16, *tp = as + lane * 2;
+        const uint8_t *ap = ac + first * col_tiles * TILE + lane * 16, *tp = as + first * col_tiles * STILE + lane * 2;
 #pragma unroll 1
         for (uint32_t k0 = part * U; k0 < col_tiles; k0 += SPLIT * U) {
             i32x4 b[U][2], a[U][FM][2];
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(const uint8_t* __restric
                 sb[u] = *reinterpret_cast<const uint16_t*>(sp + k * STILE);
 #pragma unroll
                 for (int f = 0; f < FM; f++) {
-                    const uint64_t at = (uint64_t)(f < (int)a_tiles ? f : a_tiles - 1) * col_tiles + k;
+                    const uint64_t at = ((uint64_t)f < here ? f : here - 1) * col_tiles + k;
                     a[u][f][0] = *reinterpret_cast<const i32x4*>(ap + at * TILE);
                     a[u][f][1] = *reinterpret_cast<const i32x4*>(ap + at * TILE + 1024);
                     sa[u][f] = *reinterpret_cast<const uint16_t*>(tp + at * STILE);
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(const uint8_t* __restric
     if (tile >= b_tiles) return;
 #pragma unroll
     for (int f = 0; f < FM; f++) {
-        const uint64_t row = f * 32 + lane % 32;
+        const uint64_t row = (first + f) * 32 + lane % 32;
         if (row >= m) continue;
 #pragma unroll
         for (int q = 0; q < 4; q++) {
@@ -207,8 +209,9 @@ struct Block {
     static constexpr int LOADS = PER_WAVE * 2 + 1;  // per wave and step: two halves of each of its tiles, and their scales
     static_assert(TILES == 2 * WAVES, "every wave loads two tiles, and their scales in one instruction of four bytes a lane");
 };
-using Big = Block<4, 2, 2, 4>;    // 256 x 256, 8 waves, one block a CU
-using Small = Block<2, 2, 2, 2>;  // 128 x 128, 4 waves, two blocks a CU
+// 256 x 256, 8 waves, one block a CU.  (128 x 128 by 4 waves, two blocks a CU, is no quicker even for a few tiles, whose steps then
+// have too few products to hide anything: 200 x 129 x 8192 64 us against 52, 45000 x 384 near pairs 447 against 220.)
+using Tiles = Block<4, 2, 2, 4>;
 
 // 16 (4) bytes of every lane from its own address to LDS, lane after lane from l on
 __device__ __forceinline__ void to_lds(const uint8_t* g, uint8_t* l) {
@@ -585,12 +588,6 @@ __global__ __launch_bounds__(B::WAVES * 64) void mx_pairs_kernel(const Packed a,
     mx_stream<B, 0>(a, a, col_tiles, lds, next, begin, finish);
 }
 
-// Large blocks read half as much from L2 per product, small ones fill the chip with fewer tiles: whichever needs less time
-// in rounds of the whole chip, a large round counted as four small ones of two blocks a CU at 5/4 of the time per product.
-bool large_blocks(uint64_t big_tiles, uint64_t small_tiles, uint64_t cus) {
-    return (big_tiles + cus - 1) / cus * 4 * 4 <= (small_tiles + 2 * cus - 1) / (2 * cus) * 2 * 5;
-}
-
 int check_packed(const char* who, const char* what, const void* codes, const void* scales) {
     REQUIRE(codes && scales, "%s: %s is NULL", who, what);
     REQUIRE(aligned_to(codes, 16) && aligned_to(scales, 16), "%s: codes and scales of %s must be 16-byte aligned", who, what);
@@ -642,33 +639,32 @@ int mdd_mx_matmul(mdd_ctx* ctx, const uint8_t* a_codes, const uint8_t* a_scales,
     REQUIRE(c && aligned_to(c, type_bytes(c_type)), "%s: c is NULL or not aligned to its elements", who);
     REQUIRE(c_stride >= n, "%s: c_stride below n", who);
     const uint64_t at = (m + 31) / 32, bt = (n + 31) / 32;
-    REQUIRE((at / Small::TA + 1) * (bt / Small::TB + 1) < MAX_TILES, "%s: m x n is above 2^31 tiles of 128 x 128", who);
+    REQUIRE((at / Tiles::TA + 1) * (bt / Tiles::TB + 1) < MAX_TILES, "%s: m x n is above 2^31 tiles of 256 x 256", who);
     ON_DEVICE(ctx);
     const uint32_t ct = (dim + 127) / 128;
     auto run = [&](auto* out) -> hipError_t {
         typedef std::remove_pointer_t<decltype(out)> O;
-        if (at <= 4) {
+        const uint64_t cus = (uint64_t)ctx->cus, groups = at <= 2 ? 1 : (at + 3) / 4;
+        // Up to 64 rows are quicker beside streamed rows of B than in tiles that stay mostly empty (64 x 262144 x 1024: 39 us, tiles 48),
+        // and so are results too small for tiles to fill the chip, up to a block a CU (1024 x 1000 x 4096: 12 us, tiles 34; with two
+        // blocks a CU both take 34).
+        if (at <= 2 || bt * groups <= cus) {
             // one wave a row tile of B fills the chip from 8 waves a CU on; below that four waves share a tile's columns
-            const bool split = bt < (uint64_t)ctx->cus * 8 && ct > 1;
+            const bool split = bt < cus * 8 && ct > 1;
             auto kernel = split ? (at == 1 ? mx_skinny_kernel<O, 1, 4> : at == 2 ? mx_skinny_kernel<O, 2, 4> : mx_skinny_kernel<O, 4, 4>)
                                 : (at == 1 ? mx_skinny_kernel<O, 1, 1> : at == 2 ? mx_skinny_kernel<O, 2, 1> : mx_skinny_kernel<O, 4, 1>);
-            hipLaunchKernelGGL(kernel, dim3((unsigned)(split ? bt : (bt + 3) / 4)), dim3(256), 0, ctx->stream, a_codes, a_scales, m, (uint32_t)at, b_codes,
-                               b_scales, n, bt, ct, alpha, out, c_stride);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(split ? bt : (bt + 3) / 4), (unsigned)groups), dim3(256), 0, ctx->stream, a_codes, a_scales, m,
+                               (uint32_t)at, b_codes, b_scales, n, bt, ct, alpha, out, c_stride);
             return hipGetLastError();
         }
         const Packed pa = {a_codes, a_scales, (uint32_t)at}, pb = {b_codes, b_scales, (uint32_t)bt};
-        const uint64_t cus = (uint64_t)ctx->cus;
-        const uint64_t big = ((at + Big::TA - 1) / Big::TA) * ((bt + Big::TB - 1) / Big::TB), small = ((at + Small::TA - 1) / Small::TA) * ((bt + Small::TB - 1) / Small::TB);
-        auto launch = [&](auto block, uint64_t tiles, uint64_t blocks) -> hipError_t {
-            typedef decltype(block) B;
-            constexpr uint32_t bytes = B::LDS + B::WAVES * B::OUT;
-            const hipError_t e = allow_lds(mx_matmul_kernel<O, B>, bytes);
-            if (e != hipSuccess) return e;
-            hipLaunchKernelGGL((mx_matmul_kernel<O, B>), dim3((unsigned)(tiles < blocks ? tiles : blocks)), dim3(B::WAVES * 64), bytes, ctx->stream, pa, m, pb, n,
-                               ct, alpha, out, c_stride);
-            return hipGetLastError();
-        };
-        return large_blocks(big, small, cus) ? launch(Big(), big, cus) : launch(Small(), small, 2 * cus);
+        const uint64_t tiles = ((at + Tiles::TA - 1) / Tiles::TA) * ((bt + Tiles::TB - 1) / Tiles::TB);
+        constexpr uint32_t bytes = Tiles::LDS + Tiles::WAVES * Tiles::OUT;
+        const hipError_t e = allow_lds(mx_matmul_kernel<O, Tiles>, bytes);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((mx_matmul_kernel<O, Tiles>), dim3((unsigned)(tiles < cus ? tiles : cus)), dim3(Tiles::WAVES * 64), bytes, ctx->stream, pa, m, pb,
+                           n, ct, alpha, out, c_stride);
+        return hipGetLastError();
     };
     HIP_TRY(c_type == MDD_F32 ? run((float*)c) : run((__bf16*)c));
     return MDD_OK;
@@ -698,17 +694,10 @@ int mdd_mx_pairs(mdd_ctx* ctx, const uint8_t* codes, const uint8_t* scales, uint
     hipLaunchKernelGGL(mx_length_kernel, dim3((unsigned)(rt < 1 ? 1 : rt < (1u << 20) ? rt : (1u << 20))), dim3(128), 0, ctx->stream, codes, scales, ct, rt,
                        length, least, count);
     if (m) {
-        const uint64_t cus = (uint64_t)ctx->cus, big = (rt + Big::TA - 1) / Big::TA, small = (rt + Small::TA - 1) / Small::TA;
-        auto launch = [&](auto block, uint64_t g, uint64_t blocks) -> hipError_t {
-            typedef decltype(block) B;
-            const hipError_t e = allow_lds(mx_pairs_kernel<B>, B::LDS);
-            if (e != hipSuccess) return e;
-            const uint64_t places = 32 * ((g + 7) / 8) * ((g + 7) / 8 + 1);
-            hipLaunchKernelGGL((mx_pairs_kernel<B>), dim3((unsigned)(places < blocks ? places : blocks)), dim3(B::WAVES * 64), B::LDS, ctx->stream,
-                               Packed{codes, scales, (uint32_t)rt}, m, ct, length, least, min_cosine, edge_u, edge_v, edge_cap, count);
-            return hipGetLastError();
-        };
-        HIP_TRY(large_blocks(big * (big + 1) / 2, small * (small + 1) / 2, cus) ? launch(Big(), big, cus) : launch(Small(), small, 2 * cus));
+        const uint64_t cus = (uint64_t)ctx->cus, bands = (rt + 8 * Tiles::TA - 1) / (8 * Tiles::TA), places = 32 * bands * (bands + 1);
+        HIP_TRY(allow_lds(mx_pairs_kernel<Tiles>, Tiles::LDS));
+        hipLaunchKernelGGL((mx_pairs_kernel<Tiles>), dim3((unsigned)(places < cus ? places : cus)), dim3(Tiles::WAVES * 64), Tiles::LDS, ctx->stream,
+                           Packed{codes, scales, (uint32_t)rt}, m, ct, length, least, min_cosine, edge_u, edge_v, edge_cap, count);
     }
     HIP_TRY(hipGetLastError());
     return MDD_OK;

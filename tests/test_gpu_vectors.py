@@ -380,13 +380,13 @@ def test_mx_quantize(engine, dtype, n, dim):
 
 
 SHAPES = [(1, 1, 1), (1, 1000, 300), (3, 33, 129), (32, 40000, 64), (33, 100, 200), (64, 31, 1500), (65, 1000, 257), (128, 70, 128), (129, 65, 96), (300, 520, 1000),
-          (130, 40000, 130), (4100, 4200, 260)]
+          (130, 40000, 130), (4100, 4200, 260), (100, 20000, 300), (1100, 1300, 520), (1500, 1600, 130), (2000, 2, 260), (2001, 3, 100), (70000, 3, 40)]
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("m,n,dim", SHAPES)
 def test_mx_matmul(engine, out, m, n, dim):
-    """streaming, split, 128- and 256-wide blocks; rows and columns that end inside a tile"""
+    """streaming, split, groups of 128 rows, tiles; rows and columns that end inside a tile"""
     g = torch.Generator().manual_seed(m + n)
     a, b = _vectors(m, dim, g), _vectors(n, dim, g)
     qa, qb = engine.mx_quantize(a.cuda()), engine.mx_quantize(b.cuda())
@@ -417,7 +417,7 @@ def test_mx_matmul_nan_blocks_and_padding(engine):
 
 @pytest.mark.parametrize("n,dim", [(0, 64), (1, 64), (2, 100), (127, 300), (700, 256), (2999, 384), (6000, 200)])
 def test_mx_pairs(engine, n, dim):
-    """duplicates well above the threshold, unrelated rows well below: both block sizes, diagonal blocks, ragged ends"""
+    """duplicates well above the threshold, unrelated rows well below: one tile and many, diagonal ones, ragged ends"""
     g = torch.Generator().manual_seed(n)
     x = torch.randn(n, dim, generator=g)
     if n > 1:
@@ -473,3 +473,6 @@ def test_mx_pairs_all_alike(engine):
     assert (eu.cpu().numpy() == wu).all() and (ev.cpu().numpy() == wv).all()
     with pytest.raises(MddError, match="more than max_pairs"):
         engine.mx_pairs(m, 0.9, max_pairs=100)
+    with pytest.raises(MddError, match="more than max_pairs"):
+        engine.mx_pairs(m, 0.9, max_pairs=0)
+    assert all(t.numel() == 0 for t in engine.mx_pairs(engine.mx_quantize(x[:1].cuda()), 0.9, max_pairs=0))
