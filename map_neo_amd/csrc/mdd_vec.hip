@@ -731,27 +731,27 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_kernel(const T* __r
 }
 
 // The nearest 8-bit value to z = y * top / big.  zf is z rounded to 32 bits, at most 2^-24 of its size off, which is below
-// 1e-5 of a step; only next to a midpoint (`tie`) does z itself decide, a correctly rounded quotient in 64 bits -- for one
-// element in some ten thousands.  So the codes are those of exact arithmetic and do not depend on how the row was summed,
-// without a division per element.
+// 1e-5 of a step; only next to a midpoint (near_tie) does exact arithmetic decide: whether y * top is above the midpoint times
+// big, the two products' difference taken without a rounding that could change its sign.  So the codes do not depend on how the
+// row was summed, without a division per element.
 template <int KIND>
-__device__ __forceinline__ float nearest8(float zf, bool& tie) {
-    float step = 1.0f;
-    if (KIND == MDD_E4M3) {
-        const int e = (int)(__float_as_uint(zf) >> 23 & 255u) - 127;
-        step = __uint_as_float((uint32_t)((e > -6 ? e : -6) - 3 + 127) << 23);
-    }
-    const float u = zf / step, q = rintf(u);  // the step is a power of two: exact
-    tie = fabsf(fabsf(u - q) - 0.5f) <= 2e-5f;
-    return q * step;
+__device__ __forceinline__ float step8(float zf) {  // from one 8-bit value to the next, as 1 / step: a power of two
+    if (KIND == MDD_I8) return 1.0f;
+    const uint32_t e = __float_as_uint(zf) >> 23 & 255u;
+    return __uint_as_float((254u + 3u - (e > 121u ? e : 121u)) << 23);  // three bits behind the leading one, 2^-9 below 2^-6
 }
 template <int KIND>
-__device__ __forceinline__ float nearest8_exact(double z) {
-    if (KIND == MDD_E4M3) {  // the step of z itself: zf may lie across a power of two
-        const double s = exp2(fmax(floor(log2(fmax(fabs(z), 0.015625))), -6.0) - 3.0);
-        return (float)(rint(z / s) * s);
-    }
-    return (float)rint(z);
+__device__ __forceinline__ bool near_tie(float zf) {
+    const float u = zf * step8<KIND>(zf), whole = 12582912.0f;  // 1.5 * 2^23: a sum with it is rounded to a whole number
+    return fabsf(u - ((u + whole) - whole)) >= 0.49998f;
+}
+template <int KIND>
+__device__ __forceinline__ float nearest8_exact(float zf, double y, double big) {
+    const float inv = step8<KIND>(zf), f = floorf(zf * inv);
+    const double top = KIND == MDD_I8 ? 127.0 : 448.0, mid = ((double)f + 0.5) / (double)inv;
+    const double p = mid * big, d = fma(y, top, -p) - fma(mid, big, -p);
+    const bool up = d > 0.0 || (d == 0.0 && floorf(f * 0.5f) * 2.0f != f);  // between two, to the even one
+    return (up ? f + 1.0f : f) / inv;
 }
 
 template <typename T, int NC, int W, int KIND, bool ONCE>
@@ -799,26 +799,30 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* 
             if (col >= dim) continue;
             uint32_t pack[2] = {0, 0};
             if (fine && big > 0) {
-                float q[8];
+                float z[8];
                 bool tie[8], any = false;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    q[k] = nearest8<KIND>((float)(y[c][k] * inv), tie[k]);
+                    z[k] = (float)(y[c][k] * inv);
+                    tie[k] = near_tie<KIND>(z[k]);
                     any |= tie[k];
                 }
                 if (any) {
 #pragma unroll
                     for (int k = 0; k < 8; k++)
-                        if (tie[k]) q[k] = nearest8_exact<KIND>(y[c][k] * (double)top / big);
+                        if (tie[k]) z[k] = nearest8_exact<KIND>(z[k], y[c][k], big);
                 }
 #pragma unroll
                 for (int k = 0; k < 8; k += 4) {
                     if (KIND == MDD_I8) {
-                        pack[k / 4] = ((uint32_t)(int)q[k] & 255u) | ((uint32_t)(int)q[k + 1] & 255u) << 8 | ((uint32_t)(int)q[k + 2] & 255u) << 16 |
-                                      ((uint32_t)(int)q[k + 3] & 255u) << 24;
+                        uint32_t b[4];  // the low byte of the sum is the whole number's
+#pragma unroll
+                        for (int l = 0; l < 4; l++) b[l] = __float_as_uint(z[k + l] + 12582912.0f);
+                        const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0C0C0400u);
+                        pack[k / 4] = hi << 16 | lo;
                     } else {
-                        int p = __builtin_amdgcn_cvt_pk_fp8_f32(q[k], q[k + 1], 0, false);  // exact: q is an e4m3 value
-                        pack[k / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[k + 2], q[k + 3], p, true);
+                        const int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[k], z[k + 1], 0, false);  // to the nearest
+                        pack[k / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[k + 2], z[k + 3], p, true);
                     }
                 }
             }
