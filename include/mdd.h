@@ -459,7 +459,8 @@ int mdd_jsonl_decode(mdd_ctx* ctx, const uint8_t* raw, uint64_t raw_bytes, uint6
  * 32 bits and every output is rounded once.  Workspaces are the caller's, 256-byte aligned, of at least the size that the
  * *_ws_bytes function (host arithmetic, needs no GPU) gives for the same sizes; two calls that may run at the same time --
  * two captured graphs that are replayed side by side, say -- need a workspace each.  Nothing here allocates, synchronises
- * or clears memory with a memset, so every call may be captured into a HIP graph.  The caller's current device is kept. */
+ * or clears memory with a memset, so every call may be captured into a HIP graph.  The caller's current device is kept.
+ * Outputs do not overlap inputs, workspaces or each other. */
 #define MDD_F32 0
 #define MDD_BF16 1
 #define MDD_F16 2

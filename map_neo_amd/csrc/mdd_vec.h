@@ -62,12 +62,6 @@ __device__ __forceinline__ typename vec8<T>::raw load8_raw(const T* __restrict__
     }
     return v;
 }
-// For data that is read, or written, once and whole: past the caches, which keep what is used again
-template <typename T>
-__device__ __forceinline__ f32x8 load8_once(const T* __restrict__ p, uint32_t n) {
-    if (n >= 8) return __builtin_convertvector(__builtin_nontemporal_load(reinterpret_cast<const typename vec8<T>::raw_any*>(p)), f32x8);
-    return __builtin_convertvector(load8_raw<T>(p, n), f32x8);
-}
 template <typename T>
 __device__ __forceinline__ f32x8 load8(const T* __restrict__ p, uint32_t n) {
     return __builtin_convertvector(load8_raw<T>(p, n), f32x8);
@@ -85,6 +79,7 @@ __device__ __forceinline__ void store8(T* __restrict__ p, uint32_t n, f32x8 v) {
     }
 }
 
+// for data that is written once and whole: past the caches, which keep what is used again
 template <typename T>
 __device__ __forceinline__ void store8_once(T* __restrict__ p, uint32_t n, f32x8 v) {
     if (n >= 8) {
@@ -98,21 +93,9 @@ __device__ __forceinline__ void store8_once(T* __restrict__ p, uint32_t n, f32x8
 // What a call moves beyond the last-level cache goes past it (ONCE): below that the next kernel finds it there
 constexpr uint64_t LAST_LEVEL = 256u << 20;
 template <typename T, bool ONCE>
-__device__ __forceinline__ f32x8 load8_or_once(const T* __restrict__ p, uint32_t n) {
-    if constexpr (ONCE) return load8_once<T>(p, n);
-    else return load8<T>(p, n);
-}
-template <typename T, bool ONCE>
 __device__ __forceinline__ void store8_or_once(T* __restrict__ p, uint32_t n, f32x8 v) {
     if constexpr (ONCE) store8_once<T>(p, n, v);
     else store8<T>(p, n, v);
-}
-
-// sum over the 64 lanes of a wave, the same in every lane; a butterfly, so the order is fixed
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, 64);
-    return v;
 }
 
 // Blocks go to the eight XCDs in turn: place of block b of n in a list of which each XCD then takes a run of neighbours

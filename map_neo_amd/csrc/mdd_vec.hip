@@ -662,71 +662,110 @@ void launch_lookup(hipStream_t s, const T* table, uint64_t n_rows, uint64_t stri
 }
 
 // ------------------------------------------------------------------------------------------------ norm
-// A row is held in registers, 8 * NC columns a lane, by W waves: one up to 2048 columns (no barrier; four rows a block),
-// four up to 8192, sixteen beyond.  x is read once and everything written once: bound by HBM.  20001 x 1000 in fp16 with
-// residual 30 us (5.3 TB/s, part of it from the last-level cache); 262144 x 768 in bf16 with residual 275 us past the caches, 290
-// through them, 8000 x 4096 41 us through and 46 past.  Into 8 bits 262144 x 768 with residual 316 us, 4.5 TB/s, where the
-// arithmetic in 64 bits takes four fifths of the same time.
-template <int W>
+// A row is held in registers, 8 * NC columns a lane, by L lanes: 16 to 64 up to 2048 columns (no barrier; 256 / L rows a block), four
+// waves up to 8192, sixteen beyond.  x is read once and everything written once: bound by HBM.  20001 x 1000 in fp16 with
+// residual 30 us (5.3 TB/s, part of it from the last-level cache); 262144 x 768 in bf16 with residual 265 us past the caches, 290
+// through them, 8000 x 4096 39 us through and 46 past.  Into 8 bits 262144 x 768 with residual 281 us, 5.0 TB/s, without 200:
+// there the arithmetic in 64 bits bounds it.
+//
+// As in the lookup, a lane's eight columns never reach over the row's end: the last lane starts early enough and overlaps its
+// neighbour, and lanes behind it read the same eight and store nothing.  So no load stands behind a branch and all of a row's are
+// on their way at once (with a branch for the end, one after the other: 262144 x 770 in bf16 185 us, so 137).
+// What a lane repeats is left out of the sums.  Rows narrower than eight (NARROW) take single elements.
+template <bool NARROW>
+struct Eight {
+    uint32_t at, skip;  // first column; how many of the eight belong to lanes before
+    bool in;            // whether any is this lane's own
+    __device__ __forceinline__ Eight(uint32_t lane_of_row, uint32_t dim) {
+        const uint32_t col = lane_of_row * 8;
+        in = col < dim;
+        at = NARROW ? 0 : col < dim - 8 ? col : dim - 8;
+        skip = NARROW ? 0 : col - at;
+    }
+    template <typename T, bool ONCE>
+    __device__ __forceinline__ f32x8 load(const T* __restrict__ row, uint32_t dim) const {
+        const auto* p = reinterpret_cast<const typename vec8<T>::raw_any*>(row + at);
+        if constexpr (NARROW) return load8<T>(row, dim);
+        else if constexpr (ONCE) return __builtin_convertvector(__builtin_nontemporal_load(p), f32x8);
+        else return __builtin_convertvector(*p, f32x8);
+    }
+    template <typename T, bool ONCE>
+    __device__ __forceinline__ void store(T* __restrict__ row, uint32_t dim, f32x8 v) const {
+        if (in) store8_or_once<T, ONCE>(row + at, NARROW ? dim : 8, v);
+    }
+    // sum of a[k] * b[k] over this lane's own
+    __device__ __forceinline__ float dot(f32x8 a, f32x8 b, uint32_t dim) const {
+        float s = 0;
+        if (!NARROW && dim % 8) {
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) s = fmaf(k >= skip ? a[k] : 0.0f, k >= skip ? b[k] : 0.0f, s);
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) s = fmaf(a[k], b[k], s);
+        }
+        return in ? s : 0.0f;
+    }
+};
+constexpr int waves_of(int l) { return l <= 64 ? 1 : l / 64; }
+template <int L>
 __device__ __forceinline__ float row_sum(float v, float* lds) {
-    v = wave_sum(v);
-    if (W == 1) return v;
+#pragma unroll
+    for (int m = (L < 64 ? L : 64) / 2; m; m >>= 1) v += __shfl_xor(v, m, 64);
+    if (L <= 64) return v;
     if (lane_id() == 0) lds[threadIdx.x / 64] = v;
     __syncthreads();
     float s = 0;
 #pragma unroll
-    for (int w = 0; w < W; w++) s += lds[w];
+    for (int w = 0; w < waves_of(L); w++) s += lds[w];
     __syncthreads();
     return s;
 }
-template <int W, typename F>
+template <int L, typename F>
 __device__ __forceinline__ F row_max(F v, F* lds) {
 #pragma unroll
-    for (int m = 32; m; m >>= 1) {
+    for (int m = (L < 64 ? L : 64) / 2; m; m >>= 1) {
         const F o = __shfl_xor(v, m, 64);
         v = v > o ? v : o;
     }
-    if (W == 1) return v;
+    if (L <= 64) return v;
     if (lane_id() == 0) lds[threadIdx.x / 64] = v;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < W; w++) v = v > lds[w] ? v : lds[w];
+    for (int w = 0; w < waves_of(L); w++) v = v > lds[w] ? v : lds[w];
     __syncthreads();
     return v;
 }
 
-template <typename T, int NC, int W, bool ONCE>
-__global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_kernel(const T* __restrict__ x, uint64_t xs, const T* __restrict__ res, uint64_t rs,
+template <typename T, int NC, int L, bool NARROW, bool ONCE>
+__global__ __launch_bounds__(L == 1024 ? 1024 : 256) void norm_kernel(const T* __restrict__ x, uint64_t xs, const T* __restrict__ res, uint64_t rs,
                                                                     const T* __restrict__ weight, float eps, uint64_t n, uint32_t dim, T* __restrict__ y,
                                                                     T* __restrict__ sum_out, float* __restrict__ rstd) {
-    constexpr uint32_t RPB = W == 1 ? 4 : 1, TPR = W * 64;
-    __shared__ float lds[W];
-    const uint32_t t = threadIdx.x % TPR;
-    for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < n; row += (uint64_t)gridDim.x * RPB) {
-        f32x8 h[NC];
+    constexpr uint32_t RPB = L <= 64 ? 256 / L : 1;  // rows a block
+    __shared__ float lds[waves_of(L)];
+    const uint32_t t = threadIdx.x % L;
+    for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / L; row < n; row += (uint64_t)gridDim.x * RPB) {
+        f32x8 h[NC], w[NC];
+#pragma unroll
+        for (int c = 0; c < NC; c++) h[c] = Eight<NARROW>(c * L + t, dim).template load<T, ONCE>(x + row * xs, dim), w[c] = 1.0f;
+        if (weight) {
+#pragma unroll
+            for (int c = 0; c < NC; c++) w[c] = Eight<NARROW>(c * L + t, dim).template load<T, false>(weight, dim);
+        }
+        if (res) {
+#pragma unroll
+            for (int c = 0; c < NC; c++) h[c] += Eight<NARROW>(c * L + t, dim).template load<T, ONCE>(res + row * rs, dim);
+        }
         float ss = 0;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            const uint32_t col = (c * TPR + t) * 8;
-            h[c] = 0.0f;
-            if (col < dim) {
-                h[c] = load8_or_once<T, ONCE>(x + row * xs + col, dim - col);
-                if (res) h[c] += load8_or_once<T, ONCE>(res + row * rs + col, dim - col);
-                if (sum_out) store8_or_once<T, ONCE>(sum_out + row * dim + col, dim - col, h[c]);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++) ss = fmaf(h[c][k], h[c][k], ss);
+            const Eight<NARROW> own(c * L + t, dim);
+            if (sum_out) own.template store<T, ONCE>(sum_out + row * dim, dim, h[c]);
+            ss += own.dot(h[c], h[c], dim);
         }
-        const float r = 1.0f / sqrtf(row_sum<W>(ss, lds) / (float)dim + eps);
+        const float r = 1.0f / sqrtf(row_sum<L>(ss, lds) / (float)dim + eps);
         if (rstd && t == 0) rstd[row] = r;
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const uint32_t col = (c * TPR + t) * 8;
-            if (col >= dim) continue;
-            f32x8 v = h[c] * r;
-            if (weight) v *= load8<T>(weight + col, dim - col);
-            store8_or_once<T, ONCE>(y + row * dim + col, dim - col, v);
-        }
+        for (int c = 0; c < NC; c++) Eight<NARROW>(c * L + t, dim).template store<T, ONCE>(y + row * dim, dim, h[c] * r * w[c]);
     }
 }
 
@@ -754,49 +793,54 @@ __device__ __forceinline__ float nearest8_exact(float zf, double y, double big) 
     return (up ? f + 1.0f : f) / inv;
 }
 
-template <typename T, int NC, int W, int KIND, bool ONCE>
-__global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* __restrict__ x, uint64_t xs, const T* __restrict__ res, uint64_t rs,
+template <typename T, int NC, int L, int KIND, bool NARROW, bool ONCE>
+__global__ __launch_bounds__(L == 1024 ? 1024 : 256) void norm_q8_kernel(const T* __restrict__ x, uint64_t xs, const T* __restrict__ res, uint64_t rs,
                                                                        const T* __restrict__ weight, float eps, uint64_t n, uint32_t dim,
                                                                        uint8_t* __restrict__ codes, float* __restrict__ scales, T* __restrict__ sum_out) {
-    constexpr uint32_t RPB = W == 1 ? 4 : 1, TPR = W * 64;
-    __shared__ float lds[W];
-    __shared__ double ldsd[W];
-    const uint32_t t = threadIdx.x % TPR;
+    constexpr uint32_t RPB = L <= 64 ? 256 / L : 1;  // rows a block
+    __shared__ float lds[waves_of(L)];
+    __shared__ double ldsd[waves_of(L)];
+    const uint32_t t = threadIdx.x % L;
     const float top = KIND == MDD_I8 ? 127.0f : 448.0f;
-    for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < n; row += (uint64_t)gridDim.x * RPB) {
+    for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / L; row < n; row += (uint64_t)gridDim.x * RPB) {
         double y[NC][8];  // h * weight: a sum and a product of 8 to 24-bit numbers, nearly always exact in 64 bits
+        f32x8 v[NC], o[NC], w[NC];
+#pragma unroll
+        for (int c = 0; c < NC; c++) v[c] = Eight<NARROW>(c * L + t, dim).template load<T, ONCE>(x + row * xs, dim), o[c] = 0.0f, w[c] = 1.0f;
+        if (res) {
+#pragma unroll
+            for (int c = 0; c < NC; c++) o[c] = Eight<NARROW>(c * L + t, dim).template load<T, ONCE>(res + row * rs, dim);
+        }
+        if (weight) {
+#pragma unroll
+            for (int c = 0; c < NC; c++) w[c] = Eight<NARROW>(c * L + t, dim).template load<T, false>(weight, dim);
+        }
         float ss = 0;
         double big = 0;
         bool bad = false;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            const uint32_t col = (c * TPR + t) * 8;
-            f32x8 v = 0.0f, o = 0.0f, w = 1.0f;
-            if (col < dim) {
-                v = load8_or_once<T, ONCE>(x + row * xs + col, dim - col);
-                if (res) o = load8_or_once<T, ONCE>(res + row * rs + col, dim - col);
-                if (weight) w = load8<T>(weight + col, dim - col);
-                if (sum_out) store8_or_once<T, ONCE>(sum_out + row * dim + col, dim - col, v + o);
-            }
+            const Eight<NARROW> own(c * L + t, dim);
+            const f32x8 h = v[c] + o[c];
+            if (sum_out) own.template store<T, ONCE>(sum_out + row * dim, dim, h);
+            ss += own.dot(h, h, dim);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float h = v[k] + o[k];
-                ss = fmaf(h, h, ss);
-                y[c][k] = ((double)v[k] + (double)o[k]) * (double)w[k];
+                y[c][k] = ((double)v[c][k] + (double)o[c][k]) * (double)w[c][k];
                 bad |= !(fabs(y[c][k]) < __builtin_inf());
                 big = fmax(big, fabs(y[c][k]));
             }
         }
         if (bad) big = __builtin_inf();  // fmax drops a NaN: an infinity stands for both
-        big = row_max<W>(big, ldsd);
-        const float r = 1.0f / sqrtf(row_sum<W>(ss, lds) / (float)dim + eps);
+        big = row_max<L>(big, ldsd);
+        const float r = 1.0f / sqrtf(row_sum<L>(ss, lds) / (float)dim + eps);
         const bool fine = big < __builtin_inf();
         if (t == 0) scales[row] = !fine ? __builtin_nanf("") : big > 0 ? (float)(big * ((double)r / top)) : 0.0f;  // (r is infinite for zeros without eps)
         const double inv = big > 0 ? (double)top / big : 0.0;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            const uint32_t col = (c * TPR + t) * 8;
-            if (col >= dim) continue;
+            const Eight<NARROW> own(c * L + t, dim);
+            if (!own.in) continue;
             uint32_t pack[2] = {0, 0};
             if (fine && big > 0) {
                 float z[8];
@@ -826,8 +870,8 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* 
                     }
                 }
             }
-            uint8_t* to = codes + row * dim + col;
-            if (dim - col >= 8) {
+            uint8_t* to = codes + row * dim + own.at;
+            if constexpr (!NARROW) {
                 typedef uint32_t pair_any __attribute__((ext_vector_type(2), aligned(1)));
                 const pair_any v = {pack[0], pack[1]};
                 if (ONCE) __builtin_nontemporal_store(v, reinterpret_cast<pair_any*>(to));
@@ -835,7 +879,7 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* 
             } else {
 #pragma unroll
                 for (uint32_t k = 0; k < 8; k++)
-                    if (col + k < dim) to[k] = (uint8_t)(pack[k / 4] >> (8 * (k % 4)));
+                    if (k < dim) to[k] = (uint8_t)(pack[k / 4] >> (8 * (k % 4)));
             }
         }
     }
@@ -844,63 +888,61 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_q8_kernel(const T* 
 // Backward: a fixed number of blocks walks the rows; the weight's gradient stays in registers over a block's rows, goes to a
 // workspace row per block and is added up by weight_grad_kernel in block order.  20001 x 1000 in fp16: 30 us with four blocks a CU
 // (43 with two: too few loads in flight), and 5 for the join.
-template <typename T, int NC, int W>
-__global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_backward_kernel(const T* __restrict__ g, uint64_t gs, const T* __restrict__ h, uint64_t hs,
+template <typename T, int NC, int L, bool NARROW>
+__global__ __launch_bounds__(L == 1024 ? 1024 : 256) void norm_backward_kernel(const T* __restrict__ g, uint64_t gs, const T* __restrict__ h, uint64_t hs,
                                                                              const T* __restrict__ gsum, uint64_t gss, const T* __restrict__ weight,
                                                                              const float* __restrict__ rstd, uint64_t n, uint32_t dim, T* __restrict__ dx,
                                                                              float* __restrict__ part) {
-    constexpr uint32_t RPB = W == 1 ? 4 : 1, TPR = W * 64;
-    __shared__ float lds[W];
-    __shared__ __attribute__((aligned(32))) float across[W == 1 ? 3 * 512 : 8];
-    const uint32_t t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    constexpr uint32_t RPB = L <= 64 ? 256 / L : 1;  // rows a block
+    __shared__ float lds[waves_of(L)];
+    __shared__ __attribute__((aligned(32))) float across[RPB > 1 ? (RPB - 1) * L * 8 : 8];
+    const uint32_t t = threadIdx.x % L, sub = threadIdx.x / L;
     f32x8 w[NC], dw[NC];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-        const uint32_t col = (c * TPR + t) * 8;
-        w[c] = 1.0f;
-        if (weight && col < dim) w[c] = load8<T>(weight + col, dim - col);
-        dw[c] = 0.0f;
+        w[c] = 1.0f, dw[c] = 0.0f;
+        if (weight) w[c] = Eight<NARROW>(c * L + t, dim).template load<T, false>(weight, dim);
     }
     for (uint64_t row = (uint64_t)blockIdx.x * RPB + sub; row < n; row += (uint64_t)gridDim.x * RPB) {
         const float r = rstd[row];
-        f32x8 nx[NC], gw[NC];
+        f32x8 nx[NC], gw[NC], more[NC];
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const Eight<NARROW> own(c * L + t, dim);
+            nx[c] = own.template load<T, false>(h + row * hs, dim);
+            gw[c] = own.template load<T, false>(g + row * gs, dim);
+        }
+        if (gsum) {
+#pragma unroll
+            for (int c = 0; c < NC; c++) more[c] = Eight<NARROW>(c * L + t, dim).template load<T, false>(gsum + row * gss, dim);
+        }
         float dot = 0;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            const uint32_t col = (c * TPR + t) * 8;
-            nx[c] = 0.0f, gw[c] = 0.0f;
-            if (col < dim) {
-                nx[c] = load8<T>(h + row * hs + col, dim - col) * r;
-                gw[c] = load8<T>(g + row * gs + col, dim - col);
-            }
+            nx[c] *= r;
             dw[c] += gw[c] * nx[c];
             gw[c] *= w[c];
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (col + k < dim) dot = fmaf(gw[c][k], nx[c][k], dot);
+            dot += Eight<NARROW>(c * L + t, dim).dot(gw[c], nx[c], dim);
         }
-        const float mean = row_sum<W>(dot, lds) / (float)dim;
+        const float mean = row_sum<L>(dot, lds) / (float)dim;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            const uint32_t col = (c * TPR + t) * 8;
-            if (col >= dim) continue;
             f32x8 v = (gw[c] - nx[c] * mean) * r;
-            if (gsum) v += load8<T>(gsum + row * gss + col, dim - col);
-            store8<T>(dx + row * dim + col, dim - col, v);
+            if (gsum) v += more[c];
+            Eight<NARROW>(c * L + t, dim).template store<T, false>(dx + row * dim, dim, v);
         }
     }
     if (!part) return;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-        const uint32_t col = (c * TPR + t) * 8;
-        if (W == 1) {
-            if (sub) *reinterpret_cast<f32x8*>(&across[(sub - 1) * 512 + t * 8]) = dw[c];
+        if (RPB > 1) {
+            if (sub) *reinterpret_cast<f32x8*>(&across[((sub - 1) * L + t) * 8]) = dw[c];
             __syncthreads();
             if (!sub)
-                for (int s = 0; s < 3; s++) dw[c] += *reinterpret_cast<const f32x8*>(&across[s * 512 + t * 8]);
+                for (uint32_t s = 0; s < RPB - 1; s++) dw[c] += *reinterpret_cast<const f32x8*>(&across[(s * L + t) * 8]);
             __syncthreads();
         }
-        if (sub == 0 && col < dim) store8<float>(part + (uint64_t)blockIdx.x * dim + col, dim - col, dw[c]);
+        if (sub == 0) Eight<NARROW>(c * L + t, dim).template store<float, false>(part + (uint64_t)blockIdx.x * dim, dim, dw[c]);
     }
 }
 
@@ -923,25 +965,37 @@ __global__ __launch_bounds__(1024) void weight_grad_kernel(const float* __restri
     }
 }
 
-uint32_t backward_blocks(uint64_t n, uint32_t dim) {
-    const uint64_t want = dim <= 2048 ? (n + 3) / 4 : n;
-    return (uint32_t)(want < 1024 ? want : 1024);  // four blocks a CU
-}
-
-// picks NC and W of a row kernel; body(NC, W) as integral constants
+// Picks NC, L and NARROW of a row kernel, whichever lanes stay idle least: body(NC, L, NARROW) as integral constants.  262144 x 768
+// in bf16 to int8 by 32 lanes with 24 columns each 200 us, by 64 with 16 258; 100000 x 100 by 16 lanes 16 us, by 64 52.
 template <typename F>
-void for_width(uint32_t dim, F&& body) {
-    if (dim <= 512) body(std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
-    else if (dim <= 1024) body(std::integral_constant<int, 2>(), std::integral_constant<int, 1>());
-    else if (dim <= 2048) body(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
-    else if (dim <= 4096) body(std::integral_constant<int, 2>(), std::integral_constant<int, 4>());
-    else if (dim <= 8192) body(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
-    else if (dim <= 16384) body(std::integral_constant<int, 2>(), std::integral_constant<int, 16>());
-    else body(std::integral_constant<int, 4>(), std::integral_constant<int, 16>());
+auto for_width(uint32_t dim, bool backward, F&& body) {
+    auto pick = [&](auto nc, auto l) { return body(nc, l, std::false_type()); };
+    typedef std::integral_constant<int, 1> one;
+    typedef std::integral_constant<int, 2> two;
+    typedef std::integral_constant<int, 3> three;
+    typedef std::integral_constant<int, 4> four;
+    if (dim < 8) return body(one(), std::integral_constant<int, 16>(), std::true_type());
+    if (dim <= 128) return pick(one(), std::integral_constant<int, 16>());
+    if (dim <= 256) return pick(one(), std::integral_constant<int, 32>());
+    if (dim <= 384 && !backward) return pick(three(), std::integral_constant<int, 16>());  // (50000 x 384 28 -> 21 us; backward 25 -> 29)
+    if (dim <= 512) return pick(one(), std::integral_constant<int, 64>());
+    if (dim <= 768) return pick(three(), std::integral_constant<int, 32>());
+    if (dim <= 1024) return pick(two(), std::integral_constant<int, 64>());
+    if (dim <= 1536) return pick(three(), std::integral_constant<int, 64>());
+    if (dim <= 2048) return pick(four(), std::integral_constant<int, 64>());
+    if (dim <= 4096) return pick(two(), std::integral_constant<int, 256>());
+    if (dim <= 8192) return pick(four(), std::integral_constant<int, 256>());
+    if (dim <= 16384) return pick(two(), std::integral_constant<int, 1024>());
+    return pick(four(), std::integral_constant<int, 1024>());
 }
-dim3 row_grid(uint64_t n, int W) {
-    const uint64_t want = W == 1 ? (n + 3) / 4 : n;
+uint64_t row_blocks(uint64_t n, int l) { return l <= 64 ? (n * l + 255) / 256 : n; }
+dim3 row_grid(uint64_t n, int l) {
+    const uint64_t want = row_blocks(n, l);
     return dim3((unsigned)(want < (1u << 20) ? want : (1u << 20)));
+}
+uint32_t backward_blocks(uint64_t n, uint32_t dim) {
+    const uint64_t want = for_width(dim, true, [&](auto, auto l, auto) { return row_blocks(n, l.value); });
+    return (uint32_t)(want < 1024 ? want : 1024);  // four blocks a CU
 }
 
 // ------------------------------------------------------------------------------------------------ edge cosines
@@ -1171,9 +1225,9 @@ int mdd_rms_norm(mdd_ctx* ctx, const void* x, int type, uint64_t x_stride, const
     const bool once = n_rows * dim * type_bytes(type) * (2 + (residual != nullptr) + (sum_out != nullptr)) > LAST_LEVEL;
     ON_DEVICE(ctx);
     MDD_FOR_TYPE(type, T, {
-        for_width(dim, [&](auto nc, auto w) {
-            auto kernel = once ? norm_kernel<T, nc.value, w.value, true> : norm_kernel<T, nc.value, w.value, false>;
-            hipLaunchKernelGGL(kernel, row_grid(n_rows, w.value), dim3(w.value == 16 ? 1024 : 256), 0, ctx->stream,
+        for_width(dim, false, [&](auto nc, auto l, auto narrow) {
+            auto kernel = once ? norm_kernel<T, nc.value, l.value, narrow.value, true> : norm_kernel<T, nc.value, l.value, narrow.value, false>;
+            hipLaunchKernelGGL(kernel, row_grid(n_rows, l.value), dim3(l.value == 1024 ? 1024 : 256), 0, ctx->stream,
                                (const T*)x, x_stride, (const T*)residual, residual_stride, (const T*)weight, eps, n_rows, dim, (T*)y, (T*)sum_out, rstd);
         });
     });
@@ -1198,10 +1252,10 @@ int mdd_rms_norm_q8(mdd_ctx* ctx, const void* x, int type, uint64_t x_stride, co
     const bool once = n_rows * dim * (type_bytes(type) * (1 + (residual != nullptr) + (sum_out != nullptr)) + 1) > LAST_LEVEL;
     ON_DEVICE(ctx);
     MDD_FOR_TYPE(type, T, {
-        for_width(dim, [&](auto nc, auto w) {
-            auto kernel = kind == MDD_I8 ? (once ? norm_q8_kernel<T, nc.value, w.value, MDD_I8, true> : norm_q8_kernel<T, nc.value, w.value, MDD_I8, false>)
-                                         : (once ? norm_q8_kernel<T, nc.value, w.value, MDD_E4M3, true> : norm_q8_kernel<T, nc.value, w.value, MDD_E4M3, false>);
-            hipLaunchKernelGGL(kernel, row_grid(n_rows, w.value), dim3(w.value == 16 ? 1024 : 256), 0, ctx->stream, (const T*)x, x_stride,
+        for_width(dim, false, [&](auto nc, auto l, auto narrow) {
+            auto kernel = kind == MDD_I8 ? (once ? norm_q8_kernel<T, nc.value, l.value, MDD_I8, narrow.value, true> : norm_q8_kernel<T, nc.value, l.value, MDD_I8, narrow.value, false>)
+                                         : (once ? norm_q8_kernel<T, nc.value, l.value, MDD_E4M3, narrow.value, true> : norm_q8_kernel<T, nc.value, l.value, MDD_E4M3, narrow.value, false>);
+            hipLaunchKernelGGL(kernel, row_grid(n_rows, l.value), dim3(l.value == 1024 ? 1024 : 256), 0, ctx->stream, (const T*)x, x_stride,
                                (const T*)residual, residual_stride, (const T*)weight, eps, n_rows, dim, (uint8_t*)codes, scales, (T*)sum_out);
         });
     });
@@ -1239,8 +1293,8 @@ int mdd_rms_norm_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t gra
     }
     float* part = weight_grad ? (float*)ws : nullptr;
     MDD_FOR_TYPE(type, T, {
-        for_width(dim, [&](auto nc, auto w) {
-            hipLaunchKernelGGL((norm_backward_kernel<T, nc.value, w.value>), dim3(blocks), dim3(w.value == 16 ? 1024 : 256), 0, ctx->stream, (const T*)grad,
+        for_width(dim, true, [&](auto nc, auto l, auto narrow) {
+            hipLaunchKernelGGL((norm_backward_kernel<T, nc.value, l.value, narrow.value>), dim3(blocks), dim3(l.value == 1024 ? 1024 : 256), 0, ctx->stream, (const T*)grad,
                                grad_stride, (const T*)h, h_stride, (const T*)grad_sum, grad_sum_stride, (const T*)weight, rstd, n_rows, dim, (T*)x_grad, part);
         });
     });

@@ -190,7 +190,7 @@ def test_embed_backward_empty(engine):
 
 
 # ---------------------------------------------------------------------------------------------------- norm
-DIMS = [(1, 3), (7, 5), (64, 1), (100, 37), (257, 9), (384, 11), (512, 4), (768, 130), (1200, 6), (1536, 9), (1000, 3), (2048, 2), (2049, 5), (5000, 3), (8192, 2), (10001, 2), (32768, 2)]
+DIMS = [(1, 3), (7, 5), (8, 33), (9, 70), (64, 1), (100, 37), (129, 18), (250, 9), (257, 9), (384, 11), (390, 21), (515, 9), (512, 4), (768, 130), (1200, 6), (1536, 9), (1000, 3), (2048, 2), (2049, 5), (5000, 3), (8192, 2), (10001, 2), (32768, 2)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
