@@ -254,10 +254,12 @@ __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
 
 // A block per eight pieces and 512 columns. The long documents that begin in them are this block's: each of the four waves adds
 // a quarter of its shares in order, eight at a time, and the quarters are added in order.
-template <typename O>
+template <typename O, bool NARROW>
 __global__ __launch_bounds__(256) void pool_join_kernel(PoolArgs a) {
     __shared__ __attribute__((aligned(32))) float quarter[3][512];
-    const uint32_t lane = lane_id(), wave = threadIdx.x / 64, col = blockIdx.y * 512u + lane * 8u;
+    const uint32_t lane = lane_id(), wave = threadIdx.x / 64, first_col = blockIdx.y * 512u + lane * 8u, col = lane_col<NARROW>(first_col, a.dim);
+    const bool in = first_col < a.dim;
+    const uint32_t wide = NARROW ? a.dim : 8;
     for (uint64_t base = (uint64_t)blockIdx.x * 8; base < a.n_pieces; base += (uint64_t)gridDim.x * 8) {
         const uint64_t mine = lane < 8 && base + lane < a.n_pieces ? a.begins[base + lane] : ~0ull;
         for (uint64_t left = __ballot(mine < a.n_docs); left; left &= left - 1) {  // the same for the whole block
@@ -273,27 +275,25 @@ __global__ __launch_bounds__(256) void pool_join_kernel(PoolArgs a) {
 #pragma unroll
             for (int m = 32; m; m >>= 1) n_named += __shfl_xor(n_named, m, 64);
             f32x8 acc = 0.0f;
-            if (col < a.dim) {
-                const float* __restrict__ part = a.part + col;
-                const uint64_t each = (last - first + 4) / 4;  // shares first + [wave * each, (wave + 1) * each)
-                uint64_t k = first + wave * each;
-                const uint64_t stop = k + each < last + 1 ? k + each : last + 1;
-                if (wave == 0) acc = load8<float>(part + at0 * a.dim, a.dim - col), k++;
-                for (; k + 8 <= stop; k += 8) {
-                    f32x8 v[8];
+            const float* __restrict__ part = a.part + col;
+            const uint64_t each = (last - first + 4) / 4;  // shares first + [wave * each, (wave + 1) * each)
+            uint64_t k = first + wave * each;
+            const uint64_t stop = k + each < last + 1 ? k + each : last + 1;
+            if (wave == 0) acc = load8<float>(part + at0 * a.dim, wide), k++;
+            for (; k + 8 <= stop; k += 8) {
+                f32x8 v[8];
 #pragma unroll
-                    for (int u = 0; u < 8; u++) v[u] = load8<float>(part + (k + u) * 2 * a.dim, a.dim - col);
+                for (int u = 0; u < 8; u++) v[u] = load8<float>(part + (k + u) * 2 * a.dim, wide);
 #pragma unroll
-                    for (int u = 0; u < 8; u++) acc += v[u];
-                }
-                for (; k < stop; k++) acc += load8<float>(part + k * 2 * a.dim, a.dim - col);
+                for (int u = 0; u < 8; u++) acc += v[u];
             }
+            for (; k < stop; k++) acc += load8<float>(part + k * 2 * a.dim, wide);
             if (wave) *reinterpret_cast<f32x8*>(&quarter[wave - 1][lane * 8]) = acc;
             __syncthreads();
-            if (wave == 0 && col < a.dim) {
+            if (wave == 0 && in) {
 #pragma unroll
                 for (int q = 0; q < 3; q++) acc += *reinterpret_cast<const f32x8*>(&quarter[q][lane * 8]);
-                store8<O>(reinterpret_cast<O*>(a.out) + d * a.dim + col, a.dim - col, acc * pool_factor(a, n_named));
+                store8<O>(reinterpret_cast<O*>(a.out) + d * a.dim + col, wide, acc * pool_factor(a, n_named));
             }
             __syncthreads();
         }
@@ -648,7 +648,8 @@ void launch_pool(hipStream_t s, PoolArgs a) {
     if (a.n_pieces) {
         const uint32_t slabs = (a.dim + 511) / 512;
         const uint64_t cap = (1u << 20) / slabs + 1;
-        hipLaunchKernelGGL((pool_join_kernel<O>), dim3((unsigned)((a.n_pieces + 7) / 8 < cap ? (a.n_pieces + 7) / 8 : cap), slabs), dim3(256), 0, s, a);
+        auto join = a.dim < 8 ? pool_join_kernel<O, true> : pool_join_kernel<O, false>;
+        hipLaunchKernelGGL(join, dim3((unsigned)((a.n_pieces + 7) / 8 < cap ? (a.n_pieces + 7) / 8 : cap), slabs), dim3(256), 0, s, a);
     }
 }
 
@@ -999,43 +1000,63 @@ uint32_t backward_blocks(uint64_t n, uint32_t dim) {
 }
 
 // ------------------------------------------------------------------------------------------------ edge cosines
-// Sixteen lanes take an edge: four edges a wave, 1024 columns of both rows in flight at once.  Bound by the gather of two rows
-// per edge: 2 million random edges on 262144 x 768 bytes (201 MB, the last-level cache) in 410 us, 7.5 TB/s, the rate at which
-// lines that miss L2 arrive; with one chunk in flight instead of four it is the same.
-__device__ __forceinline__ u32x4 load_bytes16(const uint8_t* __restrict__ p, uint32_t n) {
-    typedef uint32_t any __attribute__((ext_vector_type(4), aligned(1)));
+// L lanes take an edge, 16 columns each and four times that in flight, of both rows: 16 lanes, or fewer for rows below 128 bytes.
+// Bound by the gather of two rows per edge: 2 million random edges on 262144 x 768 bytes (201 MB, the last-level cache) in
+// 410 us, 7.5 TB/s, the rate at which lines that miss L2 arrive; with one chunk in flight instead of four it is the same.
+// As elsewhere here the last lane's 16 bytes overlap its neighbour's, so that no load stands behind a branch, and what it
+// repeats is masked out (1 million edges of 250 bytes 111 us, with a branch for the end and always 16 lanes
+// 320; of 128 bytes 40 and 84).  Rows below 16 bytes (NARROW) take single bytes.
+__device__ __forceinline__ u32x4 load_bytes(const uint8_t* __restrict__ p, uint32_t n) {  // n < 16
     u32x4 v = 0;
-    if (n >= 16) {
-        v = *reinterpret_cast<const any*>(p);
-    } else {
-        for (uint32_t k = 0; k < n; k++) {
-            const uint32_t b = (uint32_t)p[k] << (8 * (k % 4));
-            if (k < 4) v[0] |= b;
-            else if (k < 8) v[1] |= b;
-            else if (k < 12) v[2] |= b;
-            else v[3] |= b;
-        }
+    for (uint32_t k = 0; k < n; k++) {
+        const uint32_t b = (uint32_t)p[k] << (8 * (k % 4));
+        if (k < 4) v[0] |= b;
+        else if (k < 8) v[1] |= b;
+        else if (k < 12) v[2] |= b;
+        else v[3] |= b;
     }
     return v;
 }
-template <int KIND>
+template <int KIND, int L, bool NARROW>
 __global__ __launch_bounds__(256) void edge_cosine_kernel(const uint8_t* __restrict__ codes, uint64_t stride, uint64_t n_rows, uint32_t dim,
                                                           const uint32_t* __restrict__ eu, const uint32_t* __restrict__ ev, uint64_t n_edges,
                                                           float* __restrict__ cosines) {
-    const uint32_t t = threadIdx.x % 16;
-    for (uint64_t e = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16; e < n_edges; e += (uint64_t)gridDim.x * 16) {
+    typedef uint32_t any __attribute__((ext_vector_type(4), aligned(1)));
+    constexpr uint32_t STEP = L * 16;
+    const uint32_t t = threadIdx.x % L;
+    for (uint64_t e = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L; e < n_edges; e += (uint64_t)gridDim.x * (256 / L)) {
         const uint64_t u = eu[e], v = ev[e];
         const bool ok = u < n_rows && v < n_rows;
         const uint8_t *a = codes + (ok ? u : 0) * stride, *b = codes + (ok ? v : 0) * stride;
         float ab = 0, aa = 0, bb = 0;
         int iab = 0, iaa = 0, ibb = 0;  // 32768 products of at most 2^14: below 2^30
-        for (uint32_t c0 = t * 16; c0 < (ok ? dim : 0); c0 += 1024) {
+        for (uint32_t c0 = 0; c0 < (ok ? dim : 0); c0 += 4 * STEP) {
             u32x4 x[4], y[4];
+            uint32_t skip[4];
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                const uint32_t c = c0 + s * 256;
-                x[s] = 0, y[s] = 0;
-                if (c < dim) x[s] = load_bytes16(a + c, dim - c), y[s] = load_bytes16(b + c, dim - c);
+            for (uint32_t s = 0; s < 4; s++) {
+                const uint32_t c = c0 + s * STEP + t * 16;
+                x[s] = 0, y[s] = 0, skip[s] = 0;
+                if (c0 + s * STEP < dim) {  // the same for all lanes at work
+                    if constexpr (NARROW) {
+                        if (t == 0) x[s] = load_bytes(a, dim), y[s] = load_bytes(b, dim);
+                    } else {
+                        const uint32_t at = c < dim - 16 ? c : dim - 16;
+                        skip[s] = c - at;
+                        x[s] = *reinterpret_cast<const any*>(a + at);
+                        y[s] = *reinterpret_cast<const any*>(b + at);
+                    }
+                }
+            }
+            if (!NARROW && dim % STEP) {
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int drop = (int)skip[s] - 4 * k;
+                        const uint32_t keep = drop >= 4 ? 0u : drop > 0 ? 0xFFFFFFFFu << (8 * drop) : 0xFFFFFFFFu;
+                        x[s][k] &= keep, y[s][k] &= keep;
+                    }
             }
 #pragma unroll
             for (int s = 0; s < 4; s++)
@@ -1057,7 +1078,7 @@ __global__ __launch_bounds__(256) void edge_cosine_kernel(const uint8_t* __restr
                 }
         }
 #pragma unroll
-        for (int m = 8; m; m >>= 1) {
+        for (int m = L / 2; m; m >>= 1) {
             if (KIND == MDD_I8) iab += __shfl_xor(iab, m, 64), iaa += __shfl_xor(iaa, m, 64), ibb += __shfl_xor(ibb, m, 64);
             else ab += __shfl_xor(ab, m, 64), aa += __shfl_xor(aa, m, 64), bb += __shfl_xor(bb, m, 64);
         }
@@ -1314,10 +1335,17 @@ int mdd_edge_cosines(mdd_ctx* ctx, const void* codes, int kind, uint64_t row_str
     if (n_edges == 0) return MDD_OK;
     REQUIRE((codes || n_rows == 0) && edge_u && edge_v && cosines, "%s: NULL buffer", who);
     ON_DEVICE(ctx);
-    const uint64_t want = (n_edges + 15) / 16, cap = (uint64_t)ctx->cus * 64;
-    auto kernel = kind == MDD_I8 ? edge_cosine_kernel<MDD_I8> : edge_cosine_kernel<MDD_E4M3>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(want < cap ? want : cap)), dim3(256), 0, ctx->stream, (const uint8_t*)codes, row_stride, n_rows, dim, edge_u,
-                       edge_v, n_edges, cosines);
+    auto launch = [&](auto lanes, auto narrow) {
+        constexpr int L = decltype(lanes)::value;
+        const uint64_t want = (n_edges * L + 255) / 256, cap = (uint64_t)ctx->cus * 64;
+        auto kernel = kind == MDD_I8 ? edge_cosine_kernel<MDD_I8, L, decltype(narrow)::value> : edge_cosine_kernel<MDD_E4M3, L, decltype(narrow)::value>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(want < cap ? want : cap)), dim3(256), 0, ctx->stream, (const uint8_t*)codes, row_stride, n_rows, dim, edge_u,
+                           edge_v, n_edges, cosines);
+    };
+    if (dim < 16) launch(std::integral_constant<int, 4>(), std::true_type());
+    else if (dim <= 64) launch(std::integral_constant<int, 4>(), std::false_type());
+    else if (dim <= 128) launch(std::integral_constant<int, 8>(), std::false_type());
+    else launch(std::integral_constant<int, 16>(), std::false_type());
     HIP_TRY(hipGetLastError());
     return MDD_OK;
 }

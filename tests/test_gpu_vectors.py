@@ -315,7 +315,7 @@ def test_rms_norm_q8_special_rows(engine, kind):
 
 # ---------------------------------------------------------------------------------------------------- edges
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
-@pytest.mark.parametrize("dim", [1, 15, 16, 17, 255, 256, 257, 768, 1000])
+@pytest.mark.parametrize("dim", [1, 15, 16, 17, 31, 64, 65, 100, 128, 129, 255, 256, 257, 768, 1000, 1025, 2000])
 def test_edge_cosines(engine, kind, dim):
     g = torch.Generator().manual_seed(dim)
     n, e = 40, 333
@@ -336,6 +336,7 @@ def test_edge_cosines(engine, kind, dim):
     wide.view(torch.int8)[:, 2: dim + 2] = rows.view(torch.int8)
     assert torch.equal(engine.edge_cosines(wide.cuda()[:, 2: dim + 2], eu.cuda(), ev.cuda()), got)
     assert engine.edge_cosines(rows.cuda(), eu[:0].cuda(), ev[:0].cuda()).numel() == 0
+    assert (engine.edge_cosines(rows[:0].cuda(), eu.cuda(), ev.cuda()) == 0).all()       # no rows at all
 
 
 @pytest.mark.parametrize("n,docs", [(0, 5), (1, 5), (2, 2), (63, 7), (65, 2 ** 32 - 1), (1025, 40), (4000, 3), (8191, 90), (8192, 70000), (8193, 300), (50001, 256), (100000, 2 ** 20), (30000, 2 ** 31)])
