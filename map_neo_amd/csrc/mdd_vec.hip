@@ -737,6 +737,13 @@ __device__ __forceinline__ F row_max(F v, F* lds) {
     return v;
 }
 
+// 1 / sqrt(m): the hardware's reciprocal root, a unit of the last place off, and one step of Newton's iteration in 64 bits
+__device__ __forceinline__ double inverse_root(float m) {
+    if (!(m >= 0x1p-126f && m <= 0x1p126f)) return 1.0f / sqrtf(m);  // zeros and infinities among them
+    const double x = __builtin_amdgcn_rsqf(m);
+    return fma(0.5 * x, fma(-(double)m * x, x, 1.0), x);
+}
+
 template <typename T, int NC, int L, bool NARROW, bool ONCE>
 __global__ __launch_bounds__(L == 1024 ? 1024 : 256) void norm_kernel(const T* __restrict__ x, uint64_t xs, const T* __restrict__ res, uint64_t rs,
                                                                     const T* __restrict__ weight, float eps, uint64_t n, uint32_t dim, T* __restrict__ y,
@@ -763,7 +770,7 @@ __global__ __launch_bounds__(L == 1024 ? 1024 : 256) void norm_kernel(const T* _
             if (sum_out) own.template store<T, ONCE>(sum_out + row * dim, dim, h[c]);
             ss += own.dot(h[c], h[c], dim);
         }
-        const float r = 1.0f / sqrtf(row_sum<L>(ss, lds) / (float)dim + eps);
+        const float r = (float)inverse_root(row_sum<L>(ss, lds) / (float)dim + eps);
         if (rstd && t == 0) rstd[row] = r;
 #pragma unroll
         for (int c = 0; c < NC; c++) Eight<NARROW>(c * L + t, dim).template store<T, ONCE>(y + row * dim, dim, h[c] * r * w[c]);
@@ -802,7 +809,7 @@ __global__ __launch_bounds__(L == 1024 ? 1024 : 256) void norm_q8_kernel(const T
     __shared__ float lds[waves_of(L)];
     __shared__ double ldsd[waves_of(L)];
     const uint32_t t = threadIdx.x % L;
-    const float top = KIND == MDD_I8 ? 127.0f : 448.0f;
+    const double top = KIND == MDD_I8 ? 127.0 : 448.0;
     for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / L; row < n; row += (uint64_t)gridDim.x * RPB) {
         double y[NC][8];  // h * weight: a sum and a product of 8 to 24-bit numbers, nearly always exact in 64 bits
         f32x8 v[NC], o[NC], w[NC];
@@ -834,10 +841,10 @@ __global__ __launch_bounds__(L == 1024 ? 1024 : 256) void norm_q8_kernel(const T
         }
         if (bad) big = __builtin_inf();  // fmax drops a NaN: an infinity stands for both
         big = row_max<L>(big, ldsd);
-        const float r = 1.0f / sqrtf(row_sum<L>(ss, lds) / (float)dim + eps);
+        const float m = row_sum<L>(ss, lds) / (float)dim + eps;
         const bool fine = big < __builtin_inf();
-        if (t == 0) scales[row] = !fine ? __builtin_nanf("") : big > 0 ? (float)(big * ((double)r / top)) : 0.0f;  // (r is infinite for zeros without eps)
-        const double inv = big > 0 ? (double)top / big : 0.0;
+        if (t == 0) scales[row] = !fine ? __builtin_nanf("") : big > 0 ? (float)(big * (inverse_root(m) * (1.0 / top))) : 0.0f;
+        const double inv = big > 0 ? top / big : 0.0;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             const Eight<NARROW> own(c * L + t, dim);
