@@ -17,9 +17,9 @@ constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
 // neighbouring positions.  64 ids are read at once, a batch ahead; those that name a row move up to the lowest lanes, so that
 // padding costs nothing behind this point, and are handed out by lane, up to eight rows per group in flight.
 // The table of a static embedding (64000 x 256 in bf16: 33 MB) lives in the last-level cache, so the kernel is bound by
-// the caches' gather rate and its own additions, not by HBM: 40000 documents of 480 ids, 9.7 GB of rows, take 480 us = 20 TB/s; a
-// third of the lines miss L2 and come at 5.6 TB/s, and 18 of the 20 instructions per 1 KB load convert and add.  Sixteen
-// rows in flight cost more in resident waves than they gain (690 us), four are as good as eight.
+// the caches' gather rate, not by HBM: 40000 documents of 480 ids, 9.7 GB of rows, take 480 us = 20 TB/s; a third of the lines
+// miss L2, and from a table that fits there the same sums take 330 us.  Sixteen rows in flight cost more in resident waves than
+// they gain (690 us), four are as good as eight.
 //
 // Documents longer than a piece (2^piece_log2 ids) would leave one wave with all the work: the id axis is cut into pieces, a
 // piece's share of a long document goes to a workspace row in float, and pool_join_kernel adds the shares in order.  A piece
