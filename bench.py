@@ -19,6 +19,7 @@ integer work: SURVEY.md 8(d)); `cpu_baseline` is the oracle port timed on this h
 (rank 0, N=1 only; bounded sample).
 """
 import argparse
+import gc
 import json
 import os
 import sys
@@ -111,6 +112,7 @@ def stage_benchmarks(eng, text, offsets, text_bytes, with_cpu=True):
 
     def timed(fn, reps=2):
         r = fn()
+        gc.collect()                                     # here rather than, for 40 ms, in the timed calls
         torch.cuda.synchronize()
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record()
