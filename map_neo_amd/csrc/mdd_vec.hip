@@ -189,6 +189,20 @@ __device__ __forceinline__ uint64_t wave_doc_at(const uint64_t* __restrict__ off
     return lo ? lo - 1 : n_docs;
 }
 
+// documents of 64 positions in a row, lane by lane from p on: the first one's, and the begins behind it are searched in registers
+__device__ __forceinline__ uint64_t wave_docs(const uint64_t* __restrict__ offsets, uint64_t n_docs, uint64_t p) {
+    const uint32_t lane = lane_id();
+    const uint64_t p0 = p - lane, d0 = wave_doc_at(offsets, n_docs, p0), next = d0 < n_docs ? d0 + 1 : 0;
+    const uint64_t begin = next + lane < n_docs ? offsets[next + lane] - p0 : ~0ull;
+    const uint32_t ahead = begin < 64 ? (uint32_t)begin : 64u;  // of p0, 64: behind all positions
+    if (__shfl(ahead, 63, 64) < 64) return doc_at(offsets, n_docs, p);  // many documents are empty
+    uint32_t c = 0;
+#pragma unroll
+    for (uint32_t step = 32; step; step >>= 1)
+        if (__shfl(ahead, (int)(c + step - 1), 64) <= lane) c += step;
+    return d0 < n_docs ? d0 + c : c ? c - 1 : n_docs;
+}
+
 template <typename O, int NS, bool NARROW>
 __device__ __forceinline__ void store_cols(O* __restrict__ row, const uint32_t (&col)[NS], const bool (&in)[NS], uint32_t dim, const f32x8 (&v)[NS], float f) {
 #pragma unroll
@@ -447,7 +461,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __res
 
 // What the gradient sorts.  key = id, or n_rows for padding and for positions outside every document; val = the row of the
 // gradient that the position's table row took part in.  With count given, the documents' named ids are counted (whole
-// numbers: the order of the atomics does not matter; one atomic per wave where the wave lies in one document).
+// numbers: the order of the atomics does not matter; one atomic per document that a wave's positions lie in).
 struct GradIds {
     const void* ids;
     int id_bytes;
@@ -460,11 +474,12 @@ __device__ __forceinline__ void grad_key(const GradIds& g, uint64_t p, uint32_t&
     uint64_t row = p;
     uint32_t id = NO_ROW;
     bool named = false;
+    const uint64_t doc = g.offsets ? wave_docs(g.offsets, g.n_docs, p) : 0;
     if (p < g.n_ids) {
         id = named_row(g.ids, g.id_bytes, p, g.n_rows);
         named = id != NO_ROW;
         if (g.offsets) {
-            row = doc_at(g.offsets, g.n_docs, p);
+            row = doc;
             uint64_t beg = 0, end = 0;
             if (row < g.n_docs) doc_range(g.offsets, row, g.n_ids, beg, end);
             if (p < beg || p >= end) named = false;
@@ -475,12 +490,12 @@ __device__ __forceinline__ void grad_key(const GradIds& g, uint64_t p, uint32_t&
     if (!g.count) return;
     const uint64_t live = __ballot(named);
     if (!live) return;
-    const int leader = __ffsll((unsigned long long)live) - 1;
-    const uint32_t first = __shfl((uint32_t)row, leader, 64);
-    if (__ballot(named && (uint32_t)row != first) == 0) {
-        if ((int)lane_id() == leader) atomicAdd(&g.count[first], (uint32_t)__popcll(live));
-    } else if (named) {
-        atomicAdd(&g.count[row], 1u);
+    for (uint64_t left = live; left;) {
+        const int leader = __ffsll((unsigned long long)left) - 1;
+        const uint32_t first = __shfl((uint32_t)row, leader, 64);
+        const uint64_t same = __ballot(named && (uint32_t)row == first);
+        if ((int)lane_id() == leader) atomicAdd(&g.count[first], (uint32_t)__popcll(same));
+        left &= ~same;
     }
 }
 

@@ -166,6 +166,20 @@ def test_embed_backward(engine, dtype, dim, n, v, docs):
         assert torch.equal(low, got.to(dtype))
 
 
+@pytest.mark.parametrize("mode", ["mean", "sum"])
+@pytest.mark.parametrize("long", [200, 1500, 9000])
+def test_embed_backward_many_empty_documents(engine, long, mode):
+    """more documents begin within 64 positions than a wave holds, and fewer; positions before the first and behind the last one"""
+    g = torch.Generator().manual_seed(long)
+    lens = [0] * 100 + [3] + [0] * 70 + [1] * 80 + [long] + [0] * 65 + [5, 62, 64, 1, 0, 63]
+    n = sum(lens) + 150
+    ids, offs = _ids(n, 40, g), _ragged(lens, "cuda") + 100
+    grad = torch.randn(len(lens), 9, generator=g)
+    got = engine.embed_backward(grad.cuda(), ids.cuda(), 40, offs, scale=1.5, mode=mode)
+    want, mag, cnt = R.embed_backward(grad, ids, 40, offs, 1.5, mode)
+    _close(got, want, R.half(torch.float32, want.abs()) + (cnt + 4) * R.U32 * mag)
+
+
 def test_embed_gradient_against_differences(engine):
     """d loss / d table by central differences of the forward pass (linear: any step is exact up to rounding)"""
     g = torch.Generator().manual_seed(11)
