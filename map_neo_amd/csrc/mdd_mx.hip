@@ -114,11 +114,12 @@ __device__ __forceinline__ void store_quad(O* __restrict__ p, uint32_t n, float 
 // Few rows of A, or few of both: every wave streams one row tile of B from memory and multiplies it with FM row tiles of A (of a
 // group of four by blockIdx.y), whose fragments come out of the caches.  Bound by reading B: one row against 262144 x 1024 in
 // 24 us, 142 MB at 5.9 TB/s (the last-level cache holds half).  SPLIT waves share a tile's columns where there are too few tiles
-// to fill the chip; their sums are joined in LDS in wave order.
+// to fill the chip; their sums are joined in LDS in wave order.  With few rows of B it is A that streams: then the two change
+// places, and a result goes to where its row and column say (swapped).
 template <typename O, int FM, int SPLIT>
 __global__ __launch_bounds__(256) void mx_skinny_kernel(const uint8_t* __restrict__ ac, const uint8_t* __restrict__ as, uint64_t m, uint32_t a_tiles,
                                                         const uint8_t* __restrict__ bc, const uint8_t* __restrict__ bs, uint64_t n, uint64_t b_tiles,
-                                                        uint32_t col_tiles, float alpha, O* __restrict__ c, uint64_t cs) {
+                                                        uint32_t col_tiles, float alpha, O* __restrict__ c, uint64_t cs, bool swapped) {
     constexpr int U = FM == 1 ? 4 : 2;  // column tiles in flight
     __shared__ float join[SPLIT > 1 ? (SPLIT - 1) * FM * 16 * 64 : 1];
     const uint32_t lane = lane_id(), wave = threadIdx.x / 64, part = wave % SPLIT;
@@ -183,7 +184,11 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(const uint8_t* __restric
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const uint64_t col = tile * 32 + q * 8 + lane / 32 * 4;
-            if (col < n)
+            if (swapped) {
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (col + k < n) c[(col + k) * cs + row] = (O)(alpha * acc[f][q * 4 + k]);
+            } else if (col < n)
                 store_quad<O>(c + row * cs + col, (uint32_t)(n - col < 4 ? n - col : 4), alpha * acc[f][q * 4], alpha * acc[f][q * 4 + 1],
                               alpha * acc[f][q * 4 + 2], alpha * acc[f][q * 4 + 3]);
         }
@@ -644,19 +649,23 @@ int mdd_mx_matmul(mdd_ctx* ctx, const uint8_t* a_codes, const uint8_t* a_scales,
     const uint32_t ct = (dim + 127) / 128;
     auto run = [&](auto* out) -> hipError_t {
         typedef std::remove_pointer_t<decltype(out)> O;
-        const uint64_t cus = (uint64_t)ctx->cus, groups = at <= 2 ? 1 : (at + 3) / 4;
-        // Up to 64 rows are quicker beside streamed rows of B than in tiles that stay mostly empty (64 x 262144 x 1024: 39 us, tiles 48),
-        // and so are results too small for tiles to fill the chip, up to a block a CU (1024 x 1000 x 4096: 12 us, tiles 34; with two
-        // blocks a CU both take 34).
-        if (at <= 2 || bt * groups <= cus) {
-            // one wave a row tile of B fills the chip from 8 waves a CU on; below that four waves share a tile's columns
-            const bool split = bt < cus * 8 && ct > 1;
-            auto kernel = split ? (at == 1 ? mx_skinny_kernel<O, 1, 4> : at == 2 ? mx_skinny_kernel<O, 2, 4> : mx_skinny_kernel<O, 4, 4>)
-                                : (at == 1 ? mx_skinny_kernel<O, 1, 1> : at == 2 ? mx_skinny_kernel<O, 2, 1> : mx_skinny_kernel<O, 4, 1>);
-            hipLaunchKernelGGL(kernel, dim3((unsigned)(split ? bt : (bt + 3) / 4), (unsigned)groups), dim3(256), 0, ctx->stream, a_codes, a_scales, m,
-                               (uint32_t)at, b_codes, b_scales, n, bt, ct, alpha, out, c_stride);
+        const uint64_t cus = (uint64_t)ctx->cus, groups = (at + 3) / 4;
+        auto skinny = [&](const uint8_t* few_codes, const uint8_t* few_scales, uint64_t few_rows, const uint8_t* codes, const uint8_t* scales, uint64_t rows,
+                          bool swapped) -> hipError_t {
+            const uint64_t few = (few_rows + 31) / 32, tiles = (rows + 31) / 32;
+            // one wave a row tile fills the chip from 8 waves a CU on; below that four waves share a tile's columns
+            const bool split = tiles < cus * 8 && ct > 1;
+            auto kernel = split ? (few == 1 ? mx_skinny_kernel<O, 1, 4> : few == 2 ? mx_skinny_kernel<O, 2, 4> : mx_skinny_kernel<O, 4, 4>)
+                                : (few == 1 ? mx_skinny_kernel<O, 1, 1> : few == 2 ? mx_skinny_kernel<O, 2, 1> : mx_skinny_kernel<O, 4, 1>);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(split ? tiles : (tiles + 3) / 4), (unsigned)(few <= 2 ? 1 : (few + 3) / 4)), dim3(256), 0, ctx->stream,
+                               few_codes, few_scales, few_rows, (uint32_t)few, codes, scales, rows, tiles, ct, alpha, out, c_stride, swapped);
             return hipGetLastError();
-        }
+        };
+        // Up to 64 rows are quicker beside streamed rows of the other matrix than in tiles that stay mostly empty (64 x 262144
+        // x 1024: 39 us, tiles 48; 262144 x 1 x 1024 25 and 52), and so are results too small for tiles to fill the chip, up to
+        // a block a CU (1024 x 1000 x 4096: 12 us, tiles 34; with two blocks a CU both take 34).
+        if (at <= 2 || bt * groups <= cus) return skinny(a_codes, a_scales, m, b_codes, b_scales, n, false);
+        if (bt <= 2) return skinny(b_codes, b_scales, n, a_codes, a_scales, m, true);
         const Packed pa = {a_codes, a_scales, (uint32_t)at}, pb = {b_codes, b_scales, (uint32_t)bt};
         const uint64_t tiles = ((at + Tiles::TA - 1) / Tiles::TA) * ((bt + Tiles::TB - 1) / Tiles::TB);
         constexpr uint32_t bytes = Tiles::LDS + Tiles::WAVES * Tiles::OUT;

@@ -395,7 +395,8 @@ def test_mx_quantize(engine, dtype, n, dim):
 
 
 SHAPES = [(1, 1, 1), (1, 1000, 300), (3, 33, 129), (32, 40000, 64), (33, 100, 200), (64, 31, 1500), (65, 1000, 257), (128, 70, 128), (129, 65, 96), (300, 520, 1000),
-          (130, 40000, 130), (4100, 4200, 260), (100, 20000, 300), (1100, 1300, 520), (1500, 1600, 130), (2000, 2, 260), (2001, 3, 100), (70000, 3, 40)]
+          (130, 40000, 130), (4100, 4200, 260), (100, 20000, 300), (1100, 1300, 520), (1500, 1600, 130), (2000, 2, 260), (2001, 3, 100), (70000, 3, 40), (33000, 1, 300), (30001, 64, 200),
+          (40000, 33, 130)]
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
