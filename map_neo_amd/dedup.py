@@ -15,6 +15,7 @@ logic on CPU with gloo.  Nothing in this module computes a hash or a signature i
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import numpy as np
@@ -45,7 +46,6 @@ class StageTimer:
 def verified_edges(be, sig: torch.Tensor, eu: torch.Tensor, ev: torch.Tensor, min_jaccard: float):
     """The edges whose two documents agree on at least ceil(min_jaccard * K) signature components (datasketch's
     MinHash.jaccard() >= min_jaccard).  An extension: the reference has no such step (EN:136-145 unions every pair)."""
-    import math
     need = int(math.ceil(float(min_jaccard) * sig.shape[1] - 1e-9))
     keep = be.signature_matches(sig, eu, ev) >= need
     return eu[keep], ev[keep]
@@ -56,15 +56,55 @@ def verified_edges(be, sig: torch.Tensor, eu: torch.Tensor, ev: torch.Tensor, mi
 SCREEN_MARGIN = 0.05
 
 
+def _blocks(n: int, dim: int):
+    """ranges of rows that hold about 2^25 numbers each: what the checks below take into 64 bits at a time"""
+    step = max(1, (1 << 25) // max(1, dim))
+    return [(k, min(n, k + step)) for k in range(0, n, step)]
+
+
+def _cosines64(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    a, b = a.double(), b.double()
+    return (a * b).sum(1) / torch.sqrt((a * a).sum(1) * (b * b).sum(1))
+
+
+def _angles(cosines: torch.Tensor) -> torch.Tensor:
+    return torch.acos(cosines.double().clamp(-1.0, 1.0))
+
+
+def _reach(be, vectors, eu, ev, min_cosine: float) -> torch.Tensor:
+    """which pairs have vectors with a cosine >= min_cosine, decided in 64 bits by the vectors themselves; of many pairs only those
+    that their 8-bit rows leave open.  Angles on a sphere add up like distances: the angle of two vectors is that of their 8-bit
+    rows, give or take the angles between each and its own.  Open are cosines within 0.007 of 0.9 for 768 evenly sized columns,
+    far more where one column sets the step of all codes."""
+    n, dim = vectors.shape
+    keep = torch.zeros(eu.numel(), dtype=torch.bool, device=eu.device)
+    open_ = None
+    if eu.numel() > n:                                           # a row's angle to its 8-bit form costs what a pair's cosine does
+        limit = math.acos(min(1.0, min_cosine))
+        codes, _, _ = be.rms_norm_q8(vectors)
+        off = torch.empty(n, dtype=torch.float64, device=vectors.device)
+        for a, b in _blocks(n, dim):
+            off[a:b] = _angles(_cosines64(vectors[a:b], codes[a:b]) - 2.0 ** -40)
+        open_ = []
+        for a, b in _blocks(eu.numel(), 2):
+            cos, slack = be.edge_cosines(codes, eu[a:b], ev[a:b]).double(), off[eu[a:b].long()] + off[ev[a:b].long()]
+            keep[a:b] = _angles(cos - 2.0 ** -20) + slack <= limit               # 2^-20: the roundings of a cosine in 32 bits
+            open_.append(torch.nonzero(~keep[a:b] & (_angles(cos + 2.0 ** -20) - slack <= limit)).flatten() + a)
+        open_ = torch.cat(open_)
+    for a, b in _blocks(eu.numel() if open_ is None else open_.numel(), dim):
+        k = slice(a, b) if open_ is None else open_[a:b]
+        keep[k] = _cosines64(vectors[eu[k].long()], vectors[ev[k].long()]) >= min_cosine - 2.0 ** -40             # (equal rows: 1 but for roundings)
+    return keep
+
+
 def vector_edges(be, vectors: torch.Tensor, min_cosine: float, margin: float = SCREEN_MARGIN):
-    """Near-duplicate pairs by document vectors [n, dim]: every pair whose 4-bit rows reach min_cosine - margin is checked on
-    the 8-bit rows, and kept if its cosine there (off by less than 2^-7) is >= min_cosine.  Returns (u, v), u > v, ordered.  An
-    extension: the reference compares documents by their shingles only.  Vectors of zeros, and with a NaN, pair with nothing."""
+    """Near-duplicate pairs by document vectors [n, dim]: of the pairs whose 4-bit rows reach min_cosine - margin, those whose
+    vectors have a cosine >= min_cosine.  Returns (u, v), u > v, ordered.  An extension: the reference compares documents by
+    their shingles only.  Vectors of zeros, and with a NaN, pair with nothing."""
     if not 0.0 < float(min_cosine) <= 1.0:
         raise ValueError("min_cosine must be in (0, 1]")
-    codes, _, _ = be.rms_norm_q8(vectors)
     eu, ev = be.mx_pairs(be.mx_quantize(vectors), max(float(min_cosine) - margin, 0.01))
-    keep = be.edge_cosines(codes, eu, ev) >= float(min_cosine) - 2.0 ** -20      # equal rows may come out a few 2^-24 below 1
+    keep = _reach(be, vectors, eu, ev, float(min_cosine))
     return eu[keep], ev[keep]
 
 
