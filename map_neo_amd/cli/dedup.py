@@ -56,7 +56,8 @@ def build_parser() -> argparse.ArgumentParser:
                         "that are similar to each other but not to that document are split, unlike pairwise LSH verification")
     p.add_argument("--min_cosine", type=float, default=None,
                    help="extension: documents whose vectors have a cosine of at least this are duplicates too (map_neo_amd.dedup."
-                        "vector_edges); needs --embeddings, or --embedding_table with --token_ids and --token_offsets; one-GPU path only")
+                        "vector_edges: candidates come from 4-bit vectors, which may miss a few pairs, fewer than one in a thousand, that barely "
+                        "reach it; no pair below it counts); needs --embeddings, or --embedding_table with --token_ids and --token_offsets; one-GPU path only")
     p.add_argument("--embeddings", default=None,
                    help=".npy, float32 or float16 [rows, dim]: a vector for every row of the input, in the order of the files and of the "
                         "rows that are JSON objects in them (what n_rows of summary.json counts)")

@@ -66,3 +66,72 @@ def test_pairs_on_both_sides_of_the_threshold(backend, dtype, many):
     c, (u, v) = _true_cosines(x)
     assert np.abs(c - 0.9).min() > 1e-9 and ((c >= 0.9).sum() > len(x)) == many
     assert _pairs(backend, x, 0.9) == list(zip(u[c >= 0.9], v[c >= 0.9]))
+
+
+def _columns(kind, dim, g):
+    scale = torch.ones(dim, dtype=torch.float64)
+    if kind == "lognormal":
+        scale = torch.randn(dim, generator=g, dtype=torch.float64).exp()
+    elif kind == "one in 32":
+        scale[::32] = 20
+    elif kind == "first":
+        scale[0] = dim ** 0.5
+    return scale
+
+
+@pytest.mark.parametrize("t", [0.8, 0.9, 0.95])
+@pytest.mark.parametrize("dim,kind", [(2, "even"), (4, "even"), (16, "even"), (32, "even"), (64, "one in 32"), (64, "lognormal"), (256, "lognormal"),
+                                      (256, "one in 32"), (768, "one in 32"), (768, "first"), (512, "even")])
+def test_screen_keeps_pairs_at_the_threshold(dim, kind, t):
+    """the 4-bit cosines of pairs 0.002 above the threshold, noise like the rows or alike in all columns, against the margin that is
+    measured on other rows of that kind.  Less than one in a thousand may fall below it: of n pairs at most n / 1000 + 4 sqrt(n / 1000)"""
+    n = 4000 if dim > 256 else 12000
+    g = torch.Generator().manual_seed(dim)
+    scale = _columns(kind, dim, g)
+    draw = lambda k: torch.randn(k, dim, generator=g, dtype=torch.float64) * scale
+    margin = D.screen_margin(draw(3000).float(), t)
+    assert D.SCREEN_MARGIN <= margin < 0.3
+    be, x = VectorBackend(), draw(n)
+    x /= x.norm(dim=1, keepdim=True)
+    missed = 0
+    for z in (draw(n // 2), torch.randn(n - n // 2, dim, generator=g, dtype=torch.float64)):
+        o = x[:len(z)] if missed == 0 else x[-len(z):]
+        z -= (z * o).sum(1, keepdim=True) * o
+        z /= z.norm(dim=1, keepdim=True)
+        y = (t + 0.002) * o + np.sqrt(1 - (t + 0.002) ** 2) * z
+        a, b = be.mx_quantize(o.float()), be.mx_quantize(y.float())
+        missed += int(((a * b).sum(1) / (a.norm(dim=1) * b.norm(dim=1)) < t - margin).sum())
+    assert missed <= n / 1000 + 4 * (n / 1000) ** 0.5
+
+
+@pytest.mark.parametrize("dim,kind", [(4, "even"), (16, "even"), (256, "one in 32"), (768, "first")])
+def test_narrow_and_uneven_vectors(backend, dim, kind):
+    """all pairs at 0.8, those just above it included: 300 planted ones at 0.8 + 10^-3"""
+    g = torch.Generator().manual_seed(dim + 1)
+    x = torch.randn(600, dim, generator=g, dtype=torch.float64) * _columns(kind, dim, g)
+    x /= x.norm(dim=1, keepdim=True)
+    z = x[torch.randperm(600, generator=g)[:300]]
+    z = torch.where((z - x[:300]).abs().amax(1, keepdim=True) == 0, x[300:], z)
+    z = z - (z * x[:300]).sum(1, keepdim=True) * x[:300]
+    x[300:] = 0.801 * x[:300] + np.sqrt(1 - 0.801 ** 2) * z / z.norm(dim=1, keepdim=True)
+    x = x.float()
+    c, (u, v) = _true_cosines(x)
+    assert np.abs(c - 0.8).min() > 1e-9
+    got, want = set(_pairs(backend, x, 0.8)), set(zip(u[c >= 0.8].tolist(), v[c >= 0.8].tolist()))
+    assert got <= want and {(300 + k, k) for k in range(300)} <= want
+    assert len(want - got) <= len(want) / 1000
+    narrow = D.vector_edges(backend, x.to(backend.device), 0.8, margin=0.05)[0].numel()
+    assert len(want) - narrow > 10                               # what a fixed margin of 0.05 misses
+
+
+def test_four_bits_are_the_operators():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(50, 100, generator=g) * torch.randn(100, generator=g).exp()
+    x[3, :32], x[4, 40], x[6, 96:] = 0, 2.0 ** -100, 2.0 ** -90
+    x[5, :8] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9])
+    assert torch.equal(D._four_bits(x)[:, :100].double(), VectorBackend().mx_quantize(x))
+    x[7, :32] = 2.0 ** -140
+    assert D._four_bits(x).isfinite().all()
+    x[8, 50], x[9, 7] = float("inf"), float("nan")
+    assert 0.05 <= D.screen_margin(x, 0.9) < 0.3
+    assert D.screen_margin(torch.zeros(5, 8), 0.9) == D.screen_margin(x[:1], 0.9) == D.SCREEN_MARGIN
