@@ -532,7 +532,7 @@ int mdd_sort_edges(mdd_ctx* ctx, uint32_t* edge_u, uint32_t* edge_v, uint64_t n_
  *            edge_v in no fixed order, at most edge_cap of them; *n_edges (device u64, set by the call) counts all of them.
  *            The comparison is one of 32-bit numbers: a pair within 2^-20 of min_cosine may fall on either side.
  *            Rows of zeros, with a NaN, or of a length outside [2^-60, 2^60] have no pairs.  Rows of similar length are fastest.  m <= MDD_MX_MAX_PAIR_ROWS
- *            (2^22: 10^13 pairs; larger sets are compared block by block with matmul). */
+ *            (2^22: 10^13 pairs; larger sets in ranges of rows, two at a time side by side). */
 #define MDD_MX_MAX_PAIR_ROWS 4194304
 #define MDD_MX_MAX_ROWS 2147483392u /* 2^31 - 256: quantize, matmul */
 #define MDD_MX_TILE_ROWS 32

@@ -124,6 +124,9 @@ def _write_shard(task):
     return kept
 
 
+MAX_IDS = (1 << 31) - 1          # of one embedding lookup
+
+
 def _check_vector_args(args, distributed):
     table = (args.embedding_table, args.token_ids, args.token_offsets)
     given = bool(args.embeddings) + all(table)
@@ -165,7 +168,16 @@ def document_vectors(eng, args, rows, n_rows):
     if offs.size and (offs[0] < 0 or offs[-1] > ids.size or (np.diff(offs) < 0).any()):
         raise SystemExit("%s does not ascend within the %d entries of %s" % (args.token_offsets, ids.size, args.token_ids))
     up = lambda a: torch.from_numpy(np.array(a)).to(eng.device)
-    return eng.embed(up(table), up(ids), up(offs), mode="mean")[up(rows)]
+    if ids.size <= MAX_IDS:
+        return eng.embed(up(table), up(ids), up(offs), mode="mean")[up(rows)]
+    device_table, parts, k = up(table), [], 0
+    while k < n_rows:                                            # as many whole rows as one lookup takes
+        end = int(np.searchsorted(offs, offs[k] + MAX_IDS, side="right")) - 1
+        if end == k:
+            raise SystemExit("row %d has %d token ids: more than %d" % (k, offs[k + 1] - offs[k], MAX_IDS))
+        parts.append(eng.embed(device_table, up(ids[offs[k]: offs[end]]), up(offs[k: end + 1] - offs[k]), mode="mean"))
+        k = end
+    return torch.cat(parts)[up(rows)]
 
 
 def run(args, engine_factory=None) -> dict:

@@ -22,6 +22,7 @@ import numpy as np
 import torch
 
 from .minhash import BANDS, NUM_PERM, ROWS, SEED, WIDTH
+from .vectors import MAX_PAIR_ROWS, TooManyPairs
 
 
 class StageTimer:
@@ -128,19 +129,91 @@ def _reach(be, vectors, eu, ev, min_cosine: float) -> torch.Tensor:
     return keep
 
 
-def vector_edges(be, vectors: torch.Tensor, min_cosine: float, margin: Optional[float] = None):
-    """Near-duplicate pairs by document vectors [n, dim]: of the pairs whose 4-bit rows reach min_cosine - margin (default: by
-    screen_margin), those whose vectors have a cosine >= min_cosine.  Returns (u, v), u > v, ordered.  Every pair returned reaches
-    min_cosine; the screen may miss a few, fewer than one in a thousand, of those that barely reach it.  An extension: the
-    reference compares documents by their shingles only.  Vectors of zeros, and with a NaN, pair with nothing."""
+def _near_pairs(be, vectors, min_cosine: float, margin: Optional[float] = None, split: bool = True):
+    """yields (u, v), u > v: every pair of vector_edges once, in one piece and ordered where one search takes them all.  Rows
+    beyond MAX_PAIR_ROWS, and sets with more candidates than mx_pairs returns, are cut into ranges: each is searched by itself,
+    and each two of them as one matrix, of which the pairs across count (twice the products of a single search)."""
     if not 0.0 < float(min_cosine) <= 1.0:
         raise ValueError("min_cosine must be in (0, 1]")
-    rows4 = be.mx_quantize(vectors)                              # (checks what it is given)
+    n = vectors.shape[0]
     if margin is None:
         margin = screen_margin(vectors, float(min_cosine))
-    eu, ev = be.mx_pairs(rows4, max(float(min_cosine) - margin, 0.01))
-    keep = _reach(be, vectors, eu, ev, float(min_cosine))
-    return eu[keep], ev[keep]
+    todo = [((0, n), None)]
+    while todo:
+        one, two = todo.pop()
+        first, size = one[1] - one[0], sum(r[1] - r[0] for r in (one, two) if r)
+        cuts = 2
+        if size <= MAX_PAIR_ROWS:
+            x = vectors[one[0]: one[1]] if two is None else torch.cat([vectors[r[0]: r[1]] for r in (one, two)])
+            try:
+                u, v = be.mx_pairs(be.mx_quantize(x), max(float(min_cosine) - margin, 0.01))
+            except TooManyPairs as e:
+                if not split or size <= 2:
+                    raise
+                cuts = min(size, 64, max(2, math.ceil(2 * math.sqrt(e.count / max(1, e.limit)))))
+            else:
+                if two is not None:
+                    across = (u >= first) & (v < first)
+                    u, v = u[across], v[across]
+                keep = _reach(be, x, u, v, float(min_cosine))
+                u, v = u[keep], v[keep]
+                yield (u if one[0] == 0 and two is None else u + (one[0] if two is None else two[0] - first)), (v if one[0] == 0 else v + one[0])
+                continue
+        elif not split:
+            raise TooManyPairs(size, MAX_PAIR_ROWS, min_cosine)
+        pieces = [[p for p in zip(c[:-1], c[1:]) if p[0] < p[1]] for c in ([r[0] + (r[1] - r[0]) * k // cuts for k in range(cuts + 1)] for r in (one, two) if r)]
+        if two is None:
+            todo += [(p, None) for p in pieces[0]] + [(p, q) for k, q in enumerate(pieces[0]) for p in pieces[0][:k]]
+        else:
+            todo += [(p, q) for p in pieces[0] for q in pieces[1]]
+
+
+def vector_edges(be, vectors: torch.Tensor, min_cosine: float, margin: Optional[float] = None, max_pairs: int = 1 << 28):
+    """Near-duplicate pairs by document vectors [n, dim]: of the pairs whose 4-bit rows reach min_cosine - margin (default: by
+    screen_margin), those whose vectors have a cosine >= min_cosine.  Returns (u, v), u > v, ordered; more than max_pairs raise
+    TooManyPairs.  Every pair returned reaches min_cosine; the screen may miss a few, fewer than one in a thousand, of those
+    that barely reach it.  An extension: the reference compares documents by their shingles only.  Vectors of zeros, with a
+    NaN, or of a length outside [2^-60, 2^60] pair with nothing."""
+    parts, count = [], 0
+    for u, v in _near_pairs(be, vectors, min_cosine, margin):
+        count += u.numel()
+        if count > max_pairs:
+            raise TooManyPairs(count, max_pairs, float(min_cosine))
+        parts.append((u, v))
+    if len(parts) == 1:
+        return parts[0]
+    key = torch.sort(torch.cat([u.long() << 32 | v.long() for u, v in parts])).values
+    return (key >> 32).int(), (key & 0xFFFFFFFF).int()
+
+
+def _first_equal(vectors: torch.Tensor) -> torch.Tensor:
+    """int64 [n]: the first row that holds the same bits as this one; the row itself where it pairs with nothing"""
+    n, dim = vectors.shape
+    dev, me = vectors.device, torch.arange(n, device=vectors.device)
+    mul = torch.randint(-2 ** 63, 2 ** 63 - 1, (dim,), generator=torch.Generator().manual_seed(0)).to(dev)
+    bits = {4: torch.int32, 2: torch.int16}[vectors.element_size()]
+    h, live = torch.empty(n, dtype=torch.int64, device=dev), torch.empty(n, dtype=torch.bool, device=dev)
+    for a, b in _blocks(n, dim):
+        x = vectors[a:b].contiguous()
+        h[a:b] = (x.view(bits).long() * mul).sum(1)
+        length = x.double().norm(dim=1)
+        live[a:b] = (length >= 2.0 ** -60) & (length <= 2.0 ** 60)
+    values, inverse = torch.unique(h, return_inverse=True)
+    first = torch.full((values.numel(),), n, dtype=torch.int64, device=dev).scatter_reduce_(0, inverse, me, "amin")[inverse]
+    for a, b in _blocks(n, dim):                                 # equal sums are not yet equal rows
+        live[a:b] &= (vectors[a:b] == vectors[first[a:b]]).all(1)
+    return torch.where(live, first, me)
+
+
+def _join_near(be, labels, vectors, min_cosine: float):
+    """unions the near pairs of `vectors` into labels without holding all of them: equal rows, of which a corpus may have any
+    number (empty pages, error pages), are joined to the first one and searched once"""
+    first = _first_equal(vectors)
+    me = torch.arange(first.numel(), device=first.device)
+    again, row = torch.nonzero(first != me).flatten(), torch.nonzero(first == me).flatten()
+    be.components_union(labels, again.int(), first[again].int())
+    for u, v in _near_pairs(be, vectors[row] if again.numel() else vectors, min_cosine):
+        be.components_union(labels, row[u.long()].int(), row[v.long()].int())
 
 
 def cluster_local(be, sig: torch.Tensor, bands: int = BANDS, rows: int = ROWS, key_bits: int = 64,
@@ -149,7 +222,9 @@ def cluster_local(be, sig: torch.Tensor, bands: int = BANDS, rows: int = ROWS, k
     """Band records -> buckets/edges -> union-find -> removed mask for signatures already in HBM
     (EN:133-145 / ZH-2..ZH-4).  Document index = row of `sig`.  min_jaccard (default None = the reference's behaviour)
     drops candidate edges (document, smallest document of its bucket) whose estimated Jaccard similarity is lower.  vectors
-    [n, dim] with min_cosine (default None) add the pairs of vector_edges."""
+    [n, dim] with min_cosine (default None) add the pairs of vector_edges; where one search does not take them all (more than
+    MAX_PAIR_ROWS documents, or 2^28 candidate pairs), they are joined piece by piece and edge_u / edge_v are one edge
+    for every document that is not the smallest of its component, to that one."""
     n, num_perm = sig.shape
     if (vectors is None) != (min_cosine is None):
         raise ValueError("vectors and min_cosine go together")
@@ -163,13 +238,22 @@ def cluster_local(be, sig: torch.Tensor, bands: int = BANDS, rows: int = ROWS, k
     if min_jaccard is not None:
         eu, ev = verified_edges(be, sig, eu, ev, min_jaccard)
         mark("verify")
+    joined = False
     if vectors is not None:
-        vu, vv = vector_edges(be, vectors, min_cosine)
-        eu, ev = torch.cat([eu, vu]), torch.cat([ev, vv])
+        try:
+            for vu, vv in _near_pairs(be, vectors, min_cosine, split=False):
+                eu, ev = torch.cat([eu, vu]), torch.cat([ev, vv])
+            joined = True
+        except TooManyPairs:
+            pass
         mark("vector_edges")
     labels = be.components_init(n)
     be.components_union(labels, eu, ev)
+    if vectors is not None and not joined:
+        _join_near(be, labels, vectors, min_cosine)
     be.components_finish(labels)
+    if vectors is not None and not joined:
+        eu, ev = be.forest_edges(labels, n)
     removed, n_removed = be.removed_mask(labels, 0, n)
     mark("components")
     return {"sig": sig, "key": key, "meta": meta, "edge_u": eu, "edge_v": ev, "labels": labels,

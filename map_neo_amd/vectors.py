@@ -21,6 +21,15 @@ _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _Q8 = {"int8": (3, torch.int8), "e4m3": (4, torch.float8_e4m3fn)}
 _Q8_OF = {torch.int8: 3, torch.float8_e4m3fn: 4}
 MAX_DIM = 32768
+MAX_PAIR_ROWS = 1 << 22          # of one search for near pairs
+
+
+class TooManyPairs(_lib.MddError):
+    """a search for near pairs found `count` of them, more than the caller's `limit`"""
+
+    def __init__(self, count: int, limit: int, min_cosine: float):
+        super().__init__(f"{count} pairs reach {min_cosine}: more than max_pairs={limit}")
+        self.count, self.limit = count, limit
 
 
 class MxMatrix(NamedTuple):
@@ -286,7 +295,7 @@ class VectorOps:
     def mx_pairs(self, m: MxMatrix, min_cosine: float, max_pairs: int = 1 << 28):
         """Every pair of rows u > v whose 4-bit values have a cosine >= min_cosine, ordered by (u, v): int32 tensors (u, v).  The
         n x n matrix is never stored.  Rows of zeros, with a NaN, or of a length outside [2^-60, 2^60] have no pairs.  One synchronisation, for the number of pairs; a second pass when there are more than eight
-        per row.  More than max_pairs raise MddError."""
+        per row.  More than max_pairs raise TooManyPairs, an MddError."""
         mc, ms = self._packed(m, "m")
         _need(max_pairs >= 0, "max_pairs is negative")
         cnt = torch.empty(1, dtype=torch.int64, device=self.device)
@@ -299,7 +308,7 @@ class VectorOps:
                        "mdd_mx_pairs")
             n = int(cnt.item())
             if n > max_pairs:
-                _refuse(f"{n} pairs reach {min_cosine}: more than max_pairs={max_pairs}")
+                raise TooManyPairs(n, max_pairs, min_cosine)
             if n <= cap:
                 break
             cap = n

@@ -9,6 +9,7 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from map_neo_amd import dedup as D  # noqa: E402
+from map_neo_amd.vectors import TooManyPairs  # noqa: E402
 from test_vectors_path import VectorBackend  # noqa: E402
 
 
@@ -135,3 +136,137 @@ def test_four_bits_are_the_operators():
     x[8, 50], x[9, 7] = float("inf"), float("nan")
     assert 0.05 <= D.screen_margin(x, 0.9) < 0.3
     assert D.screen_margin(torch.zeros(5, 8), 0.9) == D.screen_margin(x[:1], 0.9) == D.SCREEN_MARGIN
+
+
+# ------------------------------------------------------------------------------------------------ more pairs or rows than a search takes
+def _limited(backend, monkeypatch, pairs=None, rows=None):
+    """the backend with a search that returns at most `pairs` pairs; ranges of at most `rows` rows"""
+    if rows is not None:
+        monkeypatch.setattr(D, "MAX_PAIR_ROWS", rows)
+    calls, search = [], backend.mx_pairs
+
+    def limited(m, t):
+        calls.append(m)
+        if isinstance(backend, VectorBackend):
+            u, v = search(m, t)
+            if pairs is not None and u.numel() > pairs:
+                raise TooManyPairs(u.numel(), pairs, t)
+            return u, v
+        return search(m, t) if pairs is None else search(m, t, max_pairs=pairs)
+
+    monkeypatch.setattr(backend, "mx_pairs", limited, raising=False)
+    return calls
+
+
+def _groups(n, dim, groups, noise, g):
+    """random rows; the rows of each group are one vector, but for noise"""
+    x = torch.randn(n, dim, generator=g)
+    for rows in groups:
+        x[rows] = x[rows[0]] + noise * torch.randn(len(rows), dim, generator=g)
+    return x
+
+
+@pytest.mark.parametrize("rows,pairs", [(64, None), (33, None), (None, 40), (50, 40), (2, None), (3, 1)])
+def test_edges_do_not_depend_on_the_search(backend, monkeypatch, rows, pairs):
+    """in ranges of few rows, and of few pairs: the same edges in the same order"""
+    g = torch.Generator().manual_seed(8)
+    n = 21 if rows in (2, 3) else 150
+    p = torch.randperm(n, generator=g).tolist()
+    x = _groups(n, 256, [p[:n // 10], p[n // 5: n // 5 + 2], p[n // 2: n // 2 + 7]], 0.05, g)
+    x[p[0]] = 0
+    want = _pairs(backend, x, 0.95)
+    assert len(want) > 20 and want == sorted(want)
+    calls = _limited(backend, monkeypatch, pairs, rows)
+    assert _pairs(backend, x, 0.95) == want and len(calls) > 3
+    with pytest.raises(TooManyPairs, match="max_pairs=20"):
+        D.vector_edges(backend, x.to(backend.device), 0.95, max_pairs=20)
+
+
+@pytest.mark.parametrize("rows,pairs", [(None, 500), (100, None), (None, 50), (1000, 10 ** 9)])
+def test_clusters_of_many_alike_vectors(backend, monkeypatch, rows, pairs):
+    """200 equal rows (19900 pairs), 60 nearly equal ones, a row near to the equal ones; rows of zeros and of NaN, which are as
+    equal as can be and pair with nothing; a shingle duplicate"""
+    g = torch.Generator().manual_seed(9)
+    n = 400
+    p = torch.randperm(n, generator=g).tolist()
+    same, alike, zero, nan = sorted(p[:200]), sorted(p[200:260]), p[260:280], p[280:300]
+    x = _groups(n, 128, [same], 0.0, g)
+    x[alike] = x[alike[0]] + 0.02 * torch.randn(60, 128, generator=g)
+    x[p[300]] = x[same[0]] + 0.02 * torch.randn(128, generator=g)
+    x[zero], x[nan] = 0, float("nan")
+    sig = np.random.default_rng(0).integers(0, 2 ** 32, (n, 128), dtype=np.uint64).astype(np.uint32)
+    sig[p[302]] = sig[p[301]]
+    want = np.arange(n)
+    for c in (same + [p[300]], alike, [p[301], p[302]]):
+        want[c] = min(c)
+    calls = _limited(backend, monkeypatch, pairs, rows)
+    out = D.cluster_local(backend, backend.to_device(sig), vectors=x.to(backend.device), min_cosine=0.95)
+    assert (out["labels"].cpu().numpy() == want).all() and (len(calls) == 1) == (pairs == 10 ** 9)
+    assert out["removed"].cpu().numpy().astype(bool).tolist() == (want != np.arange(n)).tolist()
+    # the edges that come back join the same components
+    labels = backend.components_init(n)
+    backend.components_union(labels, out["edge_u"], out["edge_v"])
+    backend.components_finish(labels)
+    assert (labels.cpu().numpy() == want).all()
+    if len(calls) > 1:
+        assert out["edge_u"].numel() == (want != np.arange(n)).sum()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_first_equal_row(dtype):
+    x = torch.randn(9, 40, generator=torch.Generator().manual_seed(1)).to(dtype)
+    x[4], x[8], x[5] = x[2], x[2], x[3]
+    x[6:8] = 0
+    x[5, 39] += 1                                                # all but equal
+    assert D._first_equal(x).tolist() == [0, 1, 2, 3, 2, 5, 6, 7, 2]
+    assert D._first_equal(x[:, ::2].contiguous()[:, 1:]).tolist() == [0, 1, 2, 3, 2, 3, 6, 7, 2]
+    assert D._first_equal(x[:0]).tolist() == []
+
+
+def test_token_ids_in_several_lookups(monkeypatch, tmp_path):
+    """more ids than one lookup takes: whole rows at a time, empty ones among them; a row that alone is too long is refused"""
+    from map_neo_amd.cli import dedup as stage
+    rng = np.random.default_rng(3)
+    table, lens = rng.standard_normal((50, 12)).astype(np.float32), [3, 0, 7, 9, 0, 0, 1, 4, 9, 0]
+    ids = rng.integers(0, 50, sum(lens) + 5).astype(np.int32)
+    offs = np.concatenate([[2], 2 + np.cumsum(lens)]).astype(np.int64)
+    for name, a in (("t", table), ("i", ids), ("o", offs)):
+        np.save(tmp_path / (name + ".npy"), a)
+    args = stage.build_parser().parse_args(["--input_dir", "x", "--output_dir", "y", "--min_cosine", "0.9", "--embedding_table", str(tmp_path / "t.npy"),
+                                            "--token_ids", str(tmp_path / "i.npy"), "--token_offsets", str(tmp_path / "o.npy")])
+    rows = np.array([0, 1, 3, 7, 8, 9])
+    want = stage.document_vectors(VectorBackend(), args, rows, 10)
+    assert want.shape == (6, 12) and (want[1] == 0).all() and (want[2] != 0).any()
+    for limit in (9, 10, 12, 33):
+        monkeypatch.setattr(stage, "MAX_IDS", limit)
+        assert torch.equal(stage.document_vectors(VectorBackend(), args, rows, 10), want)
+    monkeypatch.setattr(stage, "MAX_IDS", 8)
+    with pytest.raises(SystemExit, match="row 3 has 9 token ids"):
+        stage.document_vectors(VectorBackend(), args, rows, 10)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_search_takes(engine):
+    """2^22 + 5000 documents: pairs within the first half, within the second and across, and 30000 equal rows (4.5 * 10^8 pairs)"""
+    n, dim = (1 << 22) + 5000, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(n, dim, device="cuda", generator=g)
+    p = torch.randperm(n, device="cuda", generator=g)[:40000]
+    a, b = p[:4000], p[4000: 8000]
+    x[b] = x[a] + 0.05 * torch.randn(4000, dim, device="cuda", generator=g)
+    x[p[8000: 38000]] = x[p[8000]].clone()
+    labels = engine.components_init(n)
+    D._join_near(engine, labels, x.half(), 0.97)
+    engine.components_finish(labels)
+    want = torch.arange(n, device="cuda")
+    want[torch.maximum(a, b)] = torch.minimum(a, b)
+    want[p[8000: 38000]] = p[8000: 38000].min()
+    assert torch.equal(labels.long(), want)
+
+
+@pytest.mark.gpu
+def test_too_many_pairs_says_how_many(engine):
+    m = engine.mx_quantize(torch.ones(300, 40).cuda())
+    with pytest.raises(TooManyPairs, match="44850 pairs reach 0.5: more than max_pairs=1000") as e:
+        engine.mx_pairs(m, 0.5, max_pairs=1000)
+    assert (e.value.count, e.value.limit) == (44850, 1000)
