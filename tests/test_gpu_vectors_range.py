@@ -1,0 +1,76 @@
+"""GPU suite: the document-vector operators at the ends of the 32-bit range.  Bounds as in test_gpu_vectors.py."""
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import vec_ref as R  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+def _close(got, want, tol, what=""):
+    got = got.double().cpu()
+    off = (got - want).abs()
+    worst = (off - tol).max().item()
+    assert got.shape == want.shape and worst <= 0, f"{what}: off by {off.max().item():.3g}, {worst:.3g} beyond the bound"
+
+
+# sizes of rows: with eps = 0 the squares of all but those near 1 leave the 32-bit numbers or their normal range
+SIZES = [1.0, 1e-17, 1e-19, 1e-21, 1.0, 1e-25, 1e-30, 3e-38, 2e-42, 1e18, 1e19, 1e25, 3e37, 1.0]
+
+
+def _rows(dim, dtype, g):
+    x = torch.randn(len(SIZES), dim, generator=g, dtype=torch.float64) * torch.tensor(SIZES, dtype=torch.float64)[:, None]
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-35, 1e-6])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [1, 5, 100, 129, 384, 500, 768, 1000, 1300, 2048, 3001, 5000, 10001, 20000])
+def test_norms_of_very_small_and_large_rows(engine, dim, dtype, eps):
+    g = torch.Generator().manual_seed(dim)
+    x, res = _rows(dim, dtype, g), _rows(dim, dtype, g)
+    w, gy = torch.randn(dim, generator=g).to(dtype), torch.randn(len(SIZES), dim, generator=g).to(dtype)
+    e = float(np.float32(eps))
+    for residual, weight in ((None, None), (res, w)):
+        c = lambda t: None if t is None else t.cuda()
+        h = x.float() if residual is None else x.float() + residual.float()      # h is a 32-bit number
+        wy, _, wr = R.rms_norm(h, weight, None, e)
+        live = h.abs().amax(1) > 0                                # (a row may round to zeros, whose r without eps is infinite)
+        y, total, rstd = engine.rms_norm(x.cuda(), c(weight), c(residual), eps=eps)
+        rel = (dim + 12) * R.U32
+        fits = live & (wr < 2.0 ** 127)
+        _close(rstd[fits], wr[fits], rel * wr[fits] + 2.0 ** -149, "rstd")
+        assert torch.isinf(rstd.cpu()[live & (wr > 2.0 ** 129)]).all()
+        _close(y[live], wy[live], (R.half(dtype, wy.abs()) + 1.01 * rel * wy.abs())[live], "y")
+        codes, scales, _ = engine.rms_norm_q8(x.cuda(), c(weight), c(residual), eps=eps)
+        q, s = R.q8(x, weight, residual, e, "int8")
+        assert torch.equal(codes.float().double().cpu(), q)
+        _close(scales[live], s[live], (dim + 16) * R.U32 * s[live].abs() + 2.0 ** -149, "scales")
+        # backward, from what the forward pass stored, where a gradient of about r is a number of the type
+        ok = [k for k in range(len(SIZES)) if fits[k] and wr[k] < 1e34 and wr[k] > 1e-37]
+        r, hh = rstd.double().cpu()[ok][:, None], total.double().cpu()[ok]
+        dx, dw = engine.rms_norm_backward(gy.cuda()[ok], total[ok], rstd[ok], c(weight))
+        nx, gw = hh * r, gy.double()[ok] * (1 if weight is None else weight.double())
+        want = r * (gw - nx * (gw * nx).mean(1, keepdim=True))
+        bound = R.half(dtype, want.abs()) + 1.01 * R.U32 * (8 * (r * gw).abs() + (dim + 12) * (r * nx).abs() * (gw * nx).abs().mean(1, keepdim=True))
+        _close(dx, want, bound, "dx")
+
+
+def test_norms_of_zeros_infinities_and_nan(engine):
+    """what they gave before: a row of zeros y = 0 * inf without eps and 0 with it; an infinity or a NaN reaches its row and no other"""
+    x = torch.randn(6, 200, generator=torch.Generator().manual_seed(1)) * 1e-25
+    x[1] = 0
+    x[2, 150], x[3, 7] = float("nan"), float("inf")
+    y, _, rstd = engine.rms_norm(x.cuda(), eps=0.0)
+    assert torch.isnan(y[1]).all() and torch.isinf(rstd[1]) and torch.isnan(y[2]).all() and torch.isnan(rstd[2])
+    assert rstd[3] == 0 and torch.isnan(y[3, 7]) and (y[3, :7] == 0).all()
+    ok = [0, 4, 5]
+    _close(y[ok], R.rms_norm(x, None, None, 0.0)[0][ok], 220 * R.U32 * R.rms_norm(x, None, None, 0.0)[0][ok].abs())
+    assert (engine.rms_norm(x[1:2].cuda())[0] == 0).all()
+    codes, scales, _ = engine.rms_norm_q8(x.cuda(), eps=0.0)
+    assert scales[1] == 0 and torch.isnan(scales[2:4]).all() and (codes[1:4] == 0).all()
