@@ -531,7 +531,8 @@ int mdd_sort_edges(mdd_ctx* ctx, uint32_t* edge_u, uint32_t* edge_v, uint64_t n_
  *   matmul   c [m, n] (MDD_F32 or MDD_BF16, c_stride) = alpha * A * B^T,  A [m, dim], B [n, dim] packed
  *   pairs    every u > v with cos(A_u, A_v) >= min_cosine (0 < min_cosine <= 1; cosine of the 4-bit values), appended to edge_u /
  *            edge_v in no fixed order, at most edge_cap of them; *n_edges (device u64, set by the call) counts all of them.
- *            The comparison is one of 32-bit numbers: a pair within 2^-20 of min_cosine may fall on either side.
+ *            Sums are held in 32 bits: a pair within (dim / 16 + 16) * 2^-24 of min_cosine may fall on either side.  Equal rows reach
+ *            every threshold up to 1 - 2^-20, whatever dim.
  *            Rows of zeros, with a NaN, or of a length outside [2^-60, 2^60] have no pairs.  Rows of similar length are fastest.  m <= MDD_MX_MAX_PAIR_ROWS
  *            (2^22: 10^13 pairs; larger sets in ranges of rows, two at a time side by side). */
 #define MDD_MX_MAX_PAIR_ROWS 4194304

@@ -477,45 +477,37 @@ __global__ __launch_bounds__(B::WAVES * 64) void mx_matmul_kernel(const Packed a
 }
 
 // ------------------------------------------------------------------------------------------------ near pairs
-// Length of every row of 4-bit values, and the least of every row tile.  The magnitudes (doubled: 0 1 2 3 4 6 8 12) are looked
-// up four at a time with a byte permute and squared with a byte dot product: a block of 32 columns is summed in whole
-// numbers.  A row of zeros, one with a NaN and one of a length outside [2^-60, 2^60], where the product of two lengths could
-// leave the 32-bit numbers, gets an infinite length, which no product reaches.
-__global__ __launch_bounds__(128) void mx_length_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t col_tiles,
+// Length of every row of 4-bit values, and the least of every row tile: the root of the row's product with itself, summed by the
+// same instructions in the same order as the products that it is compared with, so that equal rows have a cosine of 1 up to three
+// roundings whatever their width.  (A sum in another order is off by up to 2^-15 of it at 32768 columns whose blocks differ much.)
+// A wave multiplies a row tile by itself and keeps the diagonal, which of a row r is in lane r or r + 32.  A row of zeros, one
+// with a NaN and one of a length outside [2^-60, 2^60], where the product of two lengths could leave the 32-bit numbers, gets
+// an infinite length, which no product reaches.
+__global__ __launch_bounds__(256) void mx_length_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t col_tiles,
                                                         uint64_t row_tiles, float* __restrict__ length, float* __restrict__ least,
                                                         unsigned long long* n_edges) {
-    __shared__ float lds[4][32];
-    const uint32_t kb = threadIdx.x / 32, r = threadIdx.x % 32;
+    const uint32_t lane = lane_id(), r = lane % 32;
     if (blockIdx.x == 0 && threadIdx.x == 0) *n_edges = 0;
-    for (uint64_t rt = blockIdx.x; rt < row_tiles; rt += gridDim.x) {
-        float s = 0;
+    for (uint64_t rt = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; rt < row_tiles; rt += (uint64_t)gridDim.x * 4) {
+        const uint8_t *p = codes + rt * col_tiles * TILE + lane * 16, *q = scales + rt * col_tiles * STILE + lane * 2;
+        f32x16 acc = 0.0f;
 #pragma unroll 4
         for (uint32_t ct = 0; ct < col_tiles; ct++) {
-            const uint64_t tile = rt * col_tiles + ct;
-            const u32x4 p = *reinterpret_cast<const u32x4*>(codes + tile * TILE + kb * 512 + r * 16);
-            const int e = (int)scales[tile * STILE + (kb & 1) * 64 + r * 2 + (kb >> 1)];
-            int sq = 0;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint32_t lo = __builtin_amdgcn_perm(0x0C080604u, 0x03020100u, p[k] & 0x07070707u);
-                const uint32_t hi = __builtin_amdgcn_perm(0x0C080604u, 0x03020100u, p[k] >> 4 & 0x07070707u);
-                sq = __builtin_amdgcn_sdot4((int)lo, (int)lo, sq, false);
-                sq = __builtin_amdgcn_sdot4((int)hi, (int)hi, sq, false);
-            }
-            s += e == 255 ? __builtin_nanf("") : ldexpf((float)sq, 2 * (e - 127) - 2);
+            const i32x4 a0 = *reinterpret_cast<const i32x4*>(p + (uint64_t)ct * TILE), a1 = *reinterpret_cast<const i32x4*>(p + (uint64_t)ct * TILE + 1024);
+            const int sc = *reinterpret_cast<const uint16_t*>(q + (uint64_t)ct * STILE);
+            acc = mma(a0, sc, a0, sc, acc, 0);
+            acc = mma(a1, sc, a1, sc, acc, 1);
         }
-        lds[kb][r] = s;
-        __syncthreads();
-        if (kb == 0) {
-            s = lds[0][r] + lds[1][r] + lds[2][r] + lds[3][r];
-            s = s >= 0x1p-120f && s <= 0x1p120f ? sqrtf(s) : __builtin_inff();
-            length[rt * 32 + r] = s;
-            float low = s;
+        float s = 0;
 #pragma unroll
-            for (int d = 16; d; d >>= 1) low = fminf(low, __shfl_xor(low, d, 64));
-            if (r == 0) least[rt] = low;
-        }
-        __syncthreads();
+        for (uint32_t i = 0; i < 16; i++) s = i / 4 * 8 + lane / 32 * 4 + i % 4 == r ? acc[i] : s;
+        const float other = __shfl_xor(s, 32, 64);
+        s = r / 4 % 2 == lane / 32 ? s : other;
+        s = s >= 0x1p-120f && s <= 0x1p120f ? sqrtf(s) : __builtin_inff();
+        if (lane < 32) length[rt * 32 + lane] = s;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) s = fminf(s, __shfl_xor(s, d, 64));
+        if (lane == 0) least[rt] = s;
     }
 }
 
@@ -700,7 +692,8 @@ int mdd_mx_pairs(mdd_ctx* ctx, const uint8_t* codes, const uint8_t* scales, uint
     const uint32_t ct = (dim + 127) / 128;
     auto* count = reinterpret_cast<unsigned long long*>(n_edges);
     float *length = (float*)ws, *least = length + round_up(m, 64);
-    hipLaunchKernelGGL(mx_length_kernel, dim3((unsigned)(rt < 1 ? 1 : rt < (1u << 20) ? rt : (1u << 20))), dim3(128), 0, ctx->stream, codes, scales, ct, rt,
+    const uint64_t blocks = (rt + 3) / 4;
+    hipLaunchKernelGGL(mx_length_kernel, dim3((unsigned)(blocks < 1 ? 1 : blocks)), dim3(256), 0, ctx->stream, codes, scales, ct, rt,
                        length, least, count);
     if (m) {
         const uint64_t cus = (uint64_t)ctx->cus, bands = (rt + 8 * Tiles::TA - 1) / (8 * Tiles::TA), places = 32 * bands * (bands + 1);

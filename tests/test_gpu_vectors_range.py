@@ -74,3 +74,40 @@ def test_norms_of_zeros_infinities_and_nan(engine):
     assert (engine.rms_norm(x[1:2].cuda())[0] == 0).all()
     codes, scales, _ = engine.rms_norm_q8(x.cuda(), eps=0.0)
     assert scales[1] == 0 and torch.isnan(scales[2:4]).all() and (codes[1:4] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ pairs next to the threshold
+@pytest.mark.parametrize("dim", [96, 4096, 8192, 32768])
+@pytest.mark.parametrize("n", [2, 33, 300])
+def test_equal_rows_of_any_width(engine, n, dim):
+    """one large block and many small ones: sums of squares depend on their order, and equal rows have to be near at 1 - 2^-20 anyhow"""
+    x = torch.zeros(1, dim)
+    x[0, 0] = 4096
+    x[0, 32::32], x[0, 33::32] = 0.5, 0.5
+    eu, ev = engine.mx_pairs(engine.mx_quantize(x.expand(n, -1).contiguous().cuda()), 1 - 2.0 ** -20)
+    wu, wv = np.nonzero(np.tril(np.ones((n, n)), -1))
+    assert eu.tolist() == wu.tolist() and ev.tolist() == wv.tolist()           # (arrays of 0 and 1 entries would compare as equal)
+
+
+@pytest.mark.parametrize("dim", [128, 2048, 32768])
+def test_products_and_lengths_within_the_bound(engine, dim):
+    """rows whose sums lose the most: a block of 2^12 and small ones of one sign behind it.  The cosine by which a pair is chosen, from the
+    same sums, against 64 bits: within (dim / 16 + 16) * 2^-24, as mdd.h says"""
+    g = torch.Generator().manual_seed(dim)
+    x = torch.rand(64, dim, generator=g) * 0.7 + 0.1
+    x[:, 0] = torch.randint(2 ** 10, 2 ** 13, (64,), generator=g).float()
+    x[::2, 32:] *= torch.exp2(torch.randint(0, 3, (32, (dim - 32) // 32), generator=g).float()).repeat_interleave(32, 1)
+    m = engine.mx_quantize(x.cuda())
+    v = torch.from_numpy(R.mx_values(*R.mx_unpack(m.codes, m.scales, 64, dim))[:64, :dim])
+    ln = v.norm(dim=1)
+    want = (v @ v.T) / ln[:, None] / ln[None]
+    c = engine.mx_matmul(m, m).double().cpu()
+    got = c / c.diagonal().sqrt()[:, None] / c.diagonal().sqrt()[None]
+    bound = (dim / 16 + 16) * 2.0 ** -24
+    assert ((got - want).abs() <= bound).all()
+    for t in (0.3, 0.6, 0.9, 0.99, 0.9999):
+        eu, ev = engine.mx_pairs(m, t)
+        found = torch.zeros(64, 64, dtype=torch.bool)
+        found[eu.cpu().long(), ev.cpu().long()] = True
+        low = torch.ones(64, 64, dtype=torch.bool).tril(-1)
+        assert found[low & (want > t + bound)].all() and not found[want < t - bound].any()
