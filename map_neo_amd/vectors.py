@@ -5,7 +5,8 @@ A document as a row of numbers instead of a set of shingles: ids are looked up i
 bits (`mx_quantize`), compared with an index (`mx_matmul`) or among themselves (`mx_pairs`), and candidate pairs are checked on the
 8-bit rows (`edge_cosines`).  An extension: the reference compares documents by their shingles only.  torch owns the memory;
 every computation is a kernel of libmdd_hip.so on the engine's stream.  A call made under another current stream is ordered
-with it on both sides.  Matrices may be row-strided views (unit stride inside a row).  Wrong arguments raise lib.MddError.
+with it on both sides.  Matrices may be row-strided views (unit stride inside a row).  Wrong arguments raise lib.MddError.  No
+autograd node is made: the gradients have methods of their own, and a tensor that requires one is refused outside torch.no_grad().
 """
 from __future__ import annotations
 
@@ -82,6 +83,12 @@ def _refuse(what):
     raise _lib.MddError(what)
 
 
+def _no_node(name):
+    """a result without a node would cut the tensor's gradient off without a word"""
+    if torch.is_grad_enabled():
+        _refuse(f"{name} requires a gradient, and no autograd node is made: call under torch.no_grad() or pass {name}.detach(), and the *_backward method yourself")
+
+
 class VectorOps:
     """mixed into minhash.Engine"""
 
@@ -95,6 +102,8 @@ class VectorOps:
             _refuse(f"{name} must be a matrix, not {t.dim()}-dimensional")
         if t.dtype not in _TYPE if dtype is None else t.dtype != dtype:
             _refuse(f"{name} has type {t.dtype}" + (f", not {dtype}" if dtype else ""))
+        if t.requires_grad:
+            _no_node(name)
         n, d = t.shape
         if not 1 <= d <= MAX_DIM:
             _refuse(f"{name} has {d} columns: 1 to {MAX_DIM} are supported")
@@ -114,6 +123,8 @@ class VectorOps:
             _refuse(f"{name} must be a contiguous vector")
         if t.dtype not in dtypes:
             _refuse(f"{name} has type {t.dtype}")
+        if t.requires_grad:
+            _no_node(name)
         n = t.numel()
         if size is not None and n != size:
             _refuse(f"{name} has {n} entries, not {size}")
