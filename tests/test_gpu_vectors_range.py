@@ -111,3 +111,49 @@ def test_products_and_lengths_within_the_bound(engine, dim):
         found[eu.cpu().long(), ev.cpu().long()] = True
         low = torch.ones(64, 64, dtype=torch.bool).tril(-1)
         assert found[low & (want > t + bound)].all() and not found[want < t - bound].any()
+
+
+# ------------------------------------------------------------------------------------------------ subnormal numbers in sums
+@pytest.mark.parametrize("dtype,least", [(torch.bfloat16, -133), (torch.float16, -24), (torch.float32, -149)])
+@pytest.mark.parametrize("dim,lens", [(8, [1, 2, 3, 16, 0, 65]), (256, [7, 64, 100, 3000]), (520, [9, 40, 128])])
+def test_sums_of_subnormal_rows(engine, dim, lens, dtype, least):
+    """rows of a few of the type's smallest steps, alone and beside the smallest normal numbers: lookups, sums and gradients keep them"""
+    g = torch.Generator().manual_seed(dim)
+    step = 2.0 ** least
+    table = (torch.randint(-7, 8, (40, dim), generator=g).double() * step).to(dtype)
+    table[30:] = (torch.randn(10, dim, generator=g).double() * step * 2 ** 10).to(dtype)
+    assert (table.double() % step == 0).all() and (table[:30] != 0).any()
+    ids = torch.randint(0, 40, (sum(lens),), generator=g, dtype=torch.int32)
+    ids[: lens[0] + lens[1]] %= 30                               # documents of such rows only
+    offs = torch.tensor([0] + lens).cumsum(0)
+    assert torch.equal(engine.embed(table.cuda(), ids.cuda()).cpu(), table[ids.long()])
+    for mode in ("sum", "mean"):
+        want, mag, cnt = R.embed(table, ids, offs, 1.0, mode)
+        got = engine.embed(table.cuda(), ids.cuda(), offs.cuda(), mode=mode)
+        # sums in 32 bits of whole steps of 2^-149 and above; a mean is rounded once more there
+        _close(got, want, R.half(dtype, want.abs()) + (cnt[:, None].double() + 4) * R.U32 * mag + 2.0 ** -149, mode)
+        assert (got[0] != 0).any()
+    grad = table[torch.randint(0, 40, (len(lens),), generator=g)]
+    want, mag, cnt = R.embed_backward(grad, ids, 40, offs, 1.0, "sum")
+    _close(engine.embed_backward(grad.cuda(), ids.cuda(), 40, offs.cuda(), mode="sum"), want, (cnt + 4) * R.U32 * mag, "gradient")
+    rows = table[torch.randint(0, 40, (sum(lens),), generator=g)]
+    want, mag, cnt = R.embed_backward(rows, ids, 40, None, 1.0, "sum")
+    for out in {torch.float32, dtype}:
+        _close(engine.embed_backward(rows.cuda(), ids.cuda(), 40, dtype=out), want, R.half(out, want.abs()) + (cnt + 4) * R.U32 * mag, "gradient of rows")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_sums_with_infinities_and_large_numbers(engine, dtype):
+    """infinities and NaN by column, as in 64 bits; the largest finite numbers of either sign beside each other"""
+    big = torch.finfo(dtype).max
+    table = torch.zeros(6, 16, dtype=dtype)
+    table[0, 0], table[1, 0], table[2, 1], table[3, 1], table[4, 2] = float("inf"), -float("inf"), float("inf"), 3.0, float("nan")
+    table[0, 3], table[1, 3], table[0, 4], table[1, 4], table[5] = big, -big, big, 0, 1
+    ids = torch.arange(6, device="cuda")
+    for n in (2, 4, 6):
+        got = engine.embed(table.cuda(), ids[:n], torch.tensor([0, n], device="cuda"), mode="sum").double().cpu()
+        want = table[:n].double().sum(0, keepdim=True)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~want.isnan()].isinf(), want[~want.isnan()].isinf())
+        fin = want.isfinite()
+        # the result is rounded to the type: 65504 + 1 lies between 65504 and 65536, the next in float16, and is off by 1 <= half a step, 16
+        assert ((got - want)[fin].abs() <= 2.0 ** -24 * 6 * big + R.half(dtype, want[fin].abs())).all() and (got[:, 5:] == want[:, 5:]).all()
