@@ -495,9 +495,12 @@ int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_s
  *   own.  rstd is a 32-bit number itself, infinite where mean(h^2) + eps is below 2^-256)
  *   norm      y = h * r * weight;  sum_out (may be NULL) = h, rounded to the type;  rstd (may be NULL) = r, float per row
  *   norm_q8   the same with y in 8 bits (kind MDD_I8 or MDD_E4M3): with top = 127 or 448 and big = the row's largest
- *             |h * weight|, code = the nearest 8-bit value to h * weight * top / big, ties to even, decided as in exact
- *             arithmetic, and scale[row] = big * r / top, so that code * scale is y.  A row of zeros gets zeros with scale 0;
- *             a row with a NaN or an infinity gets zeros with scale NaN.
+ *             |h * weight|, code = the nearest 8-bit value to h * weight * top / big, ties to even, decided without a rounding
+ *             of the quotient, and scale[row] = big * r / top, so that code * scale is y; the scale is off by at most
+ *             (dim + 16) * 2^-24 of itself.  h * weight itself is held in 64 bits: exact without a residual and for MDD_F16, and
+ *             with one unless the two numbers added differ in size by more than 2^37 (MDD_BF16), or 2^29 (MDD_F32; with a weight,
+ *             2^5): then rounded to 53 bits.  A row of zeros gets zeros with scale 0; a row with a NaN or an infinity gets zeros
+ *             with scale NaN.
  *   backward  h as stored by norm (sum_out, or x), rstd as stored, g = gradient of y, grad_sum (may be NULL) = gradient
  *             that reaches sum_out by other ways:  x_grad = r * (g*w - h*r * mean(g*w*h*r)) + grad_sum -- the gradient of x
  *             and of residual alike;  weight_grad (float [dim], may be NULL) = sum over rows of g * h * r. */

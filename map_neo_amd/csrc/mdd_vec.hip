@@ -875,7 +875,7 @@ __global__ __launch_bounds__(L == 1024 ? 1024 : 256, L == 1024 ? 4 : NC == 4 ? 3
     const uint32_t t = threadIdx.x % L;
     const double top = KIND == MDD_I8 ? 127.0 : 448.0;
     for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / L; row < n; row += (uint64_t)gridDim.x * RPB) {
-        double y[NC][8];  // h * weight: a sum and a product of 8 to 24-bit numbers, nearly always exact in 64 bits
+        double y[NC][8];  // h * weight: a sum and a product of 8 to 24-bit numbers, exact in 64 bits unless the two of the sum lie far apart
         f32x8 v[NC], o[NC], w[NC];
 #pragma unroll
         for (int c = 0; c < NC; c++) v[c] = Eight<NARROW>(c * L + t, dim).template load<T, ONCE>(x + row * xs, dim), o[c] = 0.0f, w[c] = 1.0f;

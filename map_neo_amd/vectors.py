@@ -207,7 +207,8 @@ class VectorOps:
     def rms_norm_q8(self, x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
                     kind: str = "int8"):
         """rms_norm with y in 8 bits and a float32 scale per row (y = codes * scale): kind "int8" or "e4m3".  Returns (codes,
-        scales, h, or None without a residual).  Codes are those of exact arithmetic."""
+        scales, h, or None without a residual).  Codes are the nearest ones to h * weight, held in 64 bits, over the row's
+        largest: decided without a rounding of that quotient."""
         if kind not in _Q8:
             _refuse(f"kind {kind!r} is neither 'int8' nor 'e4m3'")
         xp, xs, rp, rs, wp, n, dim = self._norm_args(x, weight, residual)

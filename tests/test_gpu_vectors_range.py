@@ -157,3 +157,23 @@ def test_sums_with_infinities_and_large_numbers(engine, dtype):
         fin = want.isfinite()
         # the result is rounded to the type: 65504 + 1 lies between 65504 and 65536, the next in float16, and is off by 1 <= half a step, 16
         assert ((got - want)[fin].abs() <= 2.0 ** -24 * 6 * big + R.half(dtype, want[fin].abs())).all() and (got[:, 5:] == want[:, 5:]).all()
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit codes next to a midpoint
+@pytest.mark.parametrize("kind,top", [("int8", 127), ("e4m3", 448)])
+@pytest.mark.parametrize("dtype,gap,lost", [(torch.bfloat16, -36, -60), (torch.float16, -24, None), (torch.float32, -28, -60)])
+def test_codes_of_sums_of_numbers_far_apart(engine, dtype, gap, lost, kind, top):
+    """a residual that lifts or lowers a midpoint by 2^gap decides it; one below the 64 bits that h is held in does not (the tie
+    goes to the even code), as mdd.h says"""
+    mids = [2.5, 3.5, -2.5, -7.5, 0.5] if kind == "int8" else [17.0, 19.0, -17.0, -23.0, 17.0]
+    up = [3, 4, -3, -8, 1] if kind == "int8" else [18, 20, -18, -24, 18]
+    down = [2, 3, -2, -7, 0] if kind == "int8" else [16, 18, -16, -22, 16]
+    even = [2, 4, -2, -8, 0] if kind == "int8" else [16, 20, -16, -24, 16]
+    x = torch.tensor([[top] + mids]).to(dtype).cuda()
+    sign = torch.tensor([[0] + mids]).sign()
+    for power, want in ((gap, up), (gap, down), (lost, even)):
+        if power is None:
+            continue
+        res = (sign * 2.0 ** power * (-1 if want is down else 1)).to(dtype)
+        codes, _, _ = engine.rms_norm_q8(x, None, res.cuda(), kind=kind)
+        assert codes.float().cpu().tolist() == [[top] + want]
