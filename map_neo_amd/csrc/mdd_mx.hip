@@ -203,9 +203,12 @@ __global__ __launch_bounds__(256) void mx_skinny_kernel(const uint8_t* __restric
 //     wait for step s + 1, barrier
 //     multiply half 1 of step s, and between them: read half 0 of step s + 1, request step s + 3 into the buffer of step s
 // so a load has two steps to arrive, a step needs one barrier, and neither LDS nor memory latency nor the issue of loads stands
-// before the matrix unit.  8192 x 16384 x 8192: 4.2 PFLOP/s on random numbers, 5.5 on zeros -- the card lowers its clock to 1.6 to
-// 1.9 GHz under this load, so that more products per cycle no longer mean more per second.  (Four waves of 128 x 128, which
-// read a third less from LDS, do the same 4.1 but have nothing to overlap a tile's end with: 2048 columns 186 us against 147.)
+// before the matrix unit.  8192 x 16384 x 8192: 4.2 PFLOP/s on random numbers, 5.5 on zeros, of 10 that the units could do at 2.4 GHz.
+// Two things keep it there.  The units are busy 46 % of the cycles (8192 x 32768 x 2048; 44 % among pairs), on zeros as well: a step
+// multiplies for 1024 cycles and takes 96 KB of fragments and 34 KB of arriving tiles through an LDS of 128 bytes a cycle, 1040
+// cycles, and the two do not overlap fully.  And the card lowers its clock with what switches: 1.8 GHz on random numbers, 2.26 on zeros.
+// (Four waves of 128 x 128, which read a third less from LDS, do the same 4.1 but have nothing to overlap a tile's end with: 2048
+// columns 186 us against 147.)
 template <int WR_, int WC_, int FM_, int FN_>
 struct Block {
     static constexpr int WR = WR_, WC = WC_, FM = FM_, FN = FN_;
@@ -535,7 +538,7 @@ __global__ __launch_bounds__(B::WAVES * 64) void mx_pairs_kernel(const Packed a,
         }
     };
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave / B::WC, wc = wave % B::WC, last = a.tiles - 1;
-    float li[B::FM], lj[B::FN];  // least lengths of the wave's row tiles: scalar loads, on their way during the steps
+    float li[B::FM], lj[B::FN];  // least lengths of the wave's row tiles: scalar loads, for which the tile's first step waits
     auto begin = [&](const Place& t) {
         const uint32_t it = t.i0 + wr * B::FM, jt = t.j0 + wc * B::FN;
 #pragma unroll

@@ -500,9 +500,9 @@ __device__ __forceinline__ void grad_key(const GradIds& g, uint64_t p, uint32_t&
 }
 
 // Up to SMALL_SORT pairs in one block and one launch, all passes in LDS: 450 edges 10 us, 6750 30 (four passes each). Counting
-// for each edge on all CUs how many are before it takes 16 for 6750, but a workspace and a launch more: 8 us less of 474 a
-// search for near pairs, and 3 more of 54 for the small one. val_bits > 0: by the value's bits first, then by the key's. MAKE:
-// the pairs are the gradient's, made on the way in
+// for each edge on all CUs how many are before it takes 16 for 6750, but a workspace and a launch more, which cost the few edges of
+// a small search 3 us; a choice by the number of edges is not made yet. val_bits > 0: by the value's bits first, then by the
+// key's. MAKE: the pairs are the gradient's, made on the way in
 template <bool MAKE>
 __global__ __launch_bounds__(1024) void small_sort_kernel(uint32_t* __restrict__ key, uint32_t* __restrict__ val, uint32_t n, int val_bits, int bits, GradIds g) {
     __shared__ uint32_t ks[SMALL_SORT], vs[SMALL_SORT], cnt[16][256], lds4[4];
@@ -680,9 +680,9 @@ void launch_lookup(hipStream_t s, const T* table, uint64_t n_rows, uint64_t stri
 // ------------------------------------------------------------------------------------------------ norm
 // A row is held in registers, 8 * NC columns a lane, by L lanes: 16 to 64 up to 2048 columns (no barrier; 256 / L rows a block), four
 // waves up to 8192, sixteen beyond.  x is read once and everything written once: bound by HBM.  20001 x 1000 in fp16 with
-// residual 30 us (5.3 TB/s, part of it from the last-level cache); 262144 x 768 in bf16 with residual 265 us past the caches, 290
-// through them, 8000 x 4096 39 us through and 46 past.  Into 8 bits 262144 x 768 with residual 281 us, 5.0 TB/s, without 200:
-// there the arithmetic in 64 bits bounds it.
+// residual 29 us (5.5 TB/s, part of it from the last-level cache); 262144 x 768 in bf16 with residual 265 us past the caches, 290
+// through them, 8000 x 4096 39 us through and 46 past.  Into 8 bits 262144 x 768 with residual 266 us, 5.3 TB/s, without 172, into
+// e4m3 241: there the arithmetic in 64 bits bounds it.
 //
 // As in the lookup, a lane's eight columns never reach over the row's end: the last lane starts early enough and overlaps its
 // neighbour, and lanes behind it read the same eight and store nothing.  So no load stands behind a branch and all of a row's are
@@ -1044,8 +1044,10 @@ __global__ __launch_bounds__(1024) void weight_grad_kernel(const float* __restri
     }
 }
 
-// Picks NC, L and NARROW of a row kernel, whichever lanes stay idle least: body(NC, L, NARROW) as integral constants.  262144 x 768
-// in bf16 to int8 by 32 lanes with 24 columns each 200 us, by 64 with 16 258; 100000 x 100 by 16 lanes 16 us, by 64 52.
+// Picks NC, L and NARROW of a row kernel, 8 * NC * L columns: body(NC, L, NARROW) as integral constants.  Up to 2048 columns the lanes
+// that hold a row with the fewest idle: 262144 x 768 in bf16 to int8 by 32 lanes with 24 columns each 200 us, by 64 with 16 258;
+// 100000 x 100 by 16 lanes 16 us, by 64 52.  Beyond, for 4096 columns, 8192 and so on: up to half of the lanes are idle there, of which a
+// plain norm feels 6 % (24000 x 5120 in bf16 6.0 TB/s, x 8192 6.4).
 template <typename F>
 auto for_width(uint32_t dim, bool backward, F&& body) {
     auto pick = [&](auto nc, auto l) { return body(nc, l, std::false_type()); };
