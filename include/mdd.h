@@ -492,7 +492,7 @@ int mdd_embed_backward(mdd_ctx* ctx, const void* grad, int type, uint64_t grad_s
 /* Root-mean-square norm.  h = x + residual (residual may be NULL: h = x), r = 1 / sqrt(mean(h^2) + eps), weight [dim] of
  * x's type (NULL: ones).  dim <= MDD_VEC_MAX_DIM.
  *   (rows of any finite size, with eps = 0 too: where the squares leave the 32-bit numbers they are summed at a scale of the row's
- *   own.  rstd is a 32-bit number itself, infinite where mean(h^2) + eps is below 2^-256)
+ *   own; x + residual itself has to be a 32-bit number.  rstd is a 32-bit number itself, infinite where mean(h^2) + eps is below 2^-256)
  *   norm      y = h * r * weight;  sum_out (may be NULL) = h, rounded to the type;  rstd (may be NULL) = r, float per row
  *   norm_q8   the same with y in 8 bits (kind MDD_I8 or MDD_E4M3): with top = 127 or 448 and big = the row's largest
  *             |h * weight|, code = the nearest 8-bit value to h * weight * top / big, ties to even, decided without a rounding

@@ -135,6 +135,7 @@ def _near_pairs(be, vectors, min_cosine: float, margin: Optional[float] = None, 
     and each two of them as one matrix, of which the pairs across count (twice the products of a single search)."""
     if not 0.0 < float(min_cosine) <= 1.0:
         raise ValueError("min_cosine must be in (0, 1]")
+    be.mx_quantize(vectors[:0])                                  # refuses what is no matrix of vectors
     n = vectors.shape[0]
     if margin is None:
         margin = screen_margin(vectors, float(min_cosine))

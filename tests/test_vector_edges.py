@@ -9,6 +9,7 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from map_neo_amd import dedup as D  # noqa: E402
+from map_neo_amd.lib import MddError  # noqa: E402
 from map_neo_amd.vectors import TooManyPairs  # noqa: E402
 from test_vectors_path import VectorBackend  # noqa: E402
 
@@ -270,3 +271,34 @@ def test_too_many_pairs_says_how_many(engine):
     with pytest.raises(TooManyPairs, match="44850 pairs reach 0.5: more than max_pairs=1000") as e:
         engine.mx_pairs(m, 0.5, max_pairs=1000)
     assert (e.value.count, e.value.limit) == (44850, 1000)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [None, 3])
+def test_refusals_of_the_engine(engine, monkeypatch, rows):
+    """the same for one search and for more rows than one takes: before anything is measured or searched"""
+    if rows:
+        monkeypatch.setattr(D, "MAX_PAIR_ROWS", rows)
+    x = torch.randn(20, 16, device="cuda")
+    sig = torch.zeros(20, 128, dtype=torch.int32, device="cuda")
+    for bad, what in ((x.double(), "type torch.float64"), (x[0], "matrix"), (x[:, :0], "0 columns"), (x.t().contiguous().t(), "unit stride"), (x.cpu(), "tensor on"),
+                      (x.to(torch.int32), "type torch.int32"), (x.clone().requires_grad_(), "requires a gradient")):
+        with pytest.raises(MddError, match=what):
+            D.vector_edges(engine, bad, 0.9)
+        if bad.shape[0] == 20:
+            with pytest.raises(MddError, match=what):
+                D.cluster_local(engine, sig, vectors=bad, min_cosine=0.9)
+    assert D.vector_edges(engine, x[:1], 0.9)[0].numel() == 0 and D.vector_edges(engine, x[:, :1], 0.9)[0].numel() > 20
+
+
+@pytest.mark.gpu
+def test_many_pairs_of_narrow_vectors(engine):
+    """4 columns: (a - sin a cos a) / pi = 5.2 % of all pairs, a = acos(0.8), reach 0.8, 936000 of 18 million, far more candidates than rows; all pairs but those next to the threshold, in 64 bits"""
+    x = torch.randn(6000, 4, generator=torch.Generator().manual_seed(3)).half()
+    c, (u, v) = _true_cosines(x)
+    got = torch.zeros(6000, 6000, dtype=torch.bool)
+    eu, ev = D.vector_edges(engine, x.cuda(), 0.8)
+    got[eu.cpu().long(), ev.cpu().long()] = True
+    got = got.numpy()[u, v]
+    assert not got[c < 0.8 - 1e-9].any() and eu.numel() == got.sum() > 900000
+    assert (~got[c > 0.8 + 1e-9]).sum() <= (c > 0.8).sum() / 10 ** 5
